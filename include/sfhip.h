@@ -601,6 +601,51 @@ int sf_attn_bwd(const float* g, const float* dout, float* dg, const float* const
 int sf_token_outer4(const float* const* g, const float* const* a, float* const* out, const int* I,
                     const int* J, int n, void* stream);
 
+/* ---- layer norm ------------------------------------------------------------------------------ */
+/* LayerNorm over the last axis of [rows, D] (src/model/transformer_module.py:83-91 holds it inside
+ * nn.TransformerEncoderLayer; here for rows of any width up to SF_NORM_MAX_DIM, dtype f32 or bf16 for
+ * every void pointer, any element alignment): s = x, or x + residual rounded to dtype and written to
+ * `sum` (residual and sum are both NULL or both given); y = w (s - mean) / sqrt(var + eps) + b.  w, b f32
+ * [D], NULL = 1 / 0.  mean, rstd f32 [rows]: kept for the backward pass, both NULL in inference.
+ * The outputs must not overlap the inputs.
+ * Backward: dy, dsum (NULL = 0; the gradient arriving at `sum`), s (= sum, or x without a residual)
+ * -> dx (of x and of the residual alike); dw, db f32 [D], each NULL when not wanted, overwritten;
+ * ws: sf_layer_norm_bwd_workspace_bytes(rows, D, dtype) bytes when dw or db is given, any contents.
+ * Sums in f32, in a fixed order. */
+#define SF_NORM_MAX_DIM (1 << 24)
+int sf_layer_norm_fwd(const void* x, const void* residual, void* sum, const float* w, const float* b, void* y, float* mean,
+                      float* rstd, long long rows, int D, float eps, int dtype, void* stream);
+size_t sf_layer_norm_bwd_workspace_bytes(long long rows, int D, int dtype);
+int sf_layer_norm_bwd(const void* dy, const void* dsum, const void* s, const float* w, const float* mean, const float* rstd,
+                      void* dx, float* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int dtype,
+                      void* stream);
+
+/* ---- AdamW over many tensors -------------------------------------------------------------------- */
+/* One AdamW step (decoupled weight decay; the reference trains with Adam, src/train.py:80-91) of `count`
+ * tensors in as few launches as their pointers fit (40 tensors each).  All array arguments are HOST
+ * arrays of `count` entries, read during the call: p f32 parameters, g gradients (g_dtype[i] f32 or bf16),
+ * shadow_bf16 (NULL, or entries that may be NULL) copies of the updated parameters, n elements (0 allowed),
+ * lr, weight_decay, step_offset (NULL = 0; see sf_adam_guarded).  Any element alignment; no two
+ * tensors may overlap.
+ * state_bits 32: m, v f32, m_exp / v_exp unused.  state_bits 8: m, v one byte per element, m_exp / v_exp one
+ * byte per SF_ADAMW_BLOCK elements; the value of a code c under block exponent E is zero for c == 0 (first
+ * moment: c & 127 == 0), else the f32 with the bits ((c & 127) + 8 E - 120) << 20 and sign c >> 7 (first moment)
+ * or (c + 8 E - 248) << 20 (second moment).  Zeroed codes and exponents are zero moments.  Codes are rounded
+ * stochastically from a hash of (seed, steps taken, position in the list, element), so equal calls
+ * give equal results.
+ * state, found_inf: as in sf_adam_guarded, advanced by sf_adam_begin before the call.  A non-finite
+ * gradient spoils the moments of its whole block of 256 in the 8-bit form: pass found_inf.
+ * sf_adamw_moments: the values of 8-bit moments, exact in bf16. */
+#define SF_ADAMW_BLOCK 256
+int sf_adamw_step(int count, float* const* p, const void* const* g, void* const* m, void* const* v,
+                  unsigned char* const* m_exp, unsigned char* const* v_exp, void* const* shadow_bf16, const long long* n,
+                  const double* lr, const double* weight_decay, const int* g_dtype, const int* step_offset, int state_bits,
+                  double beta1, double beta2, float eps, float grad_scale, unsigned long long seed, const int* state,
+                  const int* found_inf, void* stream);
+int sf_adamw_moments(int count, const void* const* m, const void* const* v, const unsigned char* const* m_exp,
+                     const unsigned char* const* v_exp, void* const* m_bf16, void* const* v_bf16, const long long* n,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,340 @@
+// AdamW over many tensors in one launch, moments held in f32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Bound by HBM: 28 bytes per element with f32 gradients and moments, 16 with 8-bit moments, each touched
+// once.  The tensors' pointers travel as kernel arguments (no table in device memory to fill, so a launch
+// can be captured into a graph); a workgroup owns 4096 consecutive elements of one tensor and finds it
+// with one comparison per lane.
+//
+// 8-bit moments.  256 consecutive elements of a tensor share one exponent byte E, the f32 exponent of their
+// largest magnitude (one more when that lies above 1.875 times its power of two, so that rounding up never
+// leaves the range).  The codes are f32 bit patterns cut to three mantissa bits, counted from the top of the
+// block: bits = (code + 8 E - 120) << 20 for the first moment (a sign bit and 7 bits of magnitude: 15 binades
+// below the largest), bits = (code + 8 E - 248) << 20 for the second (8 bits: 31 binades); code 0 is zero.
+// Integer shifts alone convert, exactly, and every value is exact in bf16.  A moment moves by less than one
+// code per step (the second by a thousandth of its value), so rounding to nearest would hold it in place
+// for ever: codes are rounded stochastically, with 16 bits of an integer hash of (seed, step, tensor,
+// element), which keeps the moments unbiased and a run reproducible.  A second moment is never rounded to
+// zero (its square root divides).  The update of p uses the moments before they are rounded.
+#include "sf_common.h"
+#include "../../include/sfhip.h"
+
+namespace {
+
+constexpr int NT = 256;
+constexpr int CHUNK = 4096;        // elements of a workgroup: 16 per thread, four 16-byte pieces in flight per array
+constexpr int BLOCK = SF_ADAMW_BLOCK;
+constexpr int MAX_TENSORS = 40;    // tensors of one launch: their table stays below 4 KB of kernel arguments
+static_assert(BLOCK == 256 && CHUNK % (BLOCK * (NT / 64)) == 0, "one wave handles one block of moments per piece");
+
+struct Tensor {
+    float* p;
+    const void* g;
+    void* m;
+    void* v;
+    unsigned char* me;
+    unsigned char* ve;
+    bf16* shadow;
+    long long n;
+    float lr, keep;                // keep = 1 - lr * weight decay
+    int step_offset;
+    int ordinal;                   // position in the call's list (enters the hash)
+    int g_bf16;
+    int first;                     // first workgroup
+};
+struct Table { Tensor t[MAX_TENSORS]; };
+struct Hyper { double beta1, beta2; float eps, grad_scale; unsigned seed_lo, seed_hi; int count; };
+static_assert(sizeof(Table) + sizeof(Hyper) + 16 <= 4096, "kernel arguments");
+
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Four { T e[4]; };
+
+template <typename T> __device__ __forceinline__ Four<T> load4(const T* p, long long i, int have) {
+    Four<T> r{};
+    if (have == 4) {
+        r = *reinterpret_cast<const Four<T>*>(p + i);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < have) r.e[j] = p[i + j];
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, long long i, int have, const Four<T>& v) {
+    if (have == 4) {
+        *reinterpret_cast<Four<T>*>(p + i) = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (j < have) p[i + j] = v.e[j];
+    }
+}
+
+// b^t by squaring (t >= 1)
+__device__ __forceinline__ double power(double b, int t) {
+    double r = 1.0;
+    for (; t > 0; t >>= 1) {
+        if (t & 1) r *= b;
+        b *= b;
+    }
+    return r;
+}
+
+__host__ __device__ __forceinline__ unsigned mix(unsigned x) {
+    x ^= x >> 16;
+    x *= 0x6A09E667u;
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+
+__device__ __forceinline__ unsigned wave_max_u(unsigned v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const unsigned u = (unsigned)__shfl_xor((int)v, o, 64);
+        v = v > u ? v : u;
+    }
+    return v;
+}
+
+// f32 value of a code under block exponent e; SIGNED: first moment
+template <bool SIGNED> __device__ __forceinline__ float decode(unsigned c, int e) {
+    const unsigned low = SIGNED ? c & 127u : c;
+    const unsigned bits = (low + 8u * (unsigned)e - (SIGNED ? 120u : 248u)) << 20;
+    return low ? __uint_as_float(SIGNED ? bits | ((c & 128u) << 24) : bits) : 0.f;
+}
+// block exponent for the largest magnitude (as f32 bits); the lower bound keeps every code a normal f32
+template <bool SIGNED> __device__ __forceinline__ int block_exponent(unsigned largest) {
+    const unsigned e = (largest + 0xFFFFFu) >> 23;
+    const unsigned least = SIGNED ? 16u : 32u;
+    return (int)(e < least ? least : e > 255u ? 255u : e);
+}
+// code of x under block exponent e, rounded up with probability (distance to the code below) / (code spacing)
+template <bool SIGNED> __device__ __forceinline__ unsigned encode(float x, int e, unsigned r16) {
+    const unsigned bits = __float_as_uint(x) & 0x7FFFFFFFu;
+    const unsigned base = 8u * (unsigned)e - (SIGNED ? 120u : 248u);
+    const unsigned top = SIGNED ? 127u : 255u;
+    const unsigned least = (base + 1u) << 20;
+    unsigned c = ((bits + (r16 << 4)) >> 20) - base;
+    c = c > top ? top : c;
+    if (bits < least) {
+        if (SIGNED) c = __uint_as_float(bits) > (float)r16 * (1.f / 65536.f) * __uint_as_float(least) ? 1u : 0u;
+        else c = bits ? 1u : 0u;
+    }
+    return SIGNED ? c | ((__float_as_uint(x) >> 31) << 7) : c;
+}
+
+// the tensor that workgroup `bid` works on: lanes compare, the last first <= bid wins
+__device__ __forceinline__ int tensor_of(const Table& tab, int count, int bid) {
+    const int lane = threadIdx.x & 63;
+    const bool before = lane < count && tab.t[lane < count ? lane : 0].first <= bid;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
+}
+
+template <int BITS>
+__global__ __launch_bounds__(NT) void adamw_kernel(Table tab, Hyper h, const int* __restrict__ state,
+                                                   const int* __restrict__ found_inf) {
+    if (found_inf && found_inf[0] != 0) return;
+    const Tensor& T = tab.t[tensor_of(tab, h.count, blockIdx.x)];
+    const long long n = T.n, c0 = (long long)(blockIdx.x - T.first) * CHUNK;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    constexpr int U = CHUNK / (4 * NT);
+    const int t_all = state[0], t = max(t_all + T.step_offset, 1);
+    const float b1 = (float)h.beta1, b2 = (float)h.beta2, a1 = (float)(1.0 - h.beta1), a2 = (float)(1.0 - h.beta2);
+    long long at[U];
+    int have[U];
+    Four<float> p[U], m[U], v[U];
+    Four<float> g[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        at[u] = c0 + u * (4 * NT) + wave * BLOCK + lane * 4;
+        const long long left = n - at[u];
+        have[u] = left >= 4 ? 4 : left > 0 ? (int)left : 0;
+    }
+    if (T.g_bf16) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const Four<bf16> r = load4((const bf16*)T.g, at[u], have[u]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) g[u].e[j] = (float)r.e[j];
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) g[u] = load4((const float*)T.g, at[u], have[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) p[u] = load4(T.p, at[u], have[u]);
+    if constexpr (BITS == 32) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            m[u] = load4((const float*)T.m, at[u], have[u]);
+            v[u] = load4((const float*)T.v, at[u], have[u]);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const Four<unsigned char> cm = load4((const unsigned char*)T.m, at[u], have[u]);
+            const Four<unsigned char> cv = load4((const unsigned char*)T.v, at[u], have[u]);
+            const int em = have[u] ? T.me[at[u] / BLOCK] : 16, ev = have[u] ? T.ve[at[u] / BLOCK] : 32;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m[u].e[j] = decode<true>(cm.e[j], em);
+                v[u].e[j] = decode<false>(cv.e[j], ev);
+            }
+        }
+    }
+    const float step = (float)((double)T.lr / (1.0 - power(h.beta1, t)));
+    const float root = (float)(1.0 / sqrt(1.0 - power(h.beta2, t)));
+    const float keep = T.keep;
+    unsigned key = 0;
+    if constexpr (BITS == 8) key = mix(mix((h.seed_lo + (unsigned)t_all * 0x9E3779B1u) ^ h.seed_hi) + (unsigned)T.ordinal * 0x85EBCA6Bu);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float gs = g[u].e[j] * h.grad_scale;
+            m[u].e[j] = b1 * m[u].e[j] + a1 * gs;
+            v[u].e[j] = b2 * v[u].e[j] + a2 * gs * gs;
+            p[u].e[j] = p[u].e[j] * keep - step * (m[u].e[j] / (sqrtf(v[u].e[j]) * root + h.eps));
+        }
+        store4(T.p, at[u], have[u], p[u]);
+        if (T.shadow) {
+            Four<bf16> s;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s.e[j] = (bf16)p[u].e[j];
+            store4(T.shadow, at[u], have[u], s);
+        }
+        if constexpr (BITS == 32) {
+            store4((float*)T.m, at[u], have[u], m[u]);
+            store4((float*)T.v, at[u], have[u], v[u]);
+        } else {
+            // elements behind the tensor's end hold zero here (nothing was loaded) and take no part
+            unsigned mm = 0, mv = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned bm = __float_as_uint(m[u].e[j]) & 0x7FFFFFFFu, bv = __float_as_uint(v[u].e[j]) & 0x7FFFFFFFu;
+                mm = mm > bm ? mm : bm;
+                mv = mv > bv ? mv : bv;
+            }
+            const int em = block_exponent<true>(wave_max_u(mm)), ev = block_exponent<false>(wave_max_u(mv));
+            Four<unsigned char> cm, cv;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned long long i = (unsigned long long)at[u] + j;
+                const unsigned r = mix((unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0xC2B2AE35u + key);
+                cm.e[j] = (unsigned char)encode<true>(m[u].e[j], em, r >> 16);
+                cv.e[j] = (unsigned char)encode<false>(v[u].e[j], ev, r & 0xFFFFu);
+            }
+            store4((unsigned char*)T.m, at[u], have[u], cm);
+            store4((unsigned char*)T.v, at[u], have[u], cv);
+            if (lane == 0 && have[u]) {
+                T.me[at[u] / BLOCK] = (unsigned char)em;
+                T.ve[at[u] / BLOCK] = (unsigned char)ev;
+            }
+        }
+    }
+}
+
+// bf16 values of 8-bit moments (exact); T.p is unused, T.g / T.shadow hold the two outputs
+__global__ __launch_bounds__(NT) void adamw_moments_kernel(Table tab, int count) {
+    const Tensor& T = tab.t[tensor_of(tab, count, blockIdx.x)];
+    const long long n = T.n, c0 = (long long)(blockIdx.x - T.first) * CHUNK;
+    constexpr int U = CHUNK / (4 * NT);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long at = c0 + u * (4 * NT) + threadIdx.x * 4, left = n - at;
+        const int have = left >= 4 ? 4 : left > 0 ? (int)left : 0;
+        if (!have) continue;
+        const Four<unsigned char> cm = load4((const unsigned char*)T.m, at, have);
+        const Four<unsigned char> cv = load4((const unsigned char*)T.v, at, have);
+        const int em = T.me[at / BLOCK], ev = T.ve[at / BLOCK];
+        Four<bf16> m, v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m.e[j] = (bf16)decode<true>(cm.e[j], em);
+            v.e[j] = (bf16)decode<false>(cv.e[j], ev);
+        }
+        store4((bf16*)T.p, at, have, m);
+        store4(T.shadow, at, have, v);
+    }
+}
+
+// splits the list into launches of at most MAX_TENSORS non-empty tensors and 2^30 workgroups
+template <typename F, typename L> int over_tensors(int count, const long long* n, F&& fill, L&& launch) {
+    Table tab;
+    int used = 0;
+    long long groups = 0;
+    for (int i = 0; i <= count; ++i) {
+        const long long need = i < count ? (n[i] + CHUNK - 1) / CHUNK : 0;
+        if (used && (i == count || used == MAX_TENSORS || groups + need > (1LL << 30))) {
+            launch(tab, used, (int)groups);
+            used = 0;
+            groups = 0;
+        }
+        if (i < count && n[i] > 0) {
+            fill(tab.t[used], i);
+            tab.t[used].first = (int)groups;
+            groups += need;
+            ++used;
+        }
+    }
+    return SF_OK;
+}
+
+}  // namespace
+
+extern "C" int sf_adamw_step(int count, float* const* p, const void* const* g, void* const* m, void* const* v,
+                             unsigned char* const* m_exp, unsigned char* const* v_exp, void* const* shadow_bf16,
+                             const long long* n, const double* lr, const double* weight_decay, const int* g_dtype,
+                             const int* step_offset, int state_bits, double beta1, double beta2, float eps, float grad_scale,
+                             unsigned long long seed, const int* state, const int* found_inf, void* stream) {
+    SF_REQUIRE(count >= 0 && p && g && m && v && n && lr && weight_decay && g_dtype && state, "sf_adamw_step: null argument");
+    SF_REQUIRE(state_bits == 32 || state_bits == 8, "sf_adamw_step: moments are held in 32 or 8 bits, not %d", state_bits);
+    SF_REQUIRE(state_bits == 32 || (m_exp && v_exp), "sf_adamw_step: 8-bit moments need their block exponents");
+    SF_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "sf_adamw_step: betas must lie in [0, 1)");
+    SF_REQUIRE(eps >= 0.f, "sf_adamw_step: eps must not be negative");
+    for (int i = 0; i < count; ++i) {
+        SF_REQUIRE(n[i] >= 0 && n[i] <= (1LL << 41), "sf_adamw_step: tensor %d has %lld elements", i, n[i]);
+        SF_REQUIRE(n[i] == 0 || (p[i] && g[i] && m[i] && v[i]), "sf_adamw_step: tensor %d has a null pointer", i);
+        SF_REQUIRE(n[i] == 0 || state_bits == 32 || (m_exp[i] && v_exp[i]), "sf_adamw_step: tensor %d lacks its exponents", i);
+        SF_REQUIRE(g_dtype[i] == SF_F32 || g_dtype[i] == SF_BF16, "sf_adamw_step: tensor %d has gradient dtype %d", i, g_dtype[i]);
+        SF_REQUIRE(!step_offset || step_offset[i] <= 0, "sf_adamw_step: step offsets are not positive");
+    }
+    Hyper h{beta1, beta2, eps, grad_scale, (unsigned)seed, (unsigned)(seed >> 32), 0};
+    auto fill = [&](Tensor& t, int i) {
+        t = Tensor{p[i], g[i], m[i], v[i], state_bits == 8 ? m_exp[i] : nullptr, state_bits == 8 ? v_exp[i] : nullptr,
+                   shadow_bf16 ? (bf16*)shadow_bf16[i] : nullptr, n[i], (float)lr[i], (float)(1.0 - lr[i] * weight_decay[i]),
+                   step_offset ? step_offset[i] : 0, i, g_dtype[i] == SF_BF16, 0};
+    };
+    auto launch = [&](const Table& tab, int used, int groups) {
+        h.count = used;
+        if (state_bits == 32)
+            hipLaunchKernelGGL((adamw_kernel<32>), dim3(groups), dim3(NT), 0, (hipStream_t)stream, tab, h, state, found_inf);
+        else
+            hipLaunchKernelGGL((adamw_kernel<8>), dim3(groups), dim3(NT), 0, (hipStream_t)stream, tab, h, state, found_inf);
+    };
+    over_tensors(count, n, fill, launch);
+    SF_LAUNCH_CHECK("sf_adamw_step");
+    return SF_OK;
+}
+
+extern "C" int sf_adamw_moments(int count, const void* const* m, const void* const* v, const unsigned char* const* m_exp,
+                                const unsigned char* const* v_exp, void* const* m_bf16, void* const* v_bf16,
+                                const long long* n, void* stream) {
+    SF_REQUIRE(count >= 0 && m && v && m_exp && v_exp && m_bf16 && v_bf16 && n, "sf_adamw_moments: null argument");
+    for (int i = 0; i < count; ++i) {
+        SF_REQUIRE(n[i] >= 0 && n[i] <= (1LL << 41), "sf_adamw_moments: tensor %d has %lld elements", i, n[i]);
+        SF_REQUIRE(n[i] == 0 || (m[i] && v[i] && m_exp[i] && v_exp[i] && m_bf16[i] && v_bf16[i]),
+                   "sf_adamw_moments: tensor %d has a null pointer", i);
+    }
+    auto fill = [&](Tensor& t, int i) {
+        t = Tensor{(float*)m_bf16[i], nullptr, (void*)m[i], (void*)v[i], (unsigned char*)m_exp[i], (unsigned char*)v_exp[i],
+                   (bf16*)v_bf16[i], n[i], 0.f, 0.f, 0, i, 0, 0};
+    };
+    auto launch = [&](const Table& tab, int used, int groups) {
+        hipLaunchKernelGGL(adamw_moments_kernel, dim3(groups), dim3(NT), 0, (hipStream_t)stream, tab, used);
+    };
+    over_tensors(count, n, fill, launch);
+    SF_LAUNCH_CHECK("sf_adamw_moments");
+    return SF_OK;
+}

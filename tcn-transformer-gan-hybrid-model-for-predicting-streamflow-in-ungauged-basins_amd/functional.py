@@ -817,3 +817,82 @@ class BceLogitsFn(torch.autograd.Function):
         dx = ctx.dx
         ctx.dx = None
         return (dx * g).reshape(ctx.shape), None, None
+
+
+# ------------------------------------------------------------------------------ layer norm
+class LayerNormFn(torch.autograd.Function):
+    """LayerNorm over the last axis, with the residual add in front of it when one is given."""
+
+    @staticmethod
+    def forward(ctx, x, residual, w, b, eps):
+        need = any(ctx.needs_input_grad[:4])
+        y, s, mean, rstd = ops.layer_norm_fwd(x, w, b, eps, residual, need)
+        if need:
+            ctx.save_for_backward(s, w, mean, rstd)
+        ctx.has_residual = residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, s) if residual is not None else y
+
+    @staticmethod
+    def backward(ctx, dy, ds=None):
+        s, w, mean, rstd = ctx.saved_tensors
+        if dy is None:              # only the sum was used
+            return ds, ds, None, None, None
+        dx, dw, db = ops.layer_norm_bwd(dy.contiguous(), None if ds is None else ds.contiguous(), s, w, mean, rstd,
+                                        ctx.needs_input_grad[2], ctx.needs_input_grad[3])
+        return dx, dx if ctx.has_residual else None, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float = 1e-5,
+               residual: Optional[torch.Tensor] = None):
+    """y = weight * (s - mean(s)) / sqrt(var(s) + eps) + bias over the last axis, for f32 or bf16 x of any
+    leading shape (statistics in f32); weight and bias [D] or None.  Without a residual s = x and the result is y; with
+    one, s = x + residual, rounded to x's dtype as the next layer will read it, and the result is
+    (y, s).  Differentiable in all four; the gradient of x is also that of the residual."""
+    if not x.is_cuda:
+        raise RuntimeError("layer_norm: GPU tensors only (no CPU path exists)")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"layer_norm: f32 or bf16 rows, not {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise RuntimeError(f"layer_norm: no axis to normalise in shape {tuple(x.shape)}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise RuntimeError(f"layer_norm: residual {tuple(residual.shape)} {residual.dtype} on {residual.device} does not match "
+                           f"x {tuple(x.shape)} {x.dtype} on {x.device}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (tuple(t.shape) != (x.shape[-1],) or t.device != x.device):
+            raise RuntimeError(f"layer_norm: {name} {tuple(t.shape)} on {t.device} for rows of {x.shape[-1]} on {x.device}")
+    w, b = (None if t is None else t.float().contiguous() for t in (weight, bias))
+    with torch.cuda.device(x.device):
+        return LayerNormFn.apply(x.contiguous(), None if residual is None else residual.contiguous(), w, b, float(eps))
+
+
+# ------------------------------------------------------------------------------ AdamW
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs, exp_avg_sqs, state: torch.Tensor, lr,
+               betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, seed: int = 0,
+               found_inf: Optional[torch.Tensor] = None, grad_scale: float = 1.0, shadows=None, step_offsets=None):
+    """One AdamW step of many tensors in place: f32 parameters, f32 or bf16 gradients, moments either f32
+    tensors or pairs (codes uint8 [n], block exponents uint8 [ceil(n / 256)]) of 8-bit state (zeros
+    to begin with).  state: int32 [2] on the device, steps taken and steps skipped, zeros to begin with; a
+    step whose found_inf[0] is not zero changes nothing but the second count.  lr and weight_decay: one
+    number, or one per tensor.  seed: of the stochastic rounding of 8-bit moments.  shadows: bf16 copies
+    of the parameters to refresh (entries may be None).  The parameters are written behind torch's
+    back: copies the package derives from them (packed weights, shadows) are marked stale here."""
+    if not state.is_cuda:
+        raise RuntimeError("adamw_step: GPU tensors only (no CPU path exists)")
+    with torch.no_grad(), torch.cuda.device(state.device):
+        ops.adamw_step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), state, lr, betas[0], betas[1], eps,
+                       weight_decay, seed, found_inf, grad_scale, shadows, step_offsets)
+        ops.touch(params)
+
+
+def adamw_moments(exp_avgs, exp_avg_sqs, out=None):
+    """The values that 8-bit moments stand for, as (first moments, second moments): two lists of bf16
+    tensors, in which every value is exact.  out: the two lists to write to."""
+    if out is None:
+        out = tuple([torch.empty(c.shape, device=c.device, dtype=torch.bfloat16) for c, _ in x] for x in (exp_avgs, exp_avg_sqs))
+    if out[0]:
+        if not out[0][0].is_cuda:
+            raise RuntimeError("adamw_moments: GPU tensors only (no CPU path exists)")
+        with torch.cuda.device(out[0][0].device):
+            ops.adamw_moments(list(exp_avgs), list(exp_avg_sqs), list(out[0]), list(out[1]))
+    return out

@@ -202,6 +202,30 @@ class LSTMModule(nn.Module):
         return self.output_dim
 
 
+class LayerNorm(nn.Module):
+    """nn.LayerNorm's constructor for one axis, attributes and state_dict keys (the reference holds it inside
+    nn.TransformerEncoderLayer, src/model/transformer_module.py:83-91), for rows of any width and
+    number.  Called with a second tensor it normalises x + residual and returns (y, x + residual).
+    Inside torch.autocast('cuda') rows are taken in bf16 (statistics and weights stay f32)."""
+
+    def __init__(self, normalized_shape: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True):
+        super().__init__()
+        shape = tuple(normalized_shape) if isinstance(normalized_shape, (tuple, list)) else (int(normalized_shape),)
+        if len(shape) != 1:
+            raise NotImplementedError("LayerNorm over the last axis only")
+        self.normalized_shape, self.eps, self.elementwise_affine = shape, eps, elementwise_affine
+        self.weight = nn.Parameter(torch.ones(shape)) if elementwise_affine else None
+        self.bias = nn.Parameter(torch.zeros(shape)) if elementwise_affine and bias else None
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        _need_cuda(x, "LayerNorm")
+        if x.shape[-1:] != self.normalized_shape:
+            raise RuntimeError(f"LayerNorm over {self.normalized_shape[0]} values got rows of shape {tuple(x.shape)}")
+        if SF.compute_dtype() == torch.bfloat16:
+            x = x.to(torch.bfloat16)
+        return SF.layer_norm(x, self.weight, self.bias, self.eps, None if residual is None else residual.to(x.dtype))
+
+
 # ------------------------------------------------------------------------------ decoder
 class SimpleUpsamplingDecoder(nn.Module):
     """Mirror of src/model/decoder.py:125-177."""

@@ -68,6 +68,7 @@ def lib():
         L.sf_date_image_metrics_workspace_bytes.restype = ctypes.c_size_t
         L.sf_gru_save_floats.restype = ctypes.c_size_t
         L.sf_attn_save_floats.restype = ctypes.c_size_t
+        L.sf_layer_norm_bwd_workspace_bytes.restype = ctypes.c_size_t
         _lib = L
     return _lib
 
@@ -82,7 +83,8 @@ EXPORTS = ["sf_version", "sf_last_error", "sf_gemm", "sf_gemm_batch", "sf_conv3x
            "sf_bce_logits", "sf_adam", "sf_adam_begin", "sf_adam_guarded", "sf_nan_inf_flag", "sf_dataset_plane_stats", "sf_dataset_transform",
            "sf_gather_frames", "sf_date_image_metrics", "sf_date_image_metrics_workspace_bytes", "sf_bn_relu_fwd",
            "sf_relu_dropout_fwd", "sf_relu_dropout_bwd", "sf_gru_save_floats", "sf_gru_fwd", "sf_gru_bwd",
-           "sf_attn_save_floats", "sf_attn_fwd", "sf_attn_bwd", "sf_token_outer4"]
+           "sf_attn_save_floats", "sf_attn_fwd", "sf_attn_bwd", "sf_token_outer4",
+           "sf_layer_norm_fwd", "sf_layer_norm_bwd", "sf_layer_norm_bwd_workspace_bytes", "sf_adamw_step", "sf_adamw_moments"]
 
 
 def _check(rc: int, who: str):
@@ -1075,6 +1077,40 @@ def attn_bwd(g, dout, ws, dws, save):
     return dg
 
 
+# ------------------------------------------------------------------------------ layer norm
+def layer_norm_fwd(x, w, b, eps, residual=None, need_stats=False):
+    """x [..., D] f32 / bf16, w, b f32 [D] or None -> (y, s, mean, rstd): s is x, or x + residual in x's
+    dtype; the statistics are None unless wanted."""
+    _dev(x, residual, w, b, dtypes=[None, x.dtype, torch.float32, torch.float32])
+    code, D = code_of(x.dtype), x.shape[-1]
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError(f"layer_norm: residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    rows = x.numel() // D
+    y = torch.empty_like(x)
+    s = torch.empty_like(x) if residual is not None else x
+    mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0) if need_stats else (None, None)
+    if rows:
+        _check(lib().sf_layer_norm_fwd(_p(x), _p(residual), _p(s if residual is not None else None), _p(w), _p(b), _p(y), _p(mean),
+                                       _p(rstd), _c_ll(rows), D, _c_f(eps), code, _stream()), "sf_layer_norm_fwd")
+    return y, s, mean, rstd
+
+
+def layer_norm_bwd(dy, dsum, s, w, mean, rstd, need_dw=True, need_db=True):
+    """(dx, dw, db); dsum: the gradient arriving at the sum, or None."""
+    _dev(dy, dsum, s, w, mean, rstd, dtypes=[s.dtype, s.dtype, None, torch.float32, torch.float32, torch.float32])
+    D = s.shape[-1]
+    rows, code = s.numel() // D, code_of(s.dtype)
+    dx = torch.empty_like(s)
+    dw, db = ((torch.empty if rows else torch.zeros)(D, device=s.device, dtype=torch.float32) if want else None
+              for want in (need_dw, need_db))
+    if rows:
+        nb = int(lib().sf_layer_norm_bwd_workspace_bytes(_c_ll(rows), D, code)) if need_dw or need_db else 0
+        ws = torch.empty(nb, device=s.device, dtype=torch.uint8) if nb else None
+        _check(lib().sf_layer_norm_bwd(_p(dy), _p(dsum), _p(s), _p(w), _p(mean), _p(rstd), _p(dx), _p(dw), _p(db), _p(ws),
+                                       ctypes.c_size_t(nb), _c_ll(rows), D, code, _stream()), "sf_layer_norm_bwd")
+    return dx, dw, db
+
+
 # ------------------------------------------------------------------------------ losses / optimiser
 def lonlat_to_pixel(lon: torch.Tensor, lat: torch.Tensor, region, W: int, H: int):
     _dev(lon, lat, dtypes=[torch.float64, torch.float64])
@@ -1206,6 +1242,97 @@ def adam_guarded(p, g, m, v, lr, beta1, beta2, eps, state, found_inf=None, grad_
     _check(lib().sf_adam_guarded(_p(p), _p(g), _p(m), _p(v), _p(shadow), _c_ll(p.numel()), _c_f(lr), ctypes.c_double(beta1),
                                  ctypes.c_double(beta2), _c_f(eps), _c_f(grad_scale), _p(state), _p(found_inf),
                                  int(step_offset), _stream()), "sf_adam_guarded")
+
+
+ADAMW_BLOCK = 256   # SF_ADAMW_BLOCK: elements that share a block exponent in 8-bit moments
+
+
+def _adamw_moment_lists(ms, vs, numels, who):
+    """(state bits, moment tensors, exponent tensors or None) of lists of f32 tensors or (codes, exponents) pairs."""
+    bits8 = len(ms) > 0 and isinstance(ms[0], (tuple, list))
+    for x, n in zip(list(ms) + list(vs), list(numels) * 2):
+        if isinstance(x, (tuple, list)) != bits8:
+            raise TypeError(f"{who}: f32 and 8-bit moments cannot be mixed in one call")
+        if bits8:
+            _dev(*x, dtypes=[torch.uint8, torch.uint8])
+            if x[0].numel() != n or x[1].numel() != -(-n // ADAMW_BLOCK):
+                raise RuntimeError(f"{who}: {n} elements need {n} codes and {-(-n // ADAMW_BLOCK)} block exponents, "
+                                   f"got {x[0].numel()} and {x[1].numel()}")
+        else:
+            _dev(x, dtypes=[torch.float32])
+            if x.numel() != n:
+                raise RuntimeError(f"{who}: a moment of {x.numel()} elements for a parameter of {n}")
+    if not bits8:
+        return 32, ms, vs, None, None
+    return 8, [x[0] for x in ms], [x[0] for x in vs], [x[1] for x in ms], [x[1] for x in vs]
+
+
+def adamw_step(ps, gs, ms, vs, state, lr, beta1, beta2, eps, weight_decay, seed=0, found_inf=None, grad_scale=1.0, shadows=None,
+               step_offsets=None):
+    """One AdamW update of the tensors `ps`: the checks, then sf_adam_begin, then sf_adamw_step.  lr and
+    weight_decay: one number, or one per tensor."""
+    n = len(ps)
+    for name, seq in (("gradients", gs), ("first moments", ms), ("second moments", vs), ("shadows", shadows),
+                      ("step offsets", step_offsets), ("lr", lr if isinstance(lr, (list, tuple)) else None),
+                      ("weight_decay", weight_decay if isinstance(weight_decay, (list, tuple)) else None)):
+        if seq is not None and len(seq) != n:
+            raise RuntimeError(f"adamw_step: {len(seq)} {name} for {n} parameters")
+    _dev(state, found_inf, dtypes=[torch.int32, torch.int32])
+    if state.numel() != 2:
+        raise RuntimeError("adamw_step: state is int32 [2]: steps taken, steps skipped")
+    _dev(*ps, dtypes=[torch.float32] * n)
+    _dev(*gs)
+    codes = [code_of(g.dtype) for g in gs]
+    dev = state.device
+    for i, (p, g) in enumerate(zip(ps, gs)):
+        if g.numel() != p.numel():
+            raise RuntimeError(f"adamw_step: gradient {i} has {g.numel()} elements, its parameter {p.numel()}")
+        if p.device != dev or g.device != dev:
+            raise RuntimeError(f"adamw_step: tensor {i} is on {p.device} / {g.device}, the state on {dev}")
+    numels = [p.numel() for p in ps]
+    if len({p.data_ptr() for p in ps if p.numel()}) != sum(1 for k in numels if k):
+        raise RuntimeError("adamw_step: the same parameter is listed twice")
+    if shadows is not None:
+        for i, s in enumerate(shadows):
+            _dev(s, dtypes=[torch.bfloat16])
+            if s is not None and s.numel() != numels[i]:
+                raise RuntimeError(f"adamw_step: shadow {i} has {s.numel()} elements, its parameter {numels[i]}")
+    bits, ms, vs, me, ve = _adamw_moment_lists(ms, vs, numels, "adamw_step")
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and eps >= 0.0):
+        raise ValueError(f"adamw_step: betas ({beta1}, {beta2}) must lie in [0, 1), eps ({eps}) must not be negative")
+    if step_offsets is not None and any(o > 0 for o in step_offsets):
+        raise ValueError("adamw_step: step offsets are not positive")
+    adam_begin(state, found_inf)
+    if n == 0:
+        return
+    lrs = lr if isinstance(lr, (list, tuple)) else [lr] * n
+    wds = weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+    sh = None if shadows is None else (_c_vp * n)(*[None if s is None else s.data_ptr() for s in shadows])
+    _check(lib().sf_adamw_step(n, _ptr_array(ps), _ptr_array(gs), _ptr_array(ms), _ptr_array(vs),
+                               None if me is None else _ptr_array(me), None if ve is None else _ptr_array(ve), sh,
+                               (_c_ll * n)(*numels), (_c_d * n)(*lrs), (_c_d * n)(*wds),
+                               (_c_int * n)(*codes),
+                               None if step_offsets is None else (_c_int * n)(*step_offsets), bits, _c_d(beta1), _c_d(beta2),
+                               _c_f(eps), _c_f(grad_scale), ctypes.c_ulonglong(seed), _p(state), _p(found_inf), _stream()),
+           "sf_adamw_step")
+
+
+def adamw_moments(ms, vs, outs_m, outs_v):
+    """The values of 8-bit moments (lists of (codes, exponents)) into bf16 tensors of the same sizes; exact."""
+    n = len(ms)
+    if not (len(vs) == len(outs_m) == len(outs_v) == n):
+        raise RuntimeError("adamw_moments: lists of different lengths")
+    numels = [o.numel() for o in outs_m]
+    _dev(*outs_m, *outs_v, dtypes=[torch.bfloat16] * (2 * n))
+    if [o.numel() for o in outs_v] != numels:
+        raise RuntimeError("adamw_moments: outputs of different sizes")
+    if n == 0:
+        return
+    bits, ms, vs, me, ve = _adamw_moment_lists(ms, vs, numels, "adamw_moments")
+    if bits != 8:
+        raise TypeError("adamw_moments: f32 moments are their own values")
+    _check(lib().sf_adamw_moments(n, _ptr_array(ms), _ptr_array(vs), _ptr_array(me), _ptr_array(ve), _ptr_array(outs_m),
+                                  _ptr_array(outs_v), (_c_ll * n)(*numels), _stream()), "sf_adamw_moments")
 
 
 def nan_inf_flag(x: torch.Tensor, flag: torch.Tensor):
