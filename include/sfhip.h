@@ -620,6 +620,32 @@ int sf_layer_norm_bwd(const void* dy, const void* dsum, const void* s, const flo
                       void* dx, float* dw, float* db, void* ws, size_t ws_bytes, long long rows, int D, int dtype,
                       void* stream);
 
+/* ---- differential attention ----------------------------------------------------------------------- */
+/* o = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v per head, for any number of tokens (the reference
+ * attends over the window's few days inside nn.TransformerEncoderLayer, src/model/transformer_module.py:81-93).
+ * q [B,Tq,H,2,d], k [B,Tk,Hk,2,d], v [B,Tk,Hk,2d] with d and the halves contiguous and the given strides (elements:
+ * sample, token, head; multiples of 16 bytes, token stride at least 2 d and below 2^22); H a multiple of Hk (query
+ * head h reads key / value head h / (H / Hk)); d <= 64 a multiple of 8; dtype f32 or bf16; lam [H], lam_dtype f32 or bf16;
+ * scale > 0.  lengths: int32 [B] on the device, keys of each sample (clamped to [0, Tk]), or NULL; keys from
+ * there on are not read.  causal: query t sees keys up to t + Tk - Tq.  A query that sees no key gets zeros and has
+ * no gradient.  All pointers 16-byte aligned; o, o2, do, dq [B,Tq,H,2d] and dk, dv [B,Tk,Hk,2d] contiguous.
+ * Forward: o2 and lse f32 [B,H,Tq,2] are kept for the backward pass (both NULL in inference); ws:
+ * sf_diff_attn_fwd_workspace_bytes(desc) bytes (may be 0), any contents.  Backward: dlam [H] of lam's type, or NULL;
+ * every output is overwritten; ws: sf_diff_attn_bwd_workspace_bytes(desc) bytes.  No atomics: equal calls give equal
+ * results.  The workspace size functions return 0 for a descriptor that the call itself refuses. */
+typedef struct sf_diff_attn_desc {
+    int dtype, lam_dtype, B, Tq, Tk, H, Hk, d, causal;
+    float scale;
+    long long q_stride[3], k_stride[3], v_stride[3];
+} sf_diff_attn_desc;
+size_t sf_diff_attn_fwd_workspace_bytes(const sf_diff_attn_desc* desc);
+int sf_diff_attn_fwd(const sf_diff_attn_desc* desc, const void* q, const void* k, const void* v, const void* lam,
+                     const int* lengths, void* o, void* o2, float* lse, void* ws, size_t ws_bytes, void* stream);
+size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* desc);
+int sf_diff_attn_bwd(const sf_diff_attn_desc* desc, const void* q, const void* k, const void* v, const void* lam,
+                     const int* lengths, const void* o, const void* o2, const float* lse, const void* dout, void* dq,
+                     void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- AdamW over many tensors -------------------------------------------------------------------- */
 /* One AdamW step (decoupled weight decay; the reference trains with Adam, src/train.py:80-91) of `count`
  * tensors in as few launches as their pointers fit (40 tensors each).  All array arguments are HOST

@@ -866,6 +866,69 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
         return LayerNormFn.apply(x.contiguous(), None if residual is None else residual.contiguous(), w, b, float(eps))
 
 
+# ------------------------------------------------------------------------------ differential attention
+class DiffAttentionFn(torch.autograd.Function):
+    """(softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v, see diff_attention."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lam, lengths, causal, scale):
+        need = any(ctx.needs_input_grad[:4])
+        o, o2, lse = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need)
+        if need:
+            ctx.save_for_backward(q, k, v, lam, lengths, o, o2, lse)
+        ctx.cfg = (causal, scale)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, lam, lengths, o, o2, lse = ctx.saved_tensors
+        if o.numel() == 0 or k.numel() == 0:
+            return (*(torch.zeros(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, lam)), None, None, None)
+        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, *ctx.cfg, o, o2, lse, do.contiguous(), ctx.needs_input_grad[3])
+        return (*grads, None, None, None)
+
+
+def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, causal: bool = False,
+                   scale: Optional[float] = None, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Differential attention, o = (softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v per head.
+
+    q [B, Tq, H, 2, d] and k [B, Tk, Hk, 2, d] hold the two maps' halves of each head, v [B, Tk, Hk, 2d], lam [H] the learned
+    weight of the second map; f32 or bf16 (lam either), d a multiple of 8 up to 64, H a multiple of Hk (H / Hk
+    query heads share a key / value head).  scale defaults to 1 / sqrt(d).  causal: query t sees keys up to t + Tk - Tq, so that
+    the last query sees the last key.  lengths: int32 [B] on the device, the keys each sample has (the values
+    are clamped to [0, Tk]; what lies behind them is never read).  A query that sees no key gives zeros.
+    Sums and softmax statistics are f32; in bf16 the probabilities are rounded once for the second product.
+    Differentiable in q, k, v and lam; no atomics: equal inputs give equal bits.  Slices of one projection are
+    read in place where their steps are whole 16 bytes, other layouts are copied."""
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and lam.is_cuda):
+        raise RuntimeError("diff_attention: GPU tensors only (no CPU path exists)")
+    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"diff_attention: q, k, v all f32 or all bf16, not {q.dtype}, {k.dtype}, {v.dtype}")
+    if lam.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"diff_attention: lam f32 or bf16, not {lam.dtype}")
+    if q.dim() != 5 or k.dim() != 5 or v.dim() != 4 or q.shape[3] != 2 or k.shape[3] != 2:
+        raise RuntimeError(f"diff_attention: q [B,Tq,H,2,d], k [B,Tk,Hk,2,d], v [B,Tk,Hk,2d]; got {tuple(q.shape)}, "
+                           f"{tuple(k.shape)}, {tuple(v.shape)}")
+    B, Tq, H, _, d = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    if k.shape != (B, Tk, Hk, 2, d) or v.shape != (B, Tk, Hk, 2 * d) or Hk == 0 or H == 0 or H % Hk:
+        raise RuntimeError(f"diff_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    if d % 8 or not 8 <= d <= 64:
+        raise NotImplementedError(f"diff_attention: d = {d} is not a multiple of 8 up to 64")
+    if tuple(lam.shape) != (H,):
+        raise RuntimeError(f"diff_attention: lam {tuple(lam.shape)} for {H} heads")
+    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
+        raise RuntimeError(f"diff_attention: lengths is a contiguous int32 [{B}], not {lengths.dtype} {tuple(lengths.shape)}")
+    if any(t.device != q.device for t in (k, v, lam, *(() if lengths is None else (lengths,)))):
+        raise RuntimeError("diff_attention: all tensors on one device")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"diff_attention: scale must be positive, not {scale}")
+    with torch.cuda.device(q.device):
+        return DiffAttentionFn.apply(ops.kernel_layout(q), ops.kernel_layout(k), ops.kernel_layout(v), lam.contiguous(), lengths,
+                                     bool(causal), scale)
+
+
 # ------------------------------------------------------------------------------ AdamW
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs, exp_avg_sqs, state: torch.Tensor, lr,
                betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01, seed: int = 0,

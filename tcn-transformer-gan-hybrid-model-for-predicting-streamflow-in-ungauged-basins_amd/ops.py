@@ -42,6 +42,12 @@ class GemmDesc(ctypes.Structure):
                 ("aux_mode", _c_int), ("g", ConvGeom), ("split_stride", _c_ll)]
 
 
+class DiffAttnDesc(ctypes.Structure):
+    _fields_ = [("dtype", _c_int), ("lam_dtype", _c_int), ("B", _c_int), ("Tq", _c_int), ("Tk", _c_int), ("H", _c_int),
+                ("Hk", _c_int), ("d", _c_int), ("causal", _c_int), ("scale", _c_f),
+                ("q_stride", _c_ll * 3), ("k_stride", _c_ll * 3), ("v_stride", _c_ll * 3)]
+
+
 _lib = None
 
 
@@ -69,6 +75,8 @@ def lib():
         L.sf_gru_save_floats.restype = ctypes.c_size_t
         L.sf_attn_save_floats.restype = ctypes.c_size_t
         L.sf_layer_norm_bwd_workspace_bytes.restype = ctypes.c_size_t
+        L.sf_diff_attn_fwd_workspace_bytes.restype = ctypes.c_size_t
+        L.sf_diff_attn_bwd_workspace_bytes.restype = ctypes.c_size_t
         _lib = L
     return _lib
 
@@ -84,7 +92,8 @@ EXPORTS = ["sf_version", "sf_last_error", "sf_gemm", "sf_gemm_batch", "sf_conv3x
            "sf_gather_frames", "sf_date_image_metrics", "sf_date_image_metrics_workspace_bytes", "sf_bn_relu_fwd",
            "sf_relu_dropout_fwd", "sf_relu_dropout_bwd", "sf_gru_save_floats", "sf_gru_fwd", "sf_gru_bwd",
            "sf_attn_save_floats", "sf_attn_fwd", "sf_attn_bwd", "sf_token_outer4",
-           "sf_layer_norm_fwd", "sf_layer_norm_bwd", "sf_layer_norm_bwd_workspace_bytes", "sf_adamw_step", "sf_adamw_moments"]
+           "sf_layer_norm_fwd", "sf_layer_norm_bwd", "sf_layer_norm_bwd_workspace_bytes", "sf_adamw_step", "sf_adamw_moments",
+           "sf_diff_attn_fwd", "sf_diff_attn_fwd_workspace_bytes", "sf_diff_attn_bwd", "sf_diff_attn_bwd_workspace_bytes"]
 
 
 def _check(rc: int, who: str):
@@ -1109,6 +1118,70 @@ def layer_norm_bwd(dy, dsum, s, w, mean, rstd, need_dw=True, need_db=True):
         _check(lib().sf_layer_norm_bwd(_p(dy), _p(dsum), _p(s), _p(w), _p(mean), _p(rstd), _p(dx), _p(dw), _p(db), _p(ws),
                                        ctypes.c_size_t(nb), _c_ll(rows), D, code, _stream()), "sf_layer_norm_bwd")
     return dx, dw, db
+
+
+# ------------------------------------------------------------------------------ differential attention
+def _token_strides(t: torch.Tensor):
+    """(sample, token, head) strides of [B, T, heads, .. one head contiguous ..] as the kernels take them, or None when
+    the layout has to be copied first: halves and values not contiguous, a token step below a head, pieces
+    that are not whole 16 bytes.  Axes of length one get the stride of a contiguous tensor."""
+    width = 1
+    for n, st in zip(reversed(t.shape[3:]), reversed(t.stride()[3:])):
+        if n != 1 and st != width:
+            return None
+        width *= n
+    B, T, H = t.shape[:3]
+    sh = t.stride(2) if H != 1 else width
+    st = t.stride(1) if T != 1 else H * width
+    sb = t.stride(0) if B != 1 else T * H * width
+    unit = 16 // t.element_size()
+    if sh % unit or st % unit or sb % unit or t.data_ptr() % 16 or st < width or st >= 1 << 22:
+        return None
+    return sb, st, sh
+
+
+def kernel_layout(t: torch.Tensor) -> torch.Tensor:
+    """t itself when the attention kernels can read it in place, else a contiguous copy."""
+    return t if _token_strides(t) is not None else t.clone(memory_format=torch.contiguous_format)
+
+
+def _diff_attn_desc(q, k, v, lam, causal, scale):
+    B, Tq, H, _, d = q.shape
+    strides = [_token_strides(t) for t in (q, k, v)]
+    if None in strides:
+        raise RuntimeError("diff_attention: a layout the kernels cannot read (see kernel_layout)")
+    return DiffAttnDesc(code_of(q.dtype), code_of(lam.dtype), B, Tq, k.shape[1], H, k.shape[2], d, int(causal), scale,
+                        *[(_c_ll * 3)(*s) for s in strides])
+
+
+def diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need_save=False):
+    """q [B,Tq,H,2,d], k [B,Tk,Hk,2,d], v [B,Tk,Hk,2d], lam [H] -> (o [B,Tq,H,2d], o2, lse); o2 and lse (what the
+    backward pass needs) are None unless wanted."""
+    B, Tq, H, _, d = q.shape
+    o = torch.empty((B, Tq, H, 2 * d), device=q.device, dtype=q.dtype)
+    o2 = torch.empty_like(o) if need_save else None
+    lse = torch.empty((B, H, Tq, 2), device=q.device, dtype=torch.float32) if need_save else None
+    if o.numel() == 0 or k.numel() == 0:        # no query, or no key for anyone
+        return o.zero_(), o2, lse
+    desc = _diff_attn_desc(q, k, v, lam, causal, scale)
+    nb = int(lib().sf_diff_attn_fwd_workspace_bytes(ctypes.byref(desc)))
+    ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
+    _check(lib().sf_diff_attn_fwd(ctypes.byref(desc), _p(q), _p(k), _p(v), _p(lam), _p(lengths), _p(o), _p(o2), _p(lse), _p(ws),
+                                  ctypes.c_size_t(nb), _stream()), "sf_diff_attn_fwd")
+    return o, o2, lse
+
+
+def diff_attn_bwd(q, k, v, lam, lengths, causal, scale, o, o2, lse, do, need_dlam=True):
+    """(dq, dk, dv, dlam), contiguous."""
+    _dev(o, o2, lse, do, dtypes=[q.dtype, q.dtype, torch.float32, q.dtype])
+    dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+    dlam = torch.empty_like(lam) if need_dlam else None
+    desc = _diff_attn_desc(q, k, v, lam, causal, scale)
+    nb = int(lib().sf_diff_attn_bwd_workspace_bytes(ctypes.byref(desc)))
+    ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
+    _check(lib().sf_diff_attn_bwd(ctypes.byref(desc), _p(q), _p(k), _p(v), _p(lam), _p(lengths), _p(o), _p(o2), _p(lse), _p(do),
+                                  _p(dq), _p(dk), _p(dv), _p(dlam), _p(ws), ctypes.c_size_t(nb), _stream()), "sf_diff_attn_bwd")
+    return dq, dk, dv, dlam
 
 
 # ------------------------------------------------------------------------------ losses / optimiser
