@@ -628,8 +628,9 @@ int sf_layer_norm_bwd(const void* dy, const void* dsum, const void* s, const flo
  * head h reads key / value head h / (H / Hk)); d <= 64 a multiple of 8; dtype f32 or bf16; lam [H], lam_dtype f32 or bf16;
  * scale > 0.  lengths: int32 [B] on the device, keys of each sample (clamped to [0, Tk]), or NULL; keys from
  * there on are not read.  causal: query t sees keys up to t + Tk - Tq.  A query that sees no key gets zeros and has
- * no gradient.  All pointers 16-byte aligned; o, o2, do, dq [B,Tq,H,2d] and dk, dv [B,Tk,Hk,2d] contiguous.
- * Forward: o2 and lse f32 [B,H,Tq,2] are kept for the backward pass (both NULL in inference); ws:
+ * no gradient.  All pointers 16-byte aligned; o, do, dq [B,Tq,H,2d] and dk, dv [B,Tk,Hk,2d] contiguous.
+ * Forward: maps f32 [B,Tq,H,2,2d] (both softmax maps' results) and lse f32 [B,H,Tq,2] are kept for the backward pass (both
+ * NULL in inference); ws:
  * sf_diff_attn_fwd_workspace_bytes(desc) bytes (may be 0), any contents.  Backward: dlam [H] of lam's type, or NULL;
  * every output is overwritten; ws: sf_diff_attn_bwd_workspace_bytes(desc) bytes.  No atomics: equal calls give equal
  * results.  The workspace size functions return 0 for a descriptor that the call itself refuses. */
@@ -640,11 +641,11 @@ typedef struct sf_diff_attn_desc {
 } sf_diff_attn_desc;
 size_t sf_diff_attn_fwd_workspace_bytes(const sf_diff_attn_desc* desc);
 int sf_diff_attn_fwd(const sf_diff_attn_desc* desc, const void* q, const void* k, const void* v, const void* lam,
-                     const int* lengths, void* o, void* o2, float* lse, void* ws, size_t ws_bytes, void* stream);
+                     const int* lengths, void* o, float* maps, float* lse, void* ws, size_t ws_bytes, void* stream);
 size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* desc);
 int sf_diff_attn_bwd(const sf_diff_attn_desc* desc, const void* q, const void* k, const void* v, const void* lam,
-                     const int* lengths, const void* o, const void* o2, const float* lse, const void* dout, void* dq,
-                     void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream);
+                     const int* lengths, const float* maps, const float* lse, const void* dout, void* dq, void* dk,
+                     void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- AdamW over many tensors -------------------------------------------------------------------- */
 /* One AdamW step (decoupled weight decay; the reference trains with Adam, src/train.py:80-91) of `count`

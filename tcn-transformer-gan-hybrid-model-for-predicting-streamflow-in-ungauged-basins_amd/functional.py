@@ -873,18 +873,18 @@ class DiffAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, lengths, causal, scale):
         need = any(ctx.needs_input_grad[:4])
-        o, o2, lse = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need)
+        o, maps, lse = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need)
         if need:
-            ctx.save_for_backward(q, k, v, lam, lengths, o, o2, lse)
+            ctx.save_for_backward(q, k, v, lam, lengths, maps, lse)
         ctx.cfg = (causal, scale)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, lam, lengths, o, o2, lse = ctx.saved_tensors
-        if o.numel() == 0 or k.numel() == 0:
+        q, k, v, lam, lengths, maps, lse = ctx.saved_tensors
+        if maps.numel() == 0 or k.numel() == 0:
             return (*(torch.zeros(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, lam)), None, None, None)
-        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, *ctx.cfg, o, o2, lse, do.contiguous(), ctx.needs_input_grad[3])
+        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, *ctx.cfg, maps, lse, do.contiguous(), ctx.needs_input_grad[3])
         return (*grads, None, None, None)
 
 

@@ -1155,32 +1155,32 @@ def _diff_attn_desc(q, k, v, lam, causal, scale):
 
 
 def diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need_save=False):
-    """q [B,Tq,H,2,d], k [B,Tk,Hk,2,d], v [B,Tk,Hk,2d], lam [H] -> (o [B,Tq,H,2d], o2, lse); o2 and lse (what the
+    """q [B,Tq,H,2,d], k [B,Tk,Hk,2,d], v [B,Tk,Hk,2d], lam [H] -> (o [B,Tq,H,2d], maps, lse); maps and lse (what the
     backward pass needs) are None unless wanted."""
     B, Tq, H, _, d = q.shape
     o = torch.empty((B, Tq, H, 2 * d), device=q.device, dtype=q.dtype)
-    o2 = torch.empty_like(o) if need_save else None
+    maps = torch.empty((B, Tq, H, 2, 2 * d), device=q.device, dtype=torch.float32) if need_save else None
     lse = torch.empty((B, H, Tq, 2), device=q.device, dtype=torch.float32) if need_save else None
     if o.numel() == 0 or k.numel() == 0:        # no query, or no key for anyone
-        return o.zero_(), o2, lse
+        return o.zero_(), maps, lse
     desc = _diff_attn_desc(q, k, v, lam, causal, scale)
     nb = int(lib().sf_diff_attn_fwd_workspace_bytes(ctypes.byref(desc)))
     ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
-    _check(lib().sf_diff_attn_fwd(ctypes.byref(desc), _p(q), _p(k), _p(v), _p(lam), _p(lengths), _p(o), _p(o2), _p(lse), _p(ws),
+    _check(lib().sf_diff_attn_fwd(ctypes.byref(desc), _p(q), _p(k), _p(v), _p(lam), _p(lengths), _p(o), _p(maps), _p(lse), _p(ws),
                                   ctypes.c_size_t(nb), _stream()), "sf_diff_attn_fwd")
-    return o, o2, lse
+    return o, maps, lse
 
 
-def diff_attn_bwd(q, k, v, lam, lengths, causal, scale, o, o2, lse, do, need_dlam=True):
+def diff_attn_bwd(q, k, v, lam, lengths, causal, scale, maps, lse, do, need_dlam=True):
     """(dq, dk, dv, dlam), contiguous."""
-    _dev(o, o2, lse, do, dtypes=[q.dtype, q.dtype, torch.float32, q.dtype])
+    _dev(maps, lse, do, dtypes=[torch.float32, torch.float32, q.dtype])
     dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
     dlam = torch.empty_like(lam) if need_dlam else None
     desc = _diff_attn_desc(q, k, v, lam, causal, scale)
     nb = int(lib().sf_diff_attn_bwd_workspace_bytes(ctypes.byref(desc)))
     ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
-    _check(lib().sf_diff_attn_bwd(ctypes.byref(desc), _p(q), _p(k), _p(v), _p(lam), _p(lengths), _p(o), _p(o2), _p(lse), _p(do),
-                                  _p(dq), _p(dk), _p(dv), _p(dlam), _p(ws), ctypes.c_size_t(nb), _stream()), "sf_diff_attn_bwd")
+    _check(lib().sf_diff_attn_bwd(ctypes.byref(desc), _p(q), _p(k), _p(v), _p(lam), _p(lengths), _p(maps), _p(lse), _p(do), _p(dq),
+                                  _p(dk), _p(dv), _p(dlam), _p(ws), ctypes.c_size_t(nb), _stream()), "sf_diff_attn_bwd")
     return dq, dk, dv, dlam
 
 

@@ -6,7 +6,7 @@ tens: each probability is off by (|argument| <= 64) f32 half-steps from the argu
 sums of d products; 2^-24 * 256 of the sum of the terms' magnitudes bounds every output.  bf16: inputs are exact in
 both; each probability (and score gradient) enters the second product rounded by half a step 2^-9 * 2 = u of its
 size at most u = 2^-8 (the bound is per element, the sums below add the magnitudes), outputs are rounded once more (u of
-the value), delta carries the rounding of o and o2 (u of the sum of |do| |o| terms).  So an output is within
+the value), delta carries the rounding of the probabilities in the saved maps (u of the sum of |do| |o| terms).  So an output is within
 u * (|value| + 2.5 * sum of the magnitudes of its terms), where the terms of dS hold |dP| + |delta| and the rounding
 of delta; the factor 2.5 covers probability, delta and score-gradient rounding, one u each being the worst
 case of a whole row rounded the same way, at half weight as 2^-8 is twice the half step bf16 has."""
@@ -59,7 +59,7 @@ def oracle(q, k, v, lam, causal, lengths, scale, do=None):
             mag["dlam"][h] += (G.abs() * (P[1] @ vb[:, j].abs())).sum()
             for i, f in ((0, 1.0), (1, -lam[h])):
                 delta = (P[i] * dP).sum(1, keepdim=True)
-                # delta comes from the rounded o and o2: |do| . (|o| + |lam| |o2|) in magnitude
+                # delta carries the rounding of the probabilities: |do| . (P_1 + |lam| 2 P_2) |v| in magnitude
                 dm = (G.abs() * ((P[0] + lam[h].abs() * 2 * P[1]) @ vb[:, j].abs())).sum(1, keepdim=True)
                 dS = f * P[i] * (dP - delta) * scale
                 dSm = abs(f) * P[i] * (dP.abs() + dm) * scale
@@ -360,23 +360,23 @@ def test_library_refusals():
                  ll3(*f["q"]), ll3(*f["k"]), ll3(*f["v"]))
     a = ctypes.c_void_p(4096)
 
-    def fwd(d, q=a, lam=a, o2=None, lse=None, ws=None, nbytes=0):
-        return L.sf_diff_attn_fwd(ctypes.byref(d), q, a, a, lam, None, a, o2, lse, ws, ctypes.c_size_t(nbytes), None)
+    def fwd(d, q=a, lam=a, maps=None, lse=None, ws=None, nbytes=0):
+        return L.sf_diff_attn_fwd(ctypes.byref(d), q, a, a, lam, None, a, maps, lse, ws, ctypes.c_size_t(nbytes), None)
     for bad in (dict(dtype=2), dict(lam_dtype=5), dict(B=0), dict(Tq=0), dict(Tk=0), dict(H=3, Hk=2), dict(Hk=0), dict(d=12), dict(d=72),
                 dict(d=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(q=(256, 68, 32)), dict(k=(128, 16, 32)),
                 dict(v=(128, 1 << 22, 32)), dict(q=(-256, 64, 32)), dict(Tq=(1 << 24) + 1)):
         assert fwd(desc(**bad)) == -22, bad
         assert int(L.sf_diff_attn_fwd_workspace_bytes(ctypes.byref(desc(**bad)))) == 0
     assert fwd(desc(), q=ctypes.c_void_p(4104)) == -22 and fwd(desc(), q=None) == -22
-    assert fwd(desc(), lam=None) == -22 and fwd(desc(), o2=a) == -22 and fwd(desc(), lse=a) == -22
+    assert fwd(desc(), lam=None) == -22 and fwd(desc(), maps=a) == -22 and fwd(desc(), lse=a) == -22
     long = desc(Tq=1, Tk=4000)
     need = int(L.sf_diff_attn_fwd_workspace_bytes(ctypes.byref(long)))
     assert need > 0 and fwd(long) == -22 and fwd(long, ws=a, nbytes=need - 1) == -22
     nb = int(L.sf_diff_attn_bwd_workspace_bytes(ctypes.byref(desc())))
-    assert nb == 1 * 2 * 4 * 16
+    assert nb >= 1 * 2 * 4 * 16
 
     def bwd(ws=a, n=nb, do=a):
-        return L.sf_diff_attn_bwd(ctypes.byref(desc()), a, a, a, a, None, a, a, a, do, a, a, a, a, ws, ctypes.c_size_t(n), None)
+        return L.sf_diff_attn_bwd(ctypes.byref(desc()), a, a, a, a, None, a, a, do, a, a, a, a, ws, ctypes.c_size_t(n), None)
     assert bwd(ws=None) == -22 and bwd(n=nb - 1) == -22 and bwd(do=None) == -22
 
 
