@@ -316,6 +316,15 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
     lds_ptr const buf0 = (lds_ptr)smem;
     lds_ptr const buf1 = buf0 + 2 * TB;
 
+    auto exponentials = [&](float* p, const f32x16& s, float ref) {
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(s[r] * a.c - ref);
+            sum += p[r];
+        }
+        return sum;
+    };
     auto sub_tile = [&](lds_cptr kt, lds_cptr vt, int sub, int key0) {
         if (key0 >= vmax) return;
         f32x16 s[2] = {zero16(), zero16()};
@@ -335,27 +344,24 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
         Frag<T> pf[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float top = s[i][0];
+            // The reference point m of the exponentials only has to keep them in range: it moves when a lane's 16 of them
+            // add up to more than 2^12 (always at a row's first visible key, m being -1e30 before), then to the row's
+            // maximum.  The usual tile so needs no maximum, no exchange between lanes and no rescaling.
+            float p[16];
+            float sum = exponentials(p, s[i], m[i]);
+            if (__any(sum > 4096.f)) {
+                float top = s[i][0];
 #pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[i][r]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
-            // The maximum only has to keep the exponentials in range: it follows when a row outgrows it by 2^8, so the
-            // accumulators are rescaled a few times per row instead of at every tile.
-            if (__any(top > m[i] + 8.f)) {
-                const float mn = fmaxf(m[i], top);
-                const float f = exp2f(m[i] - mn);
+                for (int r = 1; r < 16; ++r) top = fmaxf(top, s[i][r]);
+                top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
+                const float mn = fmaxf(m[i], top), f = exp2f(m[i] - mn);
                 m[i] = mn;
                 l[i] *= f;
 #pragma unroll
                 for (int n = 0; n < DT; ++n)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[i][n][r] *= f;
-            }
-            float p[16], sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                p[r] = __builtin_amdgcn_exp2f(s[i][r] * a.c - m[i]);
-                sum += p[r];
+                sum = exponentials(p, s[i], m[i]);
             }
             l[i] += sum;
             pack(pf[i][0], p);
