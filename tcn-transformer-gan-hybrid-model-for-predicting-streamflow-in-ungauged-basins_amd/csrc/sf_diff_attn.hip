@@ -130,39 +130,35 @@ __device__ __forceinline__ void copy_piece(__amdgpu_buffer_rsrc_t rs, lds_ptr ds
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off, 0, 0, 0);
 }
 
-// Copies ROWS rows of a [.., 2, d] array into a tile, NW waves together.  The byte offsets of a thread's pieces do not
-// change from tile to tile; the tile's first row enters through the buffer's base address (64 bits).
+// Copies ROWS rows of a [.., 2, d] array into a tile, NW waves together, STEP rows at a time.  A lane's byte offset is the
+// same in every step of every tile (the XOR of a row's pieces repeats every STEP rows); the step's first row enters
+// through the buffer's base address (64 bits).
 template <typename T, int DP, int ROWS, int NW> struct Copy {
     using L = Tile<T, DP>;
-    static constexpr int PIECES = ROWS * L::NCH;
-    static constexpr int JOBS = (PIECES + 64 * NW - 1) / (64 * NW);
-    static_assert(PIECES % 64 == 0, "whole waves copy");
-    int off[JOBS];
+    static constexpr int STEP = NW * L::GROUP < ROWS ? NW * L::GROUP : ROWS;
+    static_assert(ROWS % STEP == 0 && (STEP % 16 == 0 || L::x(STEP) == L::x(0)), "whole steps that repeat the XOR");
+    int off;
     long long stride;         // bytes from row to row
     int row_bytes;
     __device__ __forceinline__ Copy(long long stride_elems, int d) {
         stride = stride_elems * (long long)sizeof(T);
         row_bytes = 2 * d * (int)sizeof(T);
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-#pragma unroll
-        for (int j = 0; j < JOBS; ++j) {
-            const int i = (j * NW + wave) * 64 + lane, row = i / L::NCH;
-            const int piece = (i % L::NCH) ^ L::x(row);
-            const int half = piece / (L::NCH / 2), e = (piece % (L::NCH / 2)) * L::EPC;
-            off[j] = e < d ? (int)(row * stride) + (half * d + e) * (int)sizeof(T) : (int)0x80000000;
-        }
+        const int i = threadIdx.x, row = i / L::NCH, piece = (i % L::NCH) ^ L::x(row);
+        const int half = piece / (L::NCH / 2), e = (piece % (L::NCH / 2)) * L::EPC;
+        off = e < d ? (int)(row * stride) + (half * d + e) * (int)sizeof(T) : (int)0x80000000;
     }
     // rows row0 .. row0 + ROWS of `base`, of which those below `end` exist
-    __device__ __forceinline__ void issue(const T* base, long long row0, long long end, lds_ptr dst) const {
-        const long long have = end - row0 < ROWS ? end - row0 : ROWS;
-        const unsigned bytes = have > 0 ? (unsigned)((have - 1) * stride) + (unsigned)row_bytes : 0u;
-        const __amdgpu_buffer_rsrc_t rs =
-            __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + row0 * stride), 0, bytes, 0x00020000);
+    __device__ __forceinline__ void issue(const T* base, int row0, int end, lds_ptr dst) const {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (wave * L::GROUP >= STEP) return;
+        const char* p = (const char*)base + row0 * stride;
 #pragma unroll
-        for (int j = 0; j < JOBS; ++j)
-            if (PIECES % (64 * NW) == 0 || (j * NW + wave) * 64 < PIECES)
-                copy_piece(rs, dst + L::row_off((j * NW + wave) * L::GROUP), off[j]);
+        for (int r = 0; r < ROWS; r += STEP) {
+            const int have = min(end - row0 - r, STEP);
+            const unsigned bytes = have > 0 ? (unsigned)(have - 1) * (unsigned)stride + (unsigned)row_bytes : 0u;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p + r * stride), 0, bytes, 0x00020000);
+            copy_piece(rs, dst + (L::row_off(r) + L::row_off(wave * L::GROUP)), off);
+        }
     }
 };
 
@@ -379,8 +375,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
     // `cur` holds tile i, `fill` takes tile i + 1 (restrict: the reads need not wait for that copy)
     auto step = [&](int i, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill) {
         if (i + 1 < last) {
-            kc.issue(kbase, (long long)(i + 1) * KT, kend, fill);
-            vc.issue(vbase, (long long)(i + 1) * KT, kend, fill + TB);
+            kc.issue(kbase, (i + 1) * KT, kend, fill);
+            vc.issue(vbase, (i + 1) * KT, kend, fill + TB);
         }
         if constexpr (KEYS_SPLIT) {
             sub_tile(cur, cur + TB, wave * 32, i * KT + wave * 32);
@@ -390,8 +386,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
         }
     };
     if (first < last) {
-        kc.issue(kbase, (long long)first * KT, kend, buf0);
-        vc.issue(vbase, (long long)first * KT, kend, buf0 + TB);
+        kc.issue(kbase, first * KT, kend, buf0);
+        vc.issue(vbase, first * KT, kend, buf0 + TB);
         for (int i = first;;) {
             stage_sync();
             step(i, buf0, buf1);
@@ -689,15 +685,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Ar
     };
     auto step = [&](int i, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill) {
         if (i + 1 < last) {
-            kc.issue(kbase, (long long)(i + 1) * KT, kend, fill);
-            vc.issue(vbase, (long long)(i + 1) * KT, kend, fill + TB);
+            kc.issue(kbase, (i + 1) * KT, kend, fill);
+            vc.issue(vbase, (i + 1) * KT, kend, fill + TB);
         }
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) sub_tile(cur, cur + TB, u * 32, i * KT + u * 32);
     };
     if (first < last) {
-        kc.issue(kbase, (long long)first * KT, kend, buf0);
-        vc.issue(vbase, (long long)first * KT, kend, buf0 + TB);
+        kc.issue(kbase, first * KT, kend, buf0);
+        vc.issue(vbase, first * KT, kend, buf0 + TB);
         for (int i = first;;) {
             stage_sync();
             step(i, buf0, buf1);
@@ -743,7 +739,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
     const int b = bh / a.Hk, hk = bh % a.Hk, k0 = x * KB;
     const int key = k0 + wave * 32 + (lane & 31);
     const int kend = keys_of(a, b), reach = a.Tk - a.Tq;
-    const int t_min = a.causal ? max(0, key - reach) : 0;                  // the key is seen by queries [t_min, Tq)
+    const int t_min = key >= kend ? 1 << 30 : a.causal ? key - reach : 0;  // the key is seen by queries from t_min on
     const int w_first = k0 + wave * 32;                                    // the wave's first key
     const int w_tmax = a.causal ? w_first + 31 - reach : 0;                // queries from here on see all keys of the wave
     const int q_first = a.causal ? max(0, k0 - reach) / QT : 0;            // first query tile that sees a key of the workgroup
@@ -752,17 +748,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
     const int all = per_head * group, per = (all + w.parts - 1) / w.parts;     // (head, query tile) pairs, head by head
     const int first = w.part * per, last = min(all, first + per);
 
-    lds_ptr const vmem = (lds_ptr)smem;                                               // [KB] value rows
-    lds_ptr const buf0 = vmem + L::bytes(KB);
+    lds_ptr const buf0 = (lds_ptr)smem;                                    // (the buffers first: their addresses fit the offset fields)
     lds_ptr const buf1 = buf0 + BUF;
+    lds_ptr const vmem = buf0 + 2 * BUF;                                   // [KB] value rows
     const T* const kbase = a.k + b * a.ks.b + hk * a.ks.h;
     const T* const vbase = a.v + b * a.vs.b + hk * a.vs.h;
     Frag<T> kf[2][KS];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-            kf[i][s] = global_piece<T>(kbase + (key < kend ? (long long)key * a.ks.t : 0), i, s * 16 + 8 * h2, a.d, key < kend);
     f32x16 dv[DT], dk[NA];
 #pragma unroll
     for (int n = 0; n < DT; ++n) dv[n] = zero16();
@@ -775,8 +766,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
     Pos pos{first < last ? first / per_head : 0, first < last ? q_first + first % per_head : 0};
     auto issue = [&](Pos p, lds_ptr dst) {
         const int hq = hk * group + p.head, qt = p.tile;
-        qc.issue(a.q + b * a.qs.b + hq * a.qs.h, (long long)qt * QT, a.Tq, dst);
-        gc.issue(a.dout + (long long)b * a.Tq * gstride + hq * (2 * a.d), (long long)qt * QT, a.Tq, dst + TB);
+        qc.issue(a.q + b * a.qs.b + hq * a.qs.h, qt * QT, a.Tq, dst);
+        gc.issue(a.dout + (long long)b * a.Tq * gstride + hq * (2 * a.d), qt * QT, a.Tq, dst + TB);
         if (wave == 0) {
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
                 (void*)(a.stat + ((long long)b * a.H + hq) * 4 * a.Tp + qt * QT), 0, (unsigned)(3 * a.Tp + QT) * 4u, 0x00020000);
@@ -796,59 +787,63 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
         const bool edge = w_first + 32 > kend || (a.causal && t0 < w_tmax);
         f32x16 dp = zero16();
 #pragma unroll
-        for (int n = 0; n < VS; ++n)
+        for (int n = 0; n < VS; ++n) {
+            if (n && n % 4 == 0) __builtin_amdgcn_sched_barrier(0);
             dp = mma(L::row_piece(gt, 0, lane & 31, n, h2), L::row_piece(vals, 0, lane & 31, n, h2), dp);
-        float p[16];                    // P_1 - lam P_2
-        Frag<T> df[2][2];
+        }
+        // One map after the other, its products included: P_1 and -lam P_2 enter dv one by one (8 more matrix instructions than
+        // their difference would) because the registers that hold the first until the second is there are not to be had;
+        // with spills a reload waits for the copies under way (16 spilled registers: 640 us at 2 x 5120 tokens).
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            // one map after the other: with the operand reads of all products in flight the kernel spills 74 registers
             __builtin_amdgcn_sched_barrier(0);
             f32x16 s = zero16();
 #pragma unroll
             for (int n = 0; n < KS; ++n) s = mma(L::row_piece(qt, 0, lane & 31, i * KS + n, h2), kf[i][n], s);
             if (edge) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = key < kend && t0 + acc_row(r, h2) >= t_min ? s[r] : -INFINITY;
+                for (int r = 0; r < 16; ++r) s[r] = t0 + acc_row(r, h2) >= t_min ? s[r] : -INFINITY;
             }
-            float ds[16];
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                if (r == 8) __builtin_amdgcn_sched_barrier(0);
-                const f32x4 lv = *(const SF_LDS f32x4*)(stat + 64 * i + acc_row(r, h2));
-                const f32x4 dl = *(const SF_LDS f32x4*)(stat + 64 * i + 32 + acc_row(r, h2));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float y = __builtin_amdgcn_exp2f(s[r + e] * a.c - lv[e]);
-                    if (i) y *= -lam;
-                    p[r + e] = i ? p[r + e] + y : y;
-                    ds[r + e] = y * (dp[r + e] - dl[e]);
-                }
-            }
-            pack(df[i][0], ds);
-            pack(df[i][1], ds + 8);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        Frag<T> pf[2];
-        pack(pf[0], p);
-        pack(pf[1], p + 8);
-#pragma unroll
-        for (int n = 0; n < DT; ++n)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) dv[n] = mma(L::col_piece(gt, 16 * u, n, lane), pf[u], dv[n]);
-#pragma unroll
-        for (int n = 0; n < NA; ++n)
+            Frag<T> pf[2], df[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int map = DP == 16 ? n : 32 * n / DP;
-                dk[n] = mma(L::col_piece(qt, 16 * u, DP == 16 ? 0 : n, lane), df[map][u], dk[n]);
+                float p[8], ds[8];
+#pragma unroll
+                for (int k = 0; k < 8; k += 4) {
+                    const int r = 8 * u + k;
+                    const f32x4 lv = *(const SF_LDS f32x4*)(stat + 64 * i + acc_row(r, h2));
+                    const f32x4 dl = *(const SF_LDS f32x4*)(stat + 64 * i + 32 + acc_row(r, h2));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[k + e] = __builtin_amdgcn_exp2f(s[r + e] * a.c - lv[e]);
+                        if (i) p[k + e] *= -lam;
+                        ds[k + e] = p[k + e] * (dp[r + e] - dl[e]);
+                    }
+                }
+                pack(pf[u], p);
+                pack(df[u], ds);
             }
+#pragma unroll
+            for (int n = 0; n < DT; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) dv[n] = mma(L::col_piece(gt, 16 * u, n, lane), pf[u], dv[n]);
+#pragma unroll
+            for (int n = 0; n < NA / 2; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    dk[i * (NA / 2) + n] = mma(L::col_piece(qt, 16 * u, DP == 16 ? 0 : i * (NA / 2) + n, lane), df[u], dk[i * (NA / 2) + n]);
+        }
     };
     if (first < last) {
         const Copy<T, DP, KB, NW> vc(a.vs.t, a.d);
         vc.issue(vbase, k0, kend, vmem);
         lds_cptr const vals = vmem + L::row_off(wave * 32);
         issue(pos, buf0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                kf[i][s] = global_piece<T>(kbase + (key < kend ? (long long)key * a.ks.t : 0), i, s * 16 + 8 * h2, a.d, key < kend);
         for (int i = first;;) {
             stage_sync();
             step(i + 1 < last, buf0, buf1, vals);
