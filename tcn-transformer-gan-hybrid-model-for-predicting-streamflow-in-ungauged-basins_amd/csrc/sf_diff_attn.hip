@@ -65,24 +65,21 @@ __device__ __forceinline__ constexpr int acc_row(int r, int h) { return 8 * (r /
 
 // ---- tiles in LDS
 // Rows of NCH 16-byte pieces.  A copy instruction of a wave fills 1 KB, GROUP rows; groups are shifted against each other
-// (pad) and the pieces of a row XORed (x), so that 16 rows at one piece, and 8 rows at 32 columns, fall on different
-// banks (256-byte window).  XOR and shift touch few bits on purpose: the rest of an address is a constant of the
-// instruction, and a lane needs 4 address registers for its row pieces and 2 for its column pieces (a full XOR of
-// the piece index takes 8 and 8, which the key gradient kernel pays for with 74 spilled registers).
+// (pad) and the pieces of a row XORed (x), so that both 16 rows at one piece and 4 rows at 64 bytes cover the 256-byte
+// bank window once.  XOR and shift touch few bits on purpose: the rest of an address is a constant of the instruction,
+// and a lane needs 4 address registers for its row pieces and 4 for its column pieces (a full XOR of the piece index takes
+// 8 and 8, which the key gradient kernel does not have).
 template <typename T, int DP> struct Tile {
     static constexpr int EPC = 16 / (int)sizeof(T);       // elements per 16-byte piece
     static constexpr int NCH = 2 * DP / EPC;
     static constexpr int ROWB = NCH * 16;
     static constexpr int GROUP = 1024 / ROWB;
-    static constexpr int XM = NCH == 32 ? 8 : NCH == 4 ? 3 : 6;           // bits of the piece index that are XORed
+    static constexpr int XM = NCH == 32 ? 8 : NCH == 16 ? 12 : NCH == 8 ? 5 : 3;      // bits of the piece index that are XORed
     static __host__ __device__ __forceinline__ constexpr int x(int row) {
-        return NCH == 32 ? (row & 1) << 3 : NCH == 16 ? (row & 3) << 1 : NCH == 8 ? ((row >> 1) & 3) << 1
-                                                                               : (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
+        return NCH == 32 ? (row & 1) << 3 : NCH == 16 ? (row & 3) << 2
+               : NCH == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 1) : (row >> 2) & 3;
     }
-    static __host__ __device__ __forceinline__ constexpr int pad(int g) {
-        return NCH == 32 ? (g >> 3) * 256 + (g & 7) * 16
-               : NCH == 16 ? (g >> 2) * 256 + ((g >> 1) & 1) * 128 + (g & 1) * 16 : NCH == 8 ? g * 16 : 0;
-    }
+    static __host__ __device__ __forceinline__ constexpr int pad(int g) { return NCH >= 16 ? g * 16 : NCH == 8 ? g * 32 : 0; }
     static __host__ __device__ __forceinline__ constexpr int row_off(int row) { return row * ROWB + pad(row / GROUP); }
     static constexpr int bytes(int rows) { return row_off(rows); }
     // byte offset of piece c_const + c_lane (no common bits) of row r_const + r_lane (r_const a multiple of 16)
@@ -124,10 +121,10 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// 64 lanes x 16 bytes from the buffer's byte offsets `off` to LDS from `dst` on (uniform); zeros where the offset lies outside
+// 64 lanes x 16 bytes from the buffer's byte offsets `off` + `soff` to LDS from `dst` on (uniform); zeros where off lies outside
 // the buffer.  (Not in a template: in one, the host pass drops the launch stubs of every kernel that uses the builtin.)
-__device__ __forceinline__ void copy_piece(__amdgpu_buffer_rsrc_t rs, lds_ptr dst, int off) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off, 0, 0, 0);
+__device__ __forceinline__ void copy_piece(__amdgpu_buffer_rsrc_t rs, lds_ptr dst, int off, int soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, dst, 16, off, soff, 0, 0);
 }
 
 // Copies ROWS rows of a [.., 2, d] array into a tile, NW waves together, STEP rows at a time.  A lane's byte offset is the
@@ -137,27 +134,34 @@ template <typename T, int DP, int ROWS, int NW> struct Copy {
     using L = Tile<T, DP>;
     static constexpr int STEP = NW * L::GROUP < ROWS ? NW * L::GROUP : ROWS;
     static_assert(ROWS % STEP == 0 && (STEP % 16 == 0 || L::x(STEP) == L::x(0)), "whole steps that repeat the XOR");
-    int off;
-    long long stride;         // bytes from row to row
-    int row_bytes;
+    int off, stride, row_bytes;         // bytes
     __device__ __forceinline__ Copy(long long stride_elems, int d) {
-        stride = stride_elems * (long long)sizeof(T);
+        stride = (int)(stride_elems * (long long)sizeof(T));
         row_bytes = 2 * d * (int)sizeof(T);
         const int i = threadIdx.x, row = i / L::NCH, piece = (i % L::NCH) ^ L::x(row);
         const int half = piece / (L::NCH / 2), e = (piece % (L::NCH / 2)) * L::EPC;
-        off = e < d ? (int)(row * stride) + (half * d + e) * (int)sizeof(T) : (int)0x80000000;
+        off = e < d ? row * stride + (half * d + e) * (int)sizeof(T) : (int)0x80000000;
     }
-    // rows row0 .. row0 + ROWS of `base`, of which those below `end` exist
-    __device__ __forceinline__ void issue(const T* base, int row0, int end, lds_ptr dst) const {
+    // ROWS rows from `p` on, of which the first `have` exist.  A whole tile takes one buffer, the steps being scalar offsets;
+    // at the end of the rows every step gets a buffer of its own.  (Offsets stay below 2^32: 128 rows of less than 2^24 bytes.)
+    __device__ __forceinline__ void issue(const T* p, int have, lds_ptr dst) const {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         if (wave * L::GROUP >= STEP) return;
-        const char* p = (const char*)base + row0 * stride;
+        dst += L::row_off(wave * L::GROUP);
+        if (have >= ROWS) {
+            const __amdgpu_buffer_rsrc_t rs =
+                __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (unsigned)(ROWS - 1) * (unsigned)stride + (unsigned)row_bytes, 0x00020000);
 #pragma unroll
-        for (int r = 0; r < ROWS; r += STEP) {
-            const int have = min(end - row0 - r, STEP);
-            const unsigned bytes = have > 0 ? (unsigned)(have - 1) * (unsigned)stride + (unsigned)row_bytes : 0u;
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p + r * stride), 0, bytes, 0x00020000);
-            copy_piece(rs, dst + (L::row_off(r) + L::row_off(wave * L::GROUP)), off);
+            for (int r = 0; r < ROWS; r += STEP) copy_piece(rs, dst + L::row_off(r), off, r * stride);
+        } else {
+#pragma unroll
+            for (int r = 0; r < ROWS; r += STEP) {
+                const int n = min(have - r, STEP);
+                const unsigned bytes = n > 0 ? (unsigned)(n - 1) * (unsigned)stride + (unsigned)row_bytes : 0u;
+                const __amdgpu_buffer_rsrc_t rs =
+                    __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)p + (long long)r * stride), 0, bytes, 0x00020000);
+                copy_piece(rs, dst + L::row_off(r), off, 0);
+            }
         }
     }
 };
@@ -375,8 +379,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
     // `cur` holds tile i, `fill` takes tile i + 1 (restrict: the reads need not wait for that copy)
     auto step = [&](int i, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill) {
         if (i + 1 < last) {
-            kc.issue(kbase, (i + 1) * KT, kend, fill);
-            vc.issue(vbase, (i + 1) * KT, kend, fill + TB);
+            kc.issue(kbase + (i + 1) * KT * a.ks.t, kend - (i + 1) * KT, fill);
+            vc.issue(vbase + (i + 1) * KT * a.vs.t, kend - (i + 1) * KT, fill + TB);
         }
         if constexpr (KEYS_SPLIT) {
             sub_tile(cur, cur + TB, wave * 32, i * KT + wave * 32);
@@ -386,8 +390,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
         }
     };
     if (first < last) {
-        kc.issue(kbase, first * KT, kend, buf0);
-        vc.issue(vbase, first * KT, kend, buf0 + TB);
+        kc.issue(kbase + first * KT * a.ks.t, kend - first * KT, buf0);
+        vc.issue(vbase + first * KT * a.vs.t, kend - first * KT, buf0 + TB);
         for (int i = first;;) {
             stage_sync();
             step(i, buf0, buf1);
@@ -685,15 +689,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Ar
     };
     auto step = [&](int i, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill) {
         if (i + 1 < last) {
-            kc.issue(kbase, (i + 1) * KT, kend, fill);
-            vc.issue(vbase, (i + 1) * KT, kend, fill + TB);
+            kc.issue(kbase + (i + 1) * KT * a.ks.t, kend - (i + 1) * KT, fill);
+            vc.issue(vbase + (i + 1) * KT * a.vs.t, kend - (i + 1) * KT, fill + TB);
         }
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) sub_tile(cur, cur + TB, u * 32, i * KT + u * 32);
     };
     if (first < last) {
-        kc.issue(kbase, first * KT, kend, buf0);
-        vc.issue(vbase, first * KT, kend, buf0 + TB);
+        kc.issue(kbase + first * KT * a.ks.t, kend - first * KT, buf0);
+        vc.issue(vbase + first * KT * a.vs.t, kend - first * KT, buf0 + TB);
         for (int i = first;;) {
             stage_sync();
             step(i, buf0, buf1);
@@ -762,25 +766,40 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
 
     const Copy<T, DP, QT, NW> qc(a.qs.t, a.d), gc((long long)a.H * 2 * a.d, a.d);
     const long long gstride = (long long)a.H * 2 * a.d;
-    struct Pos { int head, tile; };
-    Pos pos{first < last ? first / per_head : 0, first < last ? q_first + first % per_head : 0};
-    auto issue = [&](Pos p, lds_ptr dst) {
-        const int hq = hk * group + p.head, qt = p.tile;
-        qc.issue(a.q + b * a.qs.b + hq * a.qs.h, qt * QT, a.Tq, dst);
-        gc.issue(a.dout + (long long)b * a.Tq * gstride + hq * (2 * a.d), qt * QT, a.Tq, dst + TB);
+    // the next tile to copy: (head, query tile) and where it lies
+    struct Pos { int head, tile; const T* q; const T* g; const float* stat; } pos{};
+    auto go_to = [&](int head, int tile) {
+        const int hq = hk * group + head, t = tile * QT;
+        pos = {head, tile, a.q + b * a.qs.b + hq * a.qs.h + t * a.qs.t, a.dout + ((long long)b * a.Tq + t) * gstride + hq * (2 * a.d),
+               a.stat + ((long long)b * a.H + hq) * 4 * a.Tp + t};
+    };
+    if (first < last) go_to(first / per_head, q_first + first % per_head);
+    auto issue = [&](lds_ptr dst) {
+        const int have = a.Tq - pos.tile * QT;
+        qc.issue(pos.q, have, dst);
+        gc.issue(pos.g, have, dst + TB);
         if (wave == 0) {
-            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-                (void*)(a.stat + ((long long)b * a.H + hq) * 4 * a.Tp + qt * QT), 0, (unsigned)(3 * a.Tp + QT) * 4u, 0x00020000);
-            copy_piece(rs, dst + 2 * TB, lane < 32 ? (lane >> 3) * a.Tp * 4 + (lane & 7) * 16 : (int)0x80000000);
+            const __amdgpu_buffer_rsrc_t rs =
+                __builtin_amdgcn_make_buffer_rsrc((void*)pos.stat, 0, (unsigned)(3 * a.Tp + QT) * 4u, 0x00020000);
+            copy_piece(rs, dst + 2 * TB, lane < 32 ? (lane >> 3) * a.Tp * 4 + (lane & 7) * 16 : (int)0x80000000, 0);
+        }
+        if (pos.tile + 1 == q_tiles) {
+            go_to(pos.head + 1, q_first);       // (behind the last head nothing is read any more)
+        } else {
+            ++pos.tile;
+            pos.q += QT * a.qs.t;
+            pos.g += QT * gstride;
+            pos.stat += QT;
         }
     };
-    // `pos` in `cur`, the next one goes to `fill`
+    // `cur` holds the tile of (head, tile), the next one goes to `fill`
+    int head = pos.head, tile = pos.tile;
     auto step = [&](bool more, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill, lds_cptr __restrict__ vals) {
-        const int head = pos.head, t0 = pos.tile * QT;
-        if (++pos.tile == q_tiles) { pos.tile = q_first; ++pos.head; }
-        if (more) issue(pos, fill);
+        const int t0 = tile * QT, hq = hk * group + head;
+        if (++tile == q_tiles) { tile = q_first; ++head; }
+        if (more) issue(fill);
         if (w_first >= kend || (a.causal && t0 + QT - 1 + reach < w_first)) return;     // nothing of this wave is seen
-        const float lam = lam_of(a.lam, a.lam_bf16, hk * group + head);
+        const float lam = lam_of(a.lam, a.lam_bf16, hq);
         lds_cptr const qt = cur;
         lds_cptr const gt = cur + TB;
         const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB);        // [lse_1, delta_1, lse_2, delta_2][32]
@@ -836,9 +855,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
     };
     if (first < last) {
         const Copy<T, DP, KB, NW> vc(a.vs.t, a.d);
-        vc.issue(vbase, k0, kend, vmem);
+        vc.issue(vbase + k0 * a.vs.t, kend - k0, vmem);
         lds_cptr const vals = vmem + L::row_off(wave * 32);
-        issue(pos, buf0);
+        issue(buf0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
