@@ -199,7 +199,7 @@ template <typename T> struct Args {
     const T* dout; const float* maps_in; const float* lse_in;
     float* stat;                            // [B,H,4,Tp]: lse_1, delta_1, lse_2, delta_2; zeros from Tq to Tp
     T* dq; T* dk; T* dv;
-    int lam_bf16, B, Tq, Tp, Tk, H, Hk, d, causal;        // Tp: Tq rounded up to 32
+    int lam_bf16, B, Tq, Tp, Tk, H, Hk, d, causal;        // Tp: Tq rounded up to 64
     int full, parts;                        // see Cut
     float scale, c;                         // c = scale * log2(e)
 };
@@ -724,14 +724,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Ar
         }
 }
 
-// Gradients of the keys and values: a wave owns 32 keys (keys in registers, values in LDS), the workgroup's 128 keys
-// meet the query rows of every head of the group 32 at a time.
-template <typename T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args<T> a) {
+// Gradients of the keys and values: a wave owns 32 keys, the workgroup's 128 keys meet the query rows of every head of the
+// group tile by tile.  PAIRED (bf16 heads of 2 x 64): eight waves, two for the same keys on alternate 32 rows of a 64-row tile,
+// keys and values both in LDS (one workgroup per CU); the pairs' sums are joined through LDS at the end.  With the keys in
+// registers, four waves and two workgroups per CU the 128 accumulators leave too few: the kernel spills, and a reload
+// waits for the copies under way (2 x 5120 tokens, 8 heads: KVTIME).  Not PAIRED: four waves, keys in registers.
+template <typename T, int DP, bool PAIRED>
+__global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args<T> a) {
     using L = Tile<T, DP>;
-    constexpr int NW = 4, KB = 32 * NW, QT = 32, KS = DP / 16, VS = 2 * DP / 16, DT = 2 * DP / 32;
+    constexpr int NW = PAIRED ? 8 : 4, KB = 128, QT = PAIRED ? 64 : 32, KS = DP / 16, VS = 2 * DP / 16, DT = 2 * DP / 32;
     constexpr int NA = DP == 16 ? 2 : DT;
-    constexpr int TB = L::bytes(QT), SB = 1024;            // query / gradient tile; row statistics (512 bytes, copied by a wave)
+    constexpr int TB = L::bytes(QT), SB = 1024;            // query / gradient tile; row statistics (16 QT bytes, copied by a wave)
     constexpr int BUF = 2 * TB + SB;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h2 = lane >> 5;
@@ -741,10 +744,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
     int bh, x;
     locate(w.item, a.B * a.Hk, tiles, a.causal, bh, x);
     const int b = bh / a.Hk, hk = bh % a.Hk, k0 = x * KB;
-    const int key = k0 + wave * 32 + (lane & 31);
+    const int kw = wave & 3, rows0 = PAIRED ? (wave >> 2) * 32 : 0;        // the wave's 32 keys, and its rows of a query tile
+    const int key = k0 + kw * 32 + (lane & 31);
     const int kend = keys_of(a, b), reach = a.Tk - a.Tq;
     const int t_min = key >= kend ? 1 << 30 : a.causal ? key - reach : 0;  // the key is seen by queries from t_min on
-    const int w_first = k0 + wave * 32;                                    // the wave's first key
+    const int w_first = k0 + kw * 32;                                    // the wave's first key
     const int w_tmax = a.causal ? w_first + 31 - reach : 0;                // queries from here on see all keys of the wave
     const int q_first = a.causal ? max(0, k0 - reach) / QT : 0;            // first query tile that sees a key of the workgroup
     const int q_tiles = (a.Tq + QT - 1) / QT;
@@ -755,9 +759,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
     lds_ptr const buf0 = (lds_ptr)smem;                                    // (the buffers first: their addresses fit the offset fields)
     lds_ptr const buf1 = buf0 + BUF;
     lds_ptr const vmem = buf0 + 2 * BUF;                                   // [KB] value rows
+    lds_ptr const kmem = vmem + L::bytes(KB);                              // [KB] key rows (PAIRED)
     const T* const kbase = a.k + b * a.ks.b + hk * a.ks.h;
     const T* const vbase = a.v + b * a.vs.b + hk * a.vs.h;
-    Frag<T> kf[2][KS];
     f32x16 dv[DT], dk[NA];
 #pragma unroll
     for (int n = 0; n < DT; ++n) dv[n] = zero16();
@@ -781,7 +785,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
         if (wave == 0) {
             const __amdgpu_buffer_rsrc_t rs =
                 __builtin_amdgcn_make_buffer_rsrc((void*)pos.stat, 0, (unsigned)(3 * a.Tp + QT) * 4u, 0x00020000);
-            copy_piece(rs, dst + 2 * TB, lane < 32 ? (lane >> 3) * a.Tp * 4 + (lane & 7) * 16 : (int)0x80000000, 0);
+            copy_piece(rs, dst + 2 * TB, lane < QT ? lane / (QT / 4) * a.Tp * 4 + lane % (QT / 4) * 16 : (int)0x80000000, 0);
         }
         if (pos.tile + 1 == q_tiles) {
             go_to(pos.head + 1, q_first);       // (behind the last head nothing is read any more)
@@ -794,15 +798,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
     };
     // `cur` holds the tile of (head, tile), the next one goes to `fill`
     int head = pos.head, tile = pos.tile;
+    Frag<T> kf[2][PAIRED ? 1 : KS];
     auto step = [&](bool more, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill, lds_cptr __restrict__ vals) {
-        const int t0 = tile * QT, hq = hk * group + head;
+        const int t0 = tile * QT + rows0, hq = hk * group + head;
         if (++tile == q_tiles) { tile = q_first; ++head; }
         if (more) issue(fill);
-        if (w_first >= kend || (a.causal && t0 + QT - 1 + reach < w_first)) return;     // nothing of this wave is seen
+        if (w_first >= kend || (a.causal && t0 + 31 + reach < w_first)) return;     // nothing of this wave is seen
         const float lam = lam_of(a.lam, a.lam_bf16, hq);
-        lds_cptr const qt = cur;
-        lds_cptr const gt = cur + TB;
-        const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB);        // [lse_1, delta_1, lse_2, delta_2][32]
+        lds_cptr const qt = cur + L::row_off(rows0);
+        lds_cptr const gt = qt + TB;
+        lds_cptr const keys = vals + L::bytes(KB);
+        const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB) + rows0;    // [lse_1, delta_1, lse_2, delta_2][QT]
         const bool edge = w_first + 32 > kend || (a.causal && t0 < w_tmax);
         f32x16 dp = zero16();
 #pragma unroll
@@ -810,59 +816,72 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
             if (n && n % 4 == 0) __builtin_amdgcn_sched_barrier(0);
             dp = mma(L::row_piece(gt, 0, lane & 31, n, h2), L::row_piece(vals, 0, lane & 31, n, h2), dp);
         }
-        // One map after the other, its products included: P_1 and -lam P_2 enter dv one by one (8 more matrix instructions than
-        // their difference would) because the registers that hold the first until the second is there are not to be had;
-        // with spills a reload waits for the copies under way (16 spilled registers: 640 us at 2 x 5120 tokens).
+        f32x16 p = zero16();            // P_1 - lam P_2
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);          // (one map after the other: fewer operands in flight)
             f32x16 s = zero16();
 #pragma unroll
-            for (int n = 0; n < KS; ++n) s = mma(L::row_piece(qt, 0, lane & 31, i * KS + n, h2), kf[i][n], s);
+            for (int n = 0; n < KS; ++n) {
+                const Frag<T> qp = L::row_piece(qt, 0, lane & 31, i * KS + n, h2);
+                if constexpr (PAIRED) s = mma(qp, L::row_piece(keys, 0, lane & 31, i * KS + n, h2), s);
+                else s = mma(qp, kf[i][n], s);
+            }
             if (edge) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = t0 + acc_row(r, h2) >= t_min ? s[r] : -INFINITY;
             }
-            Frag<T> pf[2], df[2];
+            Frag<T> df[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                float p[8], ds[8];
+                float ds[8];
 #pragma unroll
                 for (int k = 0; k < 8; k += 4) {
                     const int r = 8 * u + k;
-                    const f32x4 lv = *(const SF_LDS f32x4*)(stat + 64 * i + acc_row(r, h2));
-                    const f32x4 dl = *(const SF_LDS f32x4*)(stat + 64 * i + 32 + acc_row(r, h2));
+                    const f32x4 lv = *(const SF_LDS f32x4*)(stat + 2 * QT * i + acc_row(r, h2));
+                    const f32x4 dl = *(const SF_LDS f32x4*)(stat + 2 * QT * i + QT + acc_row(r, h2));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[k + e] = __builtin_amdgcn_exp2f(s[r + e] * a.c - lv[e]);
-                        if (i) p[k + e] *= -lam;
-                        ds[k + e] = p[k + e] * (dp[r + e] - dl[e]);
+                        float y = __builtin_amdgcn_exp2f(s[r + e] * a.c - lv[e]);
+                        if (i) y *= -lam;
+                        p[r + e] = i ? p[r + e] + y : y;
+                        ds[k + e] = y * (dp[r + e] - dl[e]);
                     }
                 }
-                pack(pf[u], p);
                 pack(df[u], ds);
             }
-#pragma unroll
-            for (int n = 0; n < DT; ++n)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) dv[n] = mma(L::col_piece(gt, 16 * u, n, lane), pf[u], dv[n]);
 #pragma unroll
             for (int n = 0; n < NA / 2; ++n)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     dk[i * (NA / 2) + n] = mma(L::col_piece(qt, 16 * u, DP == 16 ? 0 : i * (NA / 2) + n, lane), df[u], dk[i * (NA / 2) + n]);
         }
+        Frag<T> pf[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = p[8 * u + j];
+            pack(pf[u], x);
+        }
+#pragma unroll
+        for (int n = 0; n < DT; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) dv[n] = mma(L::col_piece(gt, 16 * u, n, lane), pf[u], dv[n]);
     };
     if (first < last) {
         const Copy<T, DP, KB, NW> vc(a.vs.t, a.d);
         vc.issue(vbase + k0 * a.vs.t, kend - k0, vmem);
-        lds_cptr const vals = vmem + L::row_off(wave * 32);
+        if constexpr (PAIRED) Copy<T, DP, KB, NW>(a.ks.t, a.d).issue(kbase + k0 * a.ks.t, kend - k0, kmem);
+        lds_cptr const vals = vmem + L::row_off(kw * 32);
         issue(buf0);
+        if constexpr (!PAIRED) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-                kf[i][s] = global_piece<T>(kbase + (key < kend ? (long long)key * a.ks.t : 0), i, s * 16 + 8 * h2, a.d, key < kend);
+                for (int s = 0; s < KS; ++s)
+                    kf[i][s] = global_piece<T>(kbase + (key < kend ? (long long)key * a.ks.t : 0), i, s * 16 + 8 * h2, a.d, key < kend);
+        }
         for (int i = first;;) {
             stage_sync();
             step(i + 1 < last, buf0, buf1, vals);
@@ -871,6 +890,30 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(A
             step(i + 1 < last, buf1, buf0, vals);
             if (++i >= last) break;
         }
+    }
+    if constexpr (PAIRED) {
+        // the second wave of each pair hands its sums over, 64 floats of every lane at a time
+        SF_LDS float* const box = (SF_LDS float*)smem + (kw * 128) * 64 + lane;
+        static_assert((DT + NA) * 16 <= 128, "one box per pair");
+        __syncthreads();
+        if (wave >= 4) {
+#pragma unroll
+            for (int n = 0; n < DT; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    box[(n * 16 + r) * 64] = dv[n][r];
+                    box[((DT + n) * 16 + r) * 64] = dk[n][r];
+                }
+        }
+        __syncthreads();
+        if (wave >= 4) return;
+#pragma unroll
+        for (int n = 0; n < DT; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dv[n][r] += box[(n * 16 + r) * 64];
+                dk[n][r] += box[((DT + n) * 16 + r) * 64];
+            }
     }
     if (key >= a.Tk) return;
     const long long out = (((long long)b * a.Tk + key) * a.Hk + hk) * (2 * a.d);
@@ -971,7 +1014,8 @@ int per_cu(const sf_diff_attn_desc* p, bool keys_split, bool dkv) {
     const int dp = padded(p->d);
     if (p->dtype == SF_F32) return dp == 16 && !dkv ? 2 : 1;
     if (keys_split) return dp == 16 ? 4 : 2;
-    return dp == 16 ? (dkv ? 3 : 4) : dp == 32 && !dkv ? 3 : 2;
+    if (dkv) return dp == 16 ? 3 : dp == 32 ? 2 : 1;
+    return dp == 16 ? 4 : dp == 32 ? 3 : 2;
 }
 // Up to 32 query rows per key/value head the waves of a workgroup share out the keys of a tile, beyond that the rows.
 struct FwdPlan { bool keys; int nw, kt, rb; Cut cut; };
@@ -1004,7 +1048,7 @@ template <typename T> Args<T> make_args(const sf_diff_attn_desc* p, const void* 
     a.ks = {p->k_stride[0], p->k_stride[1], p->k_stride[2]};
     a.vs = {p->v_stride[0], p->v_stride[1], p->v_stride[2]};
     a.lam = lam; a.lam_bf16 = p->lam_dtype == SF_BF16; a.lengths = lengths;
-    a.B = p->B; a.Tq = p->Tq; a.Tp = (p->Tq + 31) / 32 * 32; a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.d = p->d; a.causal = p->causal != 0;
+    a.B = p->B; a.Tq = p->Tq; a.Tp = (p->Tq + 63) / 64 * 64; a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.d = p->d; a.causal = p->causal != 0;
     a.parts = 1;
     a.scale = p->scale;
     a.c = (float)((double)p->scale * 1.4426950408889634);
@@ -1057,7 +1101,10 @@ template <typename T, int DP> int launch_bwd(Args<T> a, const Cut& cq, const Cut
     constexpr int KT = sizeof(T) == 4 ? 32 : 64;
     hipLaunchKernelGGL((attn_delta_kernel<T>), dim3(ceil_div(n, 16)), dim3(256), 0, st, a);
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (delta)");
-    constexpr int lds_q = 4 * L::bytes(KT), lds_k = L::bytes(128) + 2 * (2 * L::bytes(32) + 1024);
+    constexpr bool paired = sizeof(T) == 2 && DP == 64;
+    constexpr int lds_q = 4 * L::bytes(KT);
+    constexpr int lds_k = (paired ? 2 : 1) * L::bytes(128) + 2 * (2 * L::bytes(paired ? 64 : 32) + 1024);
+    static_assert(!paired || lds_k >= 4 * 128 * 64 * 4, "the pairs' boxes");
     SF_LDS_ONCE((attn_dq_kernel<T, DP, KT>), lds_q);
     a.full = cq.full;
     a.parts = cq.parts;
@@ -1067,10 +1114,10 @@ template <typename T, int DP> int launch_bwd(Args<T> a, const Cut& cq, const Cut
         hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, false>), dim3(cq.tail * 32), dim3(256), 0, st, a, cq.tail);
         SF_LAUNCH_CHECK("sf_diff_attn_bwd (queries, join)");
     }
-    SF_LDS_ONCE((attn_dkv_kernel<T, DP>), lds_k);
+    SF_LDS_ONCE((attn_dkv_kernel<T, DP, paired>), lds_k);
     a.full = ck.full;
     a.parts = ck.parts;
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(ck.full + ck.tail * ck.parts), dim3(256), lds_k, st, a);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, paired>), dim3(ck.full + ck.tail * ck.parts), dim3(paired ? 512 : 256), lds_k, st, a);
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (keys)");
     if (ck.tail) {
         hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, true>), dim3(ck.tail * 32), dim3(256), 0, st, a, ck.tail);
@@ -1087,7 +1134,7 @@ template <typename T> int fwd(const sf_diff_attn_desc* p, const void* q, const v
     const int dp = padded(p->d);
     return dp == 16 ? launch_fwd<T, 16>(a, f, st) : dp == 32 ? launch_fwd<T, 32>(a, f, st) : launch_fwd<T, 64>(a, f, st);
 }
-size_t stat_bytes(const sf_diff_attn_desc* p) { return (size_t)p->B * p->H * ((p->Tq + 31) / 32 * 32) * 4 * sizeof(float); }
+size_t stat_bytes(const sf_diff_attn_desc* p) { return (size_t)p->B * p->H * ((p->Tq + 63) / 64 * 64) * 4 * sizeof(float); }
 template <typename T> int bwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
                               const int* lengths, const float* maps, const float* lse, const void* dout, void* dq, void* dk,
                               void* dv, void* dlam, char* ws, hipStream_t st) {
