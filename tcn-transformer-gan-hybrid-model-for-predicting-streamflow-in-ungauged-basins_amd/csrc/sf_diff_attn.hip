@@ -994,50 +994,51 @@ int check_align(const void* const* ps, int n, const char* who) {
 
 // How a launch's work items are cut.  The chip runs `slots` workgroups at a time; items beyond a whole number of rounds
 // would leave most of it idle in the last one.  Those are cut into the number of parts for which the last rounds take
-// the least time, counted in tiles of the inner axis: one tile of overhead per part, and eight (about 10 us) for the launch
-// that joins them.  Causal items that fill the chip are not cut: they come longest first, the last ones are short.
+// the least time, counted in quarters of an inner tile (64 keys or 32 .. 64 query rows: about 1 us in bf16, 3 to 10 us in f32,
+// whose matrix rate is a sixteenth): what a part costs by itself, and about 10 us for the launch that joins them.
+// Causal items that fill the chip are not cut: they come longest first, the last ones are short.
 struct Cut { int full, tail, parts; };
-Cut cut_items(long long items, int slots, int tiles, bool causal) {
+Cut cut_items(long long items, int slots, int tiles, bool f32, bool causal) {
     const long long full = items / slots * slots, tail = items - full;
     if (!tail || (causal && full)) return {(int)items, 0, 1};
     long long best = 0;
     int parts = 0;
     for (int p = 1; p <= 64 && (p == 1 || tiles / p >= 2); ++p) {
-        const long long rounds = (tail * p + slots - 1) / slots, cost = rounds * ((tiles + p - 1) / p + 1) + (p > 1 ? 8 : 0);
+        const long long rounds = (tail * p + slots - 1) / slots;
+        const long long cost = rounds * (4 * ((tiles + p - 1) / p) + (f32 ? 1 : 4)) + (p > 1 ? (f32 ? 8 : 32) : 0);
         if (!parts || cost < best) { best = cost; parts = p; }
     }
     if (parts == 1) return {(int)items, 0, 1};
     return {(int)full, (int)tail, parts};
 }
-// workgroups that share a CU (registers; the forward pass of single tokens: LDS)
-int per_cu(const sf_diff_attn_desc* p, bool keys_split, bool dkv) {
-    const int dp = padded(p->d);
-    if (p->dtype == SF_F32) return dp == 16 && !dkv ? 2 : 1;
-    if (keys_split) return dp == 16 ? 4 : 2;
-    if (dkv) return dp == 16 ? 3 : dp == 32 ? 2 : 1;
-    return dp == 16 ? 4 : dp == 32 ? 3 : 2;
+// workgroups that share a CU: what the kernels' registers (forward pass of single tokens: LDS) leave room for
+enum Pass { FWD, FWD_KEYS, DQ, DKV };
+int slots_of(const sf_diff_attn_desc* p, Pass pass) {
+    static const int bf16_[4][3] = {{4, 3, 2}, {4, 2, 2}, {4, 3, 2}, {3, 2, 1}}, f32_[4][3] = {{2, 1, 1}, {2, 1, 1}, {2, 2, 1}, {2, 2, 1}};
+    const int w = p->d <= 16 ? 0 : p->d <= 32 ? 1 : 2;
+    return 256 * (p->dtype == SF_F32 ? f32_ : bf16_)[pass][w];
 }
 // Up to 32 query rows per key/value head the waves of a workgroup share out the keys of a tile, beyond that the rows.
-struct FwdPlan { bool keys; int nw, kt, rb; Cut cut; };
+struct FwdPlan { bool keys; int kt, rb; Cut cut; };
 FwdPlan fwd_plan(const sf_diff_attn_desc* p) {
     const long long rows = (long long)(p->H / p->Hk) * p->Tq;
     const bool f32 = p->dtype == SF_F32;
     FwdPlan f;
     f.keys = rows <= 32;
-    f.nw = f.keys && padded(p->d) == 64 ? 2 : 4;
-    f.kt = f.keys ? 32 * f.nw : f32 ? 32 : 64;
+    f.kt = f.keys ? (padded(p->d) == 64 ? 64 : 128) : f32 ? 32 : 64;
     f.rb = f.keys ? 32 : 128;
-    const long long items = (rows + f.rb - 1) / f.rb * p->B * p->Hk;
-    f.cut = cut_items(items, 256 * per_cu(p, f.keys, false), (p->Tk + f.kt - 1) / f.kt, p->causal && !f.keys);
+    f.cut = cut_items((rows + f.rb - 1) / f.rb * p->B * p->Hk, slots_of(p, f.keys ? FWD_KEYS : FWD), (p->Tk + f.kt - 1) / f.kt, f32,
+                      p->causal && !f.keys);
     return f;
 }
 Cut dq_cut(const sf_diff_attn_desc* p) {
     const long long rows = (long long)(p->H / p->Hk) * p->Tq;
-    return cut_items((rows + 127) / 128 * p->B * p->Hk, 256 * per_cu(p, false, false), (p->Tk + 63) / 64, p->causal);
+    return cut_items((rows + 127) / 128 * p->B * p->Hk, slots_of(p, DQ), (p->Tk + 63) / 64, p->dtype == SF_F32, p->causal);
 }
 Cut dkv_cut(const sf_diff_attn_desc* p) {
-    return cut_items((long long)((p->Tk + 127) / 128) * p->B * p->Hk, 256 * per_cu(p, false, true),
-                     (p->Tq + 31) / 32 * (p->H / p->Hk), p->causal);
+    const int qt = p->dtype == SF_BF16 && padded(p->d) == 64 ? 64 : 32;
+    return cut_items((long long)((p->Tk + 127) / 128) * p->B * p->Hk, slots_of(p, DKV), (p->Tq + qt - 1) / qt * (p->H / p->Hk),
+                     p->dtype == SF_F32, p->causal);
 }
 
 template <typename T> Args<T> make_args(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
