@@ -826,19 +826,19 @@ class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, w, b, eps):
         need = any(ctx.needs_input_grad[:4])
-        y, s, mean, rstd = ops.layer_norm_fwd(x, w, b, eps, residual, need)
+        y, s, stats = ops.layer_norm_fwd(x, w, b, eps, residual, need)
         if need:
-            ctx.save_for_backward(s, w, mean, rstd)
+            ctx.save_for_backward(s, w, stats)
         ctx.has_residual = residual is not None
         ctx.set_materialize_grads(False)
         return (y, s) if residual is not None else y
 
     @staticmethod
     def backward(ctx, dy, ds=None):
-        s, w, mean, rstd = ctx.saved_tensors
+        s, w, stats = ctx.saved_tensors
         if dy is None:              # only the sum was used
             return ds, ds, None, None, None
-        dx, dw, db = ops.layer_norm_bwd(dy.contiguous(), None if ds is None else ds.contiguous(), s, w, mean, rstd,
+        dx, dw, db = ops.layer_norm_bwd(dy.contiguous(), None if ds is None else ds.contiguous(), s, w, stats,
                                         ctx.needs_input_grad[2], ctx.needs_input_grad[3])
         return dx, dx if ctx.has_residual else None, dw, db, None
 
@@ -862,7 +862,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
         if t is not None and (tuple(t.shape) != (x.shape[-1],) or t.device != x.device):
             raise RuntimeError(f"layer_norm: {name} {tuple(t.shape)} on {t.device} for rows of {x.shape[-1]} on {x.device}")
     w, b = (None if t is None else t.float().contiguous() for t in (weight, bias))
-    with torch.cuda.device(x.device):
+    with ops.device_guard(x):
         return LayerNormFn.apply(x.contiguous(), None if residual is None else residual.contiguous(), w, b, float(eps))
 
 
@@ -873,18 +873,18 @@ class DiffAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, lengths, causal, scale):
         need = any(ctx.needs_input_grad[:4])
-        o, maps, lse = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need)
+        o, saved = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need)
         if need:
+            ctx.desc, maps, lse = saved or (None, None, None)       # (no query or no key: nothing to save)
             ctx.save_for_backward(q, k, v, lam, lengths, maps, lse)
-        ctx.cfg = (causal, scale)
         return o
 
     @staticmethod
     def backward(ctx, do):
         q, k, v, lam, lengths, maps, lse = ctx.saved_tensors
-        if maps.numel() == 0 or k.numel() == 0:
+        if ctx.desc is None:
             return (*(torch.zeros(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, lam)), None, None, None)
-        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, *ctx.cfg, maps, lse, do.contiguous(), ctx.needs_input_grad[3])
+        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, ctx.desc, maps, lse, do.contiguous(), ctx.needs_input_grad[3])
         return (*grads, None, None, None)
 
 
@@ -922,11 +922,11 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     if any(t.device != q.device for t in (k, v, lam, *(() if lengths is None else (lengths,)))):
         raise RuntimeError("diff_attention: all tensors on one device")
     scale = d ** -0.5 if scale is None else float(scale)
+    q, k, v = ops.kernel_layout(q), ops.kernel_layout(k), ops.kernel_layout(v)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"diff_attention: scale must be positive, not {scale}")
-    with torch.cuda.device(q.device):
-        return DiffAttentionFn.apply(ops.kernel_layout(q), ops.kernel_layout(k), ops.kernel_layout(v), lam.contiguous(), lengths,
-                                     bool(causal), scale)
+    with ops.device_guard(q):
+        return DiffAttentionFn.apply(q, k, v, lam.contiguous(), lengths, bool(causal), scale)
 
 
 # ------------------------------------------------------------------------------ AdamW
@@ -942,7 +942,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     back: copies the package derives from them (packed weights, shadows) are marked stale here."""
     if not state.is_cuda:
         raise RuntimeError("adamw_step: GPU tensors only (no CPU path exists)")
-    with torch.no_grad(), torch.cuda.device(state.device):
+    with ops.device_guard(state):
         ops.adamw_step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), state, lr, betas[0], betas[1], eps,
                        weight_decay, seed, found_inf, grad_scale, shadows, step_offsets)
         ops.touch(params)
@@ -956,6 +956,6 @@ def adamw_moments(exp_avgs, exp_avg_sqs, out=None):
     if out[0]:
         if not out[0][0].is_cuda:
             raise RuntimeError("adamw_moments: GPU tensors only (no CPU path exists)")
-        with torch.cuda.device(out[0][0].device):
+        with ops.device_guard(out[0][0]):
             ops.adamw_moments(list(exp_avgs), list(exp_avg_sqs), list(out[0]), list(out[1]))
     return out

@@ -7,6 +7,7 @@ missing or a tensor is not on the GPU the call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import List, Optional, Sequence
@@ -77,6 +78,17 @@ def lib():
         L.sf_layer_norm_bwd_workspace_bytes.restype = ctypes.c_size_t
         L.sf_diff_attn_fwd_workspace_bytes.restype = ctypes.c_size_t
         L.sf_diff_attn_bwd_workspace_bytes.restype = ctypes.c_size_t
+        # with the argument types declared, tensors' addresses are passed as plain ints (a small layer's call is host bound)
+        vp, sz, ull = _c_vp, ctypes.c_size_t, ctypes.c_ulonglong
+        L.sf_adam_begin.argtypes = [vp] * 3
+        L.sf_layer_norm_fwd.argtypes = [vp] * 8 + [_c_ll, _c_int, _c_f, _c_int, vp]
+        L.sf_layer_norm_bwd_workspace_bytes.argtypes = [_c_ll, _c_int, _c_int]
+        L.sf_layer_norm_bwd.argtypes = [vp] * 10 + [sz, _c_ll, _c_int, _c_int, vp]
+        L.sf_diff_attn_fwd_workspace_bytes.argtypes = L.sf_diff_attn_bwd_workspace_bytes.argtypes = [vp]
+        L.sf_diff_attn_fwd.argtypes = [vp] * 10 + [sz, vp]
+        L.sf_diff_attn_bwd.argtypes = [vp] * 14 + [sz, vp]
+        L.sf_adamw_step.argtypes = [_c_int] + [vp] * 12 + [_c_int, _c_d, _c_d, _c_f, _c_f, ull, vp, vp, vp]
+        L.sf_adamw_moments.argtypes = [_c_int] + [vp] * 8
         _lib = L
     return _lib
 
@@ -103,6 +115,23 @@ def _check(rc: int, who: str):
 
 def _stream():
     return _c_vp(torch.cuda.current_stream().cuda_stream)
+
+
+def _stream_of(t: torch.Tensor) -> int:
+    """The current stream of t's device, as an address."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def device_guard(t: torch.Tensor):
+    """Makes t's device the current one, if it is not (kernels are launched on the current device)."""
+    return _NO_GUARD if torch._C._cuda_getDevice() == t.device.index else torch.cuda.device(t.device)
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -1088,8 +1117,8 @@ def attn_bwd(g, dout, ws, dws, save):
 
 # ------------------------------------------------------------------------------ layer norm
 def layer_norm_fwd(x, w, b, eps, residual=None, need_stats=False):
-    """x [..., D] f32 / bf16, w, b f32 [D] or None -> (y, s, mean, rstd): s is x, or x + residual in x's
-    dtype; the statistics are None unless wanted."""
+    """x [..., D] f32 / bf16, w, b f32 [D] or None -> (y, s, stats): s is x, or x + residual in x's
+    dtype; stats f32 [2, rows] (mean, 1 / deviation) or None."""
     _dev(x, residual, w, b, dtypes=[None, x.dtype, torch.float32, torch.float32])
     code, D = code_of(x.dtype), x.shape[-1]
     if residual is not None and residual.shape != x.shape:
@@ -1097,26 +1126,29 @@ def layer_norm_fwd(x, w, b, eps, residual=None, need_stats=False):
     rows = x.numel() // D
     y = torch.empty_like(x)
     s = torch.empty_like(x) if residual is not None else x
-    mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0) if need_stats else (None, None)
+    stats = torch.empty((2, rows), device=x.device, dtype=torch.float32) if need_stats else None
     if rows:
-        _check(lib().sf_layer_norm_fwd(_p(x), _p(residual), _p(s if residual is not None else None), _p(w), _p(b), _p(y), _p(mean),
-                                       _p(rstd), _c_ll(rows), D, _c_f(eps), code, _stream()), "sf_layer_norm_fwd")
-    return y, s, mean, rstd
+        mean = _at(stats)
+        _check(lib().sf_layer_norm_fwd(x.data_ptr(), _at(residual), None if residual is None else s.data_ptr(), _at(w), _at(b),
+                                       y.data_ptr(), mean, None if mean is None else mean + 4 * rows, rows, D, eps, code,
+                                       _stream_of(x)), "sf_layer_norm_fwd")
+    return y, s, stats
 
 
-def layer_norm_bwd(dy, dsum, s, w, mean, rstd, need_dw=True, need_db=True):
+def layer_norm_bwd(dy, dsum, s, w, stats, need_dw=True, need_db=True):
     """(dx, dw, db); dsum: the gradient arriving at the sum, or None."""
-    _dev(dy, dsum, s, w, mean, rstd, dtypes=[s.dtype, s.dtype, None, torch.float32, torch.float32, torch.float32])
+    _dev(dy, dsum, s, w, stats, dtypes=[s.dtype, s.dtype, None, torch.float32, torch.float32])
     D = s.shape[-1]
     rows, code = s.numel() // D, code_of(s.dtype)
     dx = torch.empty_like(s)
     dw, db = ((torch.empty if rows else torch.zeros)(D, device=s.device, dtype=torch.float32) if want else None
               for want in (need_dw, need_db))
     if rows:
-        nb = int(lib().sf_layer_norm_bwd_workspace_bytes(_c_ll(rows), D, code)) if need_dw or need_db else 0
+        nb = lib().sf_layer_norm_bwd_workspace_bytes(rows, D, code) if need_dw or need_db else 0
         ws = torch.empty(nb, device=s.device, dtype=torch.uint8) if nb else None
-        _check(lib().sf_layer_norm_bwd(_p(dy), _p(dsum), _p(s), _p(w), _p(mean), _p(rstd), _p(dx), _p(dw), _p(db), _p(ws),
-                                       ctypes.c_size_t(nb), _c_ll(rows), D, code, _stream()), "sf_layer_norm_bwd")
+        mean = stats.data_ptr()
+        _check(lib().sf_layer_norm_bwd(dy.data_ptr(), _at(dsum), s.data_ptr(), _at(w), mean, mean + 4 * rows, dx.data_ptr(), _at(dw),
+                                       _at(db), _at(ws), nb, rows, D, code, _stream_of(s)), "sf_layer_norm_bwd")
     return dx, dw, db
 
 
@@ -1125,15 +1157,16 @@ def _token_strides(t: torch.Tensor):
     """(sample, token, head) strides of [B, T, heads, .. one head contiguous ..] as the kernels take them, or None when
     the layout has to be copied first: halves and values not contiguous, a token step below a head, pieces
     that are not whole 16 bytes.  Axes of length one get the stride of a contiguous tensor."""
+    shape, strides = t.shape, t.stride()
     width = 1
-    for n, st in zip(reversed(t.shape[3:]), reversed(t.stride()[3:])):
+    for n, st in zip(shape[:2:-1], strides[:2:-1]):
         if n != 1 and st != width:
             return None
         width *= n
-    B, T, H = t.shape[:3]
-    sh = t.stride(2) if H != 1 else width
-    st = t.stride(1) if T != 1 else H * width
-    sb = t.stride(0) if B != 1 else T * H * width
+    B, T, H = shape[:3]
+    sh = strides[2] if H != 1 else width
+    st = strides[1] if T != 1 else H * width
+    sb = strides[0] if B != 1 else T * H * width
     unit = 16 // t.element_size()
     if sh % unit or st % unit or sb % unit or t.data_ptr() % 16 or st < width or st >= 1 << 22:
         return None
@@ -1147,40 +1180,43 @@ def kernel_layout(t: torch.Tensor) -> torch.Tensor:
 
 def _diff_attn_desc(q, k, v, lam, causal, scale):
     B, Tq, H, _, d = q.shape
-    strides = [_token_strides(t) for t in (q, k, v)]
-    if None in strides:
+    qs, ks, vs = _token_strides(q), _token_strides(k), _token_strides(v)
+    if qs is None or ks is None or vs is None:
         raise RuntimeError("diff_attention: a layout the kernels cannot read (see kernel_layout)")
-    return DiffAttnDesc(code_of(q.dtype), code_of(lam.dtype), B, Tq, k.shape[1], H, k.shape[2], d, int(causal), scale,
-                        *[(_c_ll * 3)(*s) for s in strides])
+    return DiffAttnDesc(code_of(q.dtype), code_of(lam.dtype), B, Tq, k.shape[1], H, k.shape[2], d, int(causal), scale, qs, ks, vs)
 
 
 def diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need_save=False):
-    """q [B,Tq,H,2,d], k [B,Tk,Hk,2,d], v [B,Tk,Hk,2d], lam [H] -> (o [B,Tq,H,2d], maps, lse); maps and lse (what the
-    backward pass needs) are None unless wanted."""
+    """q [B,Tq,H,2,d], k [B,Tk,Hk,2,d], v [B,Tk,Hk,2d], lam [H] -> (o [B,Tq,H,2d], saved): saved (what the
+    backward pass needs) is None unless wanted."""
     B, Tq, H, _, d = q.shape
     o = torch.empty((B, Tq, H, 2 * d), device=q.device, dtype=q.dtype)
-    maps = torch.empty((B, Tq, H, 2, 2 * d), device=q.device, dtype=torch.float32) if need_save else None
-    lse = torch.empty((B, H, Tq, 2), device=q.device, dtype=torch.float32) if need_save else None
     if o.numel() == 0 or k.numel() == 0:        # no query, or no key for anyone
-        return o.zero_(), maps, lse
+        return o.zero_(), None
     desc = _diff_attn_desc(q, k, v, lam, causal, scale)
-    nb = int(lib().sf_diff_attn_fwd_workspace_bytes(ctypes.byref(desc)))
+    at = ctypes.addressof(desc)
+    maps = lse = None
+    if need_save:
+        maps = torch.empty((B, Tq, H, 2, 2 * d), device=q.device, dtype=torch.float32)
+        lse = torch.empty((B, H, Tq, 2), device=q.device, dtype=torch.float32)
+    nb = lib().sf_diff_attn_fwd_workspace_bytes(at)
     ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
-    _check(lib().sf_diff_attn_fwd(ctypes.byref(desc), _p(q), _p(k), _p(v), _p(lam), _p(lengths), _p(o), _p(maps), _p(lse), _p(ws),
-                                  ctypes.c_size_t(nb), _stream()), "sf_diff_attn_fwd")
-    return o, maps, lse
+    _check(lib().sf_diff_attn_fwd(at, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _at(lengths), o.data_ptr(),
+                                  _at(maps), _at(lse), _at(ws), nb, _stream_of(q)), "sf_diff_attn_fwd")
+    return o, (desc, maps, lse)
 
 
-def diff_attn_bwd(q, k, v, lam, lengths, causal, scale, maps, lse, do, need_dlam=True):
-    """(dq, dk, dv, dlam), contiguous."""
+def diff_attn_bwd(q, k, v, lam, lengths, desc, maps, lse, do, need_dlam=True):
+    """(dq, dk, dv, dlam), contiguous; desc, maps, lse: what diff_attn_fwd saved for the same q, k, v, lam, lengths."""
     _dev(maps, lse, do, dtypes=[torch.float32, torch.float32, q.dtype])
     dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
     dlam = torch.empty_like(lam) if need_dlam else None
-    desc = _diff_attn_desc(q, k, v, lam, causal, scale)
-    nb = int(lib().sf_diff_attn_bwd_workspace_bytes(ctypes.byref(desc)))
+    at = ctypes.addressof(desc)
+    nb = lib().sf_diff_attn_bwd_workspace_bytes(at)
     ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
-    _check(lib().sf_diff_attn_bwd(ctypes.byref(desc), _p(q), _p(k), _p(v), _p(lam), _p(lengths), _p(maps), _p(lse), _p(do), _p(dq),
-                                  _p(dk), _p(dv), _p(dlam), _p(ws), ctypes.c_size_t(nb), _stream()), "sf_diff_attn_bwd")
+    _check(lib().sf_diff_attn_bwd(at, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _at(lengths), maps.data_ptr(),
+                                  lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(dlam), ws.data_ptr(),
+                                  nb, _stream_of(q)), "sf_diff_attn_bwd")
     return dq, dk, dv, dlam
 
 
@@ -1320,24 +1356,35 @@ def adam_guarded(p, g, m, v, lr, beta1, beta2, eps, state, found_inf=None, grad_
 ADAMW_BLOCK = 256   # SF_ADAMW_BLOCK: elements that share a block exponent in 8-bit moments
 
 
-def _adamw_moment_lists(ms, vs, numels, who):
-    """(state bits, moment tensors, exponent tensors or None) of lists of f32 tensors or (codes, exponents) pairs."""
-    bits8 = len(ms) > 0 and isinstance(ms[0], (tuple, list))
-    for x, n in zip(list(ms) + list(vs), list(numels) * 2):
-        if isinstance(x, (tuple, list)) != bits8:
-            raise TypeError(f"{who}: f32 and 8-bit moments cannot be mixed in one call")
-        if bits8:
-            _dev(*x, dtypes=[torch.uint8, torch.uint8])
-            if x[0].numel() != n or x[1].numel() != -(-n // ADAMW_BLOCK):
-                raise RuntimeError(f"{who}: {n} elements need {n} codes and {-(-n // ADAMW_BLOCK)} block exponents, "
-                                   f"got {x[0].numel()} and {x[1].numel()}")
-        else:
-            _dev(x, dtypes=[torch.float32])
-            if x.numel() != n:
-                raise RuntimeError(f"{who}: a moment of {x.numel()} elements for a parameter of {n}")
-    if not bits8:
-        return 32, ms, vs, None, None
-    return 8, [x[0] for x in ms], [x[0] for x in vs], [x[1] for x in ms], [x[1] for x in vs]
+def _flat_addresses(ts, numels, index, what, dtype=torch.float32):
+    """Addresses of contiguous tensors of the wanted type, sizes and device."""
+    out = []
+    for i, (t, n) in enumerate(zip(ts, numels)):
+        if t.dtype is not dtype:
+            raise TypeError(f"{what} {i}: expected {dtype}, got {t.dtype}")
+        if t.numel() != n:
+            raise RuntimeError(f"{what} {i} has {t.numel()} elements, {n} are wanted")
+        if t.get_device() != index:
+            raise RuntimeError(f"{what} {i} is on {t.device}, not on GPU {index} with the others")
+        if not t.is_contiguous():
+            raise RuntimeError(f"{what} {i}: streamflow HIP ops need contiguous tensors")
+        out.append(t.data_ptr())
+    return out
+
+
+def _moment_addresses(ms, numels, index, what):
+    """(codes or f32 values, block exponents or None) of a list of f32 tensors or (codes, exponents) pairs."""
+    pairs = sum(isinstance(x, (tuple, list)) for x in ms)
+    if not pairs:
+        return _flat_addresses(ms, numels, index, what), None
+    if pairs != len(ms):
+        raise TypeError(f"{what}s: f32 and 8-bit moments cannot be mixed in one call")
+    return (_flat_addresses([x[0] for x in ms], numels, index, what + " codes", torch.uint8),
+            _flat_addresses([x[1] for x in ms], [-(-n // ADAMW_BLOCK) for n in numels], index, what + " block exponents", torch.uint8))
+
+
+def _pointers(values):
+    return None if values is None else (_c_vp * len(values))(*values)
 
 
 def adamw_step(ps, gs, ms, vs, state, lr, beta1, beta2, eps, weight_decay, seed=0, found_inf=None, grad_scale=1.0, shadows=None,
@@ -1345,49 +1392,47 @@ def adamw_step(ps, gs, ms, vs, state, lr, beta1, beta2, eps, weight_decay, seed=
     """One AdamW update of the tensors `ps`: the checks, then sf_adam_begin, then sf_adamw_step.  lr and
     weight_decay: one number, or one per tensor."""
     n = len(ps)
+    lrs = lr if isinstance(lr, (list, tuple)) else [lr] * n
+    wds = weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
     for name, seq in (("gradients", gs), ("first moments", ms), ("second moments", vs), ("shadows", shadows),
-                      ("step offsets", step_offsets), ("lr", lr if isinstance(lr, (list, tuple)) else None),
-                      ("weight_decay", weight_decay if isinstance(weight_decay, (list, tuple)) else None)):
+                      ("step offsets", step_offsets), ("lr", lrs), ("weight_decay", wds)):
         if seq is not None and len(seq) != n:
             raise RuntimeError(f"adamw_step: {len(seq)} {name} for {n} parameters")
     _dev(state, found_inf, dtypes=[torch.int32, torch.int32])
-    if state.numel() != 2:
-        raise RuntimeError("adamw_step: state is int32 [2]: steps taken, steps skipped")
-    _dev(*ps, dtypes=[torch.float32] * n)
-    _dev(*gs)
-    codes = [code_of(g.dtype) for g in gs]
-    dev = state.device
-    for i, (p, g) in enumerate(zip(ps, gs)):
-        if g.numel() != p.numel():
-            raise RuntimeError(f"adamw_step: gradient {i} has {g.numel()} elements, its parameter {p.numel()}")
-        if p.device != dev or g.device != dev:
-            raise RuntimeError(f"adamw_step: tensor {i} is on {p.device} / {g.device}, the state on {dev}")
+    index = state.get_device()
+    if state.numel() != 2 or (found_inf is not None and found_inf.get_device() != index):
+        raise RuntimeError("adamw_step: state is int32 [2]: steps taken, steps skipped; found_inf lies on the same device")
     numels = [p.numel() for p in ps]
-    if len({p.data_ptr() for p in ps if p.numel()}) != sum(1 for k in numels if k):
+    p_at = _flat_addresses(ps, numels, index, "adamw_step: parameter")
+    codes, g_at = [], []
+    for i, (g, k) in enumerate(zip(gs, numels)):
+        codes.append(code_of(g.dtype))
+        if g.numel() != k or g.get_device() != index or not g.is_contiguous():
+            raise RuntimeError(f"adamw_step: gradient {i} of {g.numel()} elements on {g.device} does not fit its parameter of {k} on "
+                               f"GPU {index}, or is not contiguous")
+        g_at.append(g.data_ptr())
+    if len(set(p_at)) != n and len({a for a, k in zip(p_at, numels) if k}) != sum(1 for k in numels if k):
         raise RuntimeError("adamw_step: the same parameter is listed twice")
+    sh_at = None
     if shadows is not None:
-        for i, s in enumerate(shadows):
-            _dev(s, dtypes=[torch.bfloat16])
-            if s is not None and s.numel() != numels[i]:
-                raise RuntimeError(f"adamw_step: shadow {i} has {s.numel()} elements, its parameter {numels[i]}")
-    bits, ms, vs, me, ve = _adamw_moment_lists(ms, vs, numels, "adamw_step")
+        sh_at = [None if s is None else _flat_addresses([s], [k], index, f"adamw_step: shadow {i},", torch.bfloat16)[0]
+                 for i, (s, k) in enumerate(zip(shadows, numels))]
+    m_at, me_at = _moment_addresses(ms, numels, index, "adamw_step: first moment")
+    v_at, ve_at = _moment_addresses(vs, numels, index, "adamw_step: second moment")
+    if (me_at is None) != (ve_at is None):
+        raise TypeError("adamw_step: f32 and 8-bit moments cannot be mixed in one call")
     if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and eps >= 0.0):
         raise ValueError(f"adamw_step: betas ({beta1}, {beta2}) must lie in [0, 1), eps ({eps}) must not be negative")
     if step_offsets is not None and any(o > 0 for o in step_offsets):
         raise ValueError("adamw_step: step offsets are not positive")
-    adam_begin(state, found_inf)
+    stream = _stream_of(state)
+    _check(lib().sf_adam_begin(state.data_ptr(), _at(found_inf), stream), "sf_adam_begin")
     if n == 0:
         return
-    lrs = lr if isinstance(lr, (list, tuple)) else [lr] * n
-    wds = weight_decay if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
-    sh = None if shadows is None else (_c_vp * n)(*[None if s is None else s.data_ptr() for s in shadows])
-    _check(lib().sf_adamw_step(n, _ptr_array(ps), _ptr_array(gs), _ptr_array(ms), _ptr_array(vs),
-                               None if me is None else _ptr_array(me), None if ve is None else _ptr_array(ve), sh,
-                               (_c_ll * n)(*numels), (_c_d * n)(*lrs), (_c_d * n)(*wds),
-                               (_c_int * n)(*codes),
-                               None if step_offsets is None else (_c_int * n)(*step_offsets), bits, _c_d(beta1), _c_d(beta2),
-                               _c_f(eps), _c_f(grad_scale), ctypes.c_ulonglong(seed), _p(state), _p(found_inf), _stream()),
-           "sf_adamw_step")
+    _check(lib().sf_adamw_step(n, _pointers(p_at), _pointers(g_at), _pointers(m_at), _pointers(v_at), _pointers(me_at), _pointers(ve_at),
+                               _pointers(sh_at), (_c_ll * n)(*numels), (_c_d * n)(*lrs), (_c_d * n)(*wds), (_c_int * n)(*codes),
+                               None if step_offsets is None else (_c_int * n)(*step_offsets), 32 if me_at is None else 8, beta1, beta2,
+                               eps, grad_scale, seed, state.data_ptr(), _at(found_inf), stream), "sf_adamw_step")
 
 
 def adamw_moments(ms, vs, outs_m, outs_v):
@@ -1395,17 +1440,16 @@ def adamw_moments(ms, vs, outs_m, outs_v):
     n = len(ms)
     if not (len(vs) == len(outs_m) == len(outs_v) == n):
         raise RuntimeError("adamw_moments: lists of different lengths")
-    numels = [o.numel() for o in outs_m]
-    _dev(*outs_m, *outs_v, dtypes=[torch.bfloat16] * (2 * n))
-    if [o.numel() for o in outs_v] != numels:
-        raise RuntimeError("adamw_moments: outputs of different sizes")
     if n == 0:
         return
-    bits, ms, vs, me, ve = _adamw_moment_lists(ms, vs, numels, "adamw_moments")
-    if bits != 8:
+    index, numels = outs_m[0].get_device(), [o.numel() for o in outs_m]
+    to = [_flat_addresses(o, numels, index, "adamw_moments: output", torch.bfloat16) for o in (outs_m, outs_v)]
+    m_at, me_at = _moment_addresses(ms, numels, index, "adamw_moments: first moment")
+    v_at, ve_at = _moment_addresses(vs, numels, index, "adamw_moments: second moment")
+    if me_at is None or ve_at is None:
         raise TypeError("adamw_moments: f32 moments are their own values")
-    _check(lib().sf_adamw_moments(n, _ptr_array(ms), _ptr_array(vs), _ptr_array(me), _ptr_array(ve), _ptr_array(outs_m),
-                                  _ptr_array(outs_v), (_c_ll * n)(*numels), _stream()), "sf_adamw_moments")
+    _check(lib().sf_adamw_moments(n, _pointers(m_at), _pointers(v_at), _pointers(me_at), _pointers(ve_at), _pointers(to[0]),
+                                  _pointers(to[1]), (_c_ll * n)(*numels), _stream_of(outs_m[0])), "sf_adamw_moments")
 
 
 def nan_inf_flag(x: torch.Tensor, flag: torch.Tensor):
