@@ -23,10 +23,10 @@
 namespace {
 
 constexpr int NT = 256;
-constexpr int CHUNK = 4096;        // elements of a workgroup: 16 per thread, four 16-byte pieces in flight per array
+constexpr int CHUNK = 4096;        // elements of a workgroup: 16 per thread
 constexpr int BLOCK = SF_ADAMW_BLOCK;
 constexpr int MAX_TENSORS = 40;    // tensors of one launch: their table stays below 4 KB of kernel arguments
-static_assert(BLOCK == 256 && CHUNK % (BLOCK * (NT / 64)) == 0, "one wave handles one block of moments per piece");
+static_assert(BLOCK == 8 * 32 && CHUNK % (8 * NT) == 0, "32 lanes hold a block of moments");
 
 struct Tensor {
     float* p;
@@ -47,26 +47,28 @@ struct Table { Tensor t[MAX_TENSORS]; };
 struct Hyper { double beta1, beta2; float eps, grad_scale; unsigned seed_lo, seed_hi; int count; };
 static_assert(sizeof(Table) + sizeof(Hyper) + 16 <= 4096, "kernel arguments");
 
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Four { T e[4]; };
+// V elements at an address aligned to one element only: the hardware serves wide global accesses at any element alignment
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Some { T e[V]; };
 
-template <typename T> __device__ __forceinline__ Four<T> load4(const T* p, long long i, int have) {
-    Four<T> r{};
-    if (have == 4) {
-        r = *reinterpret_cast<const Four<T>*>(p + i);
+// WHOLE: the workgroup's elements all exist, otherwise the first `have` of the V do (the others read as zero)
+template <bool WHOLE, int V, typename T> __device__ __forceinline__ Some<T, V> load_some(const T* p, int have) {
+    Some<T, V> r{};
+    if constexpr (WHOLE) {
+        r = *reinterpret_cast<const Some<T, V>*>(p);
     } else {
 #pragma unroll
-        for (int j = 0; j < 3; ++j)
-            if (j < have) r.e[j] = p[i + j];
+        for (int j = 0; j < V; ++j)
+            if (j < have) r.e[j] = p[j];
     }
     return r;
 }
-template <typename T> __device__ __forceinline__ void store4(T* p, long long i, int have, const Four<T>& v) {
-    if (have == 4) {
-        *reinterpret_cast<Four<T>*>(p + i) = v;
+template <bool WHOLE, int V, typename T> __device__ __forceinline__ void store_some(T* p, int have, const Some<T, V>& v) {
+    if constexpr (WHOLE) {
+        *reinterpret_cast<Some<T, V>*>(p) = v;
     } else {
 #pragma unroll
-        for (int j = 0; j < 3; ++j)
-            if (j < have) p[i + j] = v.e[j];
+        for (int j = 0; j < V; ++j)
+            if (j < have) p[j] = v.e[j];
     }
 }
 
@@ -88,13 +90,20 @@ __host__ __device__ __forceinline__ unsigned mix(unsigned x) {
     return x ^ (x >> 16);
 }
 
-__device__ __forceinline__ unsigned wave_max_u(unsigned v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned u = (unsigned)__shfl_xor((int)v, o, 64);
-        v = v > u ? v : u;
-    }
-    return v;
+// largest value among the 32 lanes of a half wave, in all of them: rotations within 16 lanes, then the two sixteens
+// change places (vector instructions only, no trip through LDS)
+__device__ __forceinline__ unsigned half_wave_max(unsigned v) {
+    const auto turned = [](unsigned x, auto ctrl) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl.value, 0xf, 0xf, false); };
+    unsigned t = turned(v, std::integral_constant<int, 0x128>{});      // row_ror:8
+    v = v > t ? v : t;
+    t = turned(v, std::integral_constant<int, 0x124>{});
+    v = v > t ? v : t;
+    t = turned(v, std::integral_constant<int, 0x122>{});
+    v = v > t ? v : t;
+    t = turned(v, std::integral_constant<int, 0x121>{});
+    v = v > t ? v : t;
+    const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return s[0] > s[1] ? s[0] : s[1];
 }
 
 // f32 value of a code under block exponent e; SIGNED: first moment
@@ -131,103 +140,85 @@ __device__ __forceinline__ int tensor_of(const Table& tab, int count, int bid) {
     return __builtin_amdgcn_readfirstlane(__popcll(__ballot(before)) - 1);
 }
 
-template <int BITS>
-__global__ __launch_bounds__(NT) void adamw_kernel(Table tab, Hyper h, const int* __restrict__ state,
-                                                   const int* __restrict__ found_inf) {
-    if (found_inf && found_inf[0] != 0) return;
-    const Tensor& T = tab.t[tensor_of(tab, h.count, blockIdx.x)];
-    const long long n = T.n, c0 = (long long)(blockIdx.x - T.first) * CHUNK;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    constexpr int U = CHUNK / (4 * NT);
-    const int t_all = state[0], t = max(t_all + T.step_offset, 1);
+// One workgroup's 4096 elements.  BITS 32: a thread takes 4 consecutive elements at a time; BITS 8: 8, so that 32 lanes
+// hold a block of moments.
+template <int BITS, bool WHOLE, typename G>
+__device__ __forceinline__ void adamw_chunk(const Tensor& T, const Hyper& h, long long c0, int t_all) {
+    constexpr int V = BITS == 32 ? 4 : 8, U = CHUNK / (V * NT);
     const float b1 = (float)h.beta1, b2 = (float)h.beta2, a1 = (float)(1.0 - h.beta1), a2 = (float)(1.0 - h.beta2);
     long long at[U];
     int have[U];
-    Four<float> p[U], m[U], v[U];
-    Four<float> g[U];
+    Some<float, V> p[U], m[U], v[U];
+    Some<G, V> g[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        at[u] = c0 + u * (4 * NT) + wave * BLOCK + lane * 4;
-        const long long left = n - at[u];
-        have[u] = left >= 4 ? 4 : left > 0 ? (int)left : 0;
+        at[u] = c0 + u * (V * NT) + threadIdx.x * V;
+        const long long left = T.n - at[u];
+        have[u] = left >= V ? V : left > 0 ? (int)left : 0;
+        g[u] = load_some<WHOLE, V>((const G*)T.g + at[u], have[u]);
+        p[u] = load_some<WHOLE, V>(T.p + at[u], have[u]);
     }
-    if (T.g_bf16) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const Four<bf16> r = load4((const bf16*)T.g, at[u], have[u]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) g[u].e[j] = (float)r.e[j];
-        }
-    } else {
-#pragma unroll
-        for (int u = 0; u < U; ++u) g[u] = load4((const float*)T.g, at[u], have[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) p[u] = load4(T.p, at[u], have[u]);
     if constexpr (BITS == 32) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            m[u] = load4((const float*)T.m, at[u], have[u]);
-            v[u] = load4((const float*)T.v, at[u], have[u]);
+            m[u] = load_some<WHOLE, V>((const float*)T.m + at[u], have[u]);
+            v[u] = load_some<WHOLE, V>((const float*)T.v + at[u], have[u]);
         }
     } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const Four<unsigned char> cm = load4((const unsigned char*)T.m, at[u], have[u]);
-            const Four<unsigned char> cv = load4((const unsigned char*)T.v, at[u], have[u]);
-            const int em = have[u] ? T.me[at[u] / BLOCK] : 16, ev = have[u] ? T.ve[at[u] / BLOCK] : 32;
+            const auto cm = load_some<WHOLE, V>((const unsigned char*)T.m + at[u], have[u]);
+            const auto cv = load_some<WHOLE, V>((const unsigned char*)T.v + at[u], have[u]);
+            const int em = WHOLE || have[u] ? T.me[at[u] / BLOCK] : 16, ev = WHOLE || have[u] ? T.ve[at[u] / BLOCK] : 32;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < V; ++j) {
                 m[u].e[j] = decode<true>(cm.e[j], em);
                 v[u].e[j] = decode<false>(cv.e[j], ev);
             }
         }
     }
+    const int t = max(t_all + T.step_offset, 1);
     const float step = (float)((double)T.lr / (1.0 - power(h.beta1, t)));
     const float root = (float)(1.0 / sqrt(1.0 - power(h.beta2, t)));
-    const float keep = T.keep;
     unsigned key = 0;
     if constexpr (BITS == 8) key = mix(mix((h.seed_lo + (unsigned)t_all * 0x9E3779B1u) ^ h.seed_hi) + (unsigned)T.ordinal * 0x85EBCA6Bu);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+        unsigned mm = 0, mv = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float gs = g[u].e[j] * h.grad_scale;
+        for (int j = 0; j < V; ++j) {
+            const float gs = to_f32(g[u].e[j]) * h.grad_scale;
             m[u].e[j] = b1 * m[u].e[j] + a1 * gs;
             v[u].e[j] = b2 * v[u].e[j] + a2 * gs * gs;
-            p[u].e[j] = p[u].e[j] * keep - step * (m[u].e[j] / (sqrtf(v[u].e[j]) * root + h.eps));
+            p[u].e[j] = p[u].e[j] * T.keep - step * (m[u].e[j] / (sqrtf(v[u].e[j]) * root + h.eps));
+            // (elements behind the tensor's end hold zero: nothing was loaded)
+            const unsigned bm = __float_as_uint(m[u].e[j]) & 0x7FFFFFFFu, bv = __float_as_uint(v[u].e[j]) & 0x7FFFFFFFu;
+            mm = mm > bm ? mm : bm;
+            mv = mv > bv ? mv : bv;
         }
-        store4(T.p, at[u], have[u], p[u]);
+        store_some<WHOLE, V>(T.p + at[u], have[u], p[u]);
         if (T.shadow) {
-            Four<bf16> s;
+            Some<bf16, V> s;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s.e[j] = (bf16)p[u].e[j];
-            store4(T.shadow, at[u], have[u], s);
+            for (int j = 0; j < V; ++j) s.e[j] = (bf16)p[u].e[j];
+            store_some<WHOLE, V>(T.shadow + at[u], have[u], s);
         }
         if constexpr (BITS == 32) {
-            store4((float*)T.m, at[u], have[u], m[u]);
-            store4((float*)T.v, at[u], have[u], v[u]);
+            store_some<WHOLE, V>((float*)T.m + at[u], have[u], m[u]);
+            store_some<WHOLE, V>((float*)T.v + at[u], have[u], v[u]);
         } else {
-            // elements behind the tensor's end hold zero here (nothing was loaded) and take no part
-            unsigned mm = 0, mv = 0;
+            const int em = block_exponent<true>(half_wave_max(mm)), ev = block_exponent<false>(half_wave_max(mv));
+            Some<unsigned char, V> cm, cv;
+            const unsigned base = (unsigned)at[u] * 0x9E3779B1u + (unsigned)(at[u] >> 32) * 0xC2B2AE35u + key;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const unsigned bm = __float_as_uint(m[u].e[j]) & 0x7FFFFFFFu, bv = __float_as_uint(v[u].e[j]) & 0x7FFFFFFFu;
-                mm = mm > bm ? mm : bm;
-                mv = mv > bv ? mv : bv;
-            }
-            const int em = block_exponent<true>(wave_max_u(mm)), ev = block_exponent<false>(wave_max_u(mv));
-            Four<unsigned char> cm, cv;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const unsigned long long i = (unsigned long long)at[u] + j;
-                const unsigned r = mix((unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0xC2B2AE35u + key);
+            for (int j = 0; j < V; ++j) {       // (the upper half of the index is the same for all: V divides 2^32)
+                const unsigned r = mix(base + (unsigned)j * 0x9E3779B1u);
                 cm.e[j] = (unsigned char)encode<true>(m[u].e[j], em, r >> 16);
                 cv.e[j] = (unsigned char)encode<false>(v[u].e[j], ev, r & 0xFFFFu);
             }
-            store4((unsigned char*)T.m, at[u], have[u], cm);
-            store4((unsigned char*)T.v, at[u], have[u], cv);
-            if (lane == 0 && have[u]) {
+            store_some<WHOLE, V>((unsigned char*)T.m + at[u], have[u], cm);
+            store_some<WHOLE, V>((unsigned char*)T.v + at[u], have[u], cv);
+            if ((threadIdx.x & 31) == 0 && (WHOLE || have[u])) {
                 T.me[at[u] / BLOCK] = (unsigned char)em;
                 T.ve[at[u] / BLOCK] = (unsigned char)ev;
             }
@@ -235,28 +226,56 @@ __global__ __launch_bounds__(NT) void adamw_kernel(Table tab, Hyper h, const int
     }
 }
 
-// bf16 values of 8-bit moments (exact); T.p is unused, T.g / T.shadow hold the two outputs
-__global__ __launch_bounds__(NT) void adamw_moments_kernel(Table tab, int count) {
-    const Tensor& T = tab.t[tensor_of(tab, count, blockIdx.x)];
-    const long long n = T.n, c0 = (long long)(blockIdx.x - T.first) * CHUNK;
-    constexpr int U = CHUNK / (4 * NT);
+template <int BITS>
+__global__ __launch_bounds__(NT) void adamw_kernel(Table tab, Hyper h, const int* __restrict__ state,
+                                                   const int* __restrict__ found_inf) {
+    if (found_inf && found_inf[0] != 0) return;
+    const Tensor& T = tab.t[tensor_of(tab, h.count, blockIdx.x)];
+    const long long c0 = (long long)(blockIdx.x - T.first) * CHUNK;
+    const int t_all = state[0];
+    const bool whole = c0 + CHUNK <= T.n;
+    if (T.g_bf16) {
+        if (whole) adamw_chunk<BITS, true, bf16>(T, h, c0, t_all);
+        else adamw_chunk<BITS, false, bf16>(T, h, c0, t_all);
+    } else {
+        if (whole) adamw_chunk<BITS, true, float>(T, h, c0, t_all);
+        else adamw_chunk<BITS, false, float>(T, h, c0, t_all);
+    }
+}
+
+// bf16 values of 8-bit moments (exact); T.p and T.shadow hold the two outputs
+template <bool WHOLE> __device__ __forceinline__ void moments_chunk(const Tensor& T, long long c0) {
+    constexpr int V = 8, U = CHUNK / (V * NT);
+    long long at[U];
+    int have[U], em[U], ev[U];
+    Some<unsigned char, V> cm[U], cv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const long long at = c0 + u * (4 * NT) + threadIdx.x * 4, left = n - at;
-        const int have = left >= 4 ? 4 : left > 0 ? (int)left : 0;
-        if (!have) continue;
-        const Four<unsigned char> cm = load4((const unsigned char*)T.m, at, have);
-        const Four<unsigned char> cv = load4((const unsigned char*)T.v, at, have);
-        const int em = T.me[at / BLOCK], ev = T.ve[at / BLOCK];
-        Four<bf16> m, v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            m.e[j] = (bf16)decode<true>(cm.e[j], em);
-            v.e[j] = (bf16)decode<false>(cv.e[j], ev);
-        }
-        store4((bf16*)T.p, at, have, m);
-        store4(T.shadow, at, have, v);
+        at[u] = c0 + u * (V * NT) + threadIdx.x * V;
+        const long long left = T.n - at[u];
+        have[u] = left >= V ? V : left > 0 ? (int)left : 0;
+        cm[u] = load_some<WHOLE, V>((const unsigned char*)T.m + at[u], have[u]);
+        cv[u] = load_some<WHOLE, V>((const unsigned char*)T.v + at[u], have[u]);
+        em[u] = WHOLE || have[u] ? T.me[at[u] / BLOCK] : 16;
+        ev[u] = WHOLE || have[u] ? T.ve[at[u] / BLOCK] : 32;
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        Some<bf16, V> m, v;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            m.e[j] = (bf16)decode<true>(cm[u].e[j], em[u]);
+            v.e[j] = (bf16)decode<false>(cv[u].e[j], ev[u]);
+        }
+        store_some<WHOLE, V>((bf16*)T.p + at[u], have[u], m);
+        store_some<WHOLE, V>(T.shadow + at[u], have[u], v);
+    }
+}
+__global__ __launch_bounds__(NT) void adamw_moments_kernel(Table tab, int count) {
+    const Tensor& T = tab.t[tensor_of(tab, count, blockIdx.x)];
+    const long long c0 = (long long)(blockIdx.x - T.first) * CHUNK;
+    if (c0 + CHUNK <= T.n) moments_chunk<true>(T, c0);
+    else moments_chunk<false>(T, c0);
 }
 
 // splits the list into launches of at most MAX_TENSORS non-empty tensors and 2^30 workgroups

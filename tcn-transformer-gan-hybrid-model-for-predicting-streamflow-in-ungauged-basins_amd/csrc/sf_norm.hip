@@ -48,14 +48,21 @@ template <int G> __device__ __forceinline__ float row_sum(float v, float* sm) {
 // Columns of piece c of lane q: V elements from `col`.  The last piece of a row whose width V does not
 // divide is moved back to end with the row; its first `skip` elements belong to the piece before it and
 // are left out of the sums (their outputs are written twice, with the same bits).  A lane without a piece
-// works on piece 0 of the row with everything skipped.
-template <int G, int NC, int V> struct Cols {
+// works on piece 0 of the row with everything skipped.  FULL: G * NC * V is the width, nothing is ever skipped (the
+// selects that skip cost the backward pass of 4096 columns 16 us of 132).
+template <int G, int NC, int V, bool FULL> struct Cols {
     int col[NC], skip[NC];
     bool live[NC];
     __device__ __forceinline__ Cols(int q, int D) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int at = (q + c * G) * V;
+            if constexpr (FULL) {
+                col[c] = at;
+                skip[c] = 0;
+                live[c] = true;
+                continue;
+            }
             live[c] = at < D;
             col[c] = live[c] ? (at + V <= D ? at : D - V) : 0;
             skip[c] = live[c] ? at - col[c] : V;
@@ -63,7 +70,7 @@ template <int G, int NC, int V> struct Cols {
     }
 };
 
-template <typename T, int G, int NC, int V>
+template <typename T, int G, int NC, int V, bool FULL>
 __global__ __launch_bounds__(NT) void norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ res, T* __restrict__ sum,
                                                       const float* __restrict__ w, const float* __restrict__ b,
                                                       T* __restrict__ y, float* __restrict__ mean_out,
@@ -71,7 +78,7 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(const T* __restrict__ x, c
     __shared__ float sm[4];
     constexpr int RPB = NT / G;
     const int q = threadIdx.x % G;
-    const Cols<G, NC, V> C(q, D);
+    const Cols<G, NC, V, FULL> C(q, D);
     float wv[NC][V], bv[NC][V];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -130,7 +137,7 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(const T* __restrict__ x, c
     }
 }
 
-template <typename T, int G, int NC, int V>
+template <typename T, int G, int NC, int V, bool FULL>
 __global__ __launch_bounds__(NT) void norm_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ dsum,
                                                       const T* __restrict__ s, const float* __restrict__ w,
                                                       const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -139,7 +146,7 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(const T* __restrict__ dy, 
     __shared__ float sm[4];
     __shared__ float fold[G < NT ? 3 * 64 * NC * V : 1];
     const int q = threadIdx.x % G;
-    const Cols<G, NC, V> C(q, D);
+    const Cols<G, NC, V, FULL> C(q, D);
     float wv[NC][V], aw[NC][V], ab[NC][V];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -162,6 +169,11 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(const T* __restrict__ dy, 
             load_vec<T, V>(s + at + C.col[c], h[c]);
             load_vec<T, V>(dy + at + C.col[c], g[c]);
         }
+        Raw<T, V> t[NC];            // (asked for before the sums, so that it is there behind them)
+        if (dsum) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) t[c] = *reinterpret_cast<const Raw<T, V>*>(dsum + at + C.col[c]);
+        }
         float m1 = 0.f, m2 = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -180,12 +192,10 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(const T* __restrict__ dy, 
         m2 = row_sum<G>(m2, sm) * inv;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            float t[V];
-            if (dsum) load_vec<T, V>(dsum + at + C.col[c], t);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 g[c][j] = rs * (g[c][j] - m1 - h[c][j] * m2);
-                if (dsum) g[c][j] += t[j];
+                if (dsum) g[c][j] += to_f32(t[c].e[j]);
             }
             if (have && C.live[c]) store_vec<T, V>(dx + at + C.col[c], g[c]);
         }
@@ -310,23 +320,23 @@ __global__ __launch_bounds__(NT) void norm_bwd_cols_kernel(const T* __restrict__
     part[(size_t)blockIdx.y * 2 * D + D + c] = ab;
 }
 
-// dw / db = the partial rows added in order: 32 columns per workgroup, eight threads per column, each over
-// every eighth row, joined through LDS
-__global__ __launch_bounds__(NT) void norm_fold_kernel(const float* __restrict__ part, int nparts, int D,
-                                                       float* __restrict__ dw, float* __restrict__ db) {
-    __shared__ float sm[8][33];
+// dw / db = the partial rows added in order: 32 columns per workgroup, 32 threads per column, each over every 32nd row,
+// joined through LDS
+__global__ __launch_bounds__(1024) void norm_fold_kernel(const float* __restrict__ part, int nparts, int D,
+                                                         float* __restrict__ dw, float* __restrict__ db) {
+    __shared__ float sm[32][33];
     const int cx = threadIdx.x & 31, py = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + cx;
     float a = 0.f;
     if (c < 2 * D) {
 #pragma unroll 8
-        for (int p = py; p < nparts; p += 8) a += part[(size_t)p * 2 * D + c];
+        for (int p = py; p < nparts; p += 32) a += part[(size_t)p * 2 * D + c];
     }
     sm[py][cx] = a;
     __syncthreads();
     if (py == 0 && c < 2 * D) {
 #pragma unroll
-        for (int k = 1; k < 8; ++k) a += sm[k][cx];
+        for (int k = 1; k < 32; ++k) a += sm[k][cx];
         if (c < D) {
             if (dw) dw[c] = a;
         } else if (db) {
@@ -358,12 +368,16 @@ int norm_grid(const RowPlan& p, long long rows) {
     return (int)(want < most ? want : most);
 }
 
-// calls f(G, NC, V) as integral constants for the plan of a row
-template <typename T, typename F> bool with_plan(const RowPlan& p, F&& f) {
+// calls f(G, NC, V, FULL) as integral constants for the plan of a row
+template <typename T, typename F> bool with_plan(const RowPlan& p, int D, F&& f) {
     constexpr int V = ElemTraits<T>::EPC;
 #define SF_PLAN(g, n, v)                                                                                                    \
     if (p.G == g && p.NC == n && p.V == v) {                                                                                \
-        f(std::integral_constant<int, g>{}, std::integral_constant<int, n>{}, std::integral_constant<int, v>{});            \
+        const std::integral_constant<int, g> G_;                                                                            \
+        const std::integral_constant<int, n> N_;                                                                            \
+        const std::integral_constant<int, v> V_;                                                                            \
+        if (D == g * n * v) f(G_, N_, V_, std::true_type{});                                                                \
+        else f(G_, N_, V_, std::false_type{});                                                                              \
         return true;                                                                                                        \
     }
     SF_PLAN(8, 1, 1)
@@ -384,8 +398,8 @@ int norm_fwd(const void* x, const void* res, void* sum, const float* w, const fl
         hipLaunchKernelGGL((norm_fwd_wide_kernel<T>), dim3(grid), dim3(NT), 0, st, (const T*)x, (const T*)res, (T*)sum, w, b,
                            (T*)y, mean, rstd, rows, D, eps);
     } else {
-        const bool found = with_plan<T>(p, [&](auto g, auto n, auto v) {
-            hipLaunchKernelGGL((norm_fwd_kernel<T, g.value, n.value, v.value>), dim3(norm_grid(p, rows)), dim3(NT), 0, st,
+        const bool found = with_plan<T>(p, D, [&](auto g, auto n, auto v, auto full) {
+            hipLaunchKernelGGL((norm_fwd_kernel<T, g.value, n.value, v.value, full.value>), dim3(norm_grid(p, rows)), dim3(NT), 0, st,
                                (const T*)x, (const T*)res, (T*)sum, w, b, (T*)y, mean, rstd, rows, D, eps);
         });
         SF_REQUIRE(found, "sf_layer_norm_fwd: no kernel for D = %d", D);
@@ -414,15 +428,15 @@ int norm_bwd(const void* dy, const void* dsum, const void* s, const float* w, co
             hipLaunchKernelGGL((norm_bwd_cols_kernel<T>), dim3(ceil_div(D, NT), nparts), dim3(NT), 0, st, (const T*)dy,
                                (const T*)s, mean, rstd, pw, rows, (rows + nparts - 1) / nparts, D);
     } else {
-        const bool found = with_plan<T>(p, [&](auto g, auto n, auto v) {
-            hipLaunchKernelGGL((norm_bwd_kernel<T, g.value, n.value, v.value>), dim3(nparts), dim3(NT), 0, st, (const T*)dy,
+        const bool found = with_plan<T>(p, D, [&](auto g, auto n, auto v, auto full) {
+            hipLaunchKernelGGL((norm_bwd_kernel<T, g.value, n.value, v.value, full.value>), dim3(nparts), dim3(NT), 0, st, (const T*)dy,
                                (const T*)dsum, (const T*)s, w, mean, rstd, (T*)dx, pw, rows, D);
         });
         SF_REQUIRE(found, "sf_layer_norm_bwd: no kernel for D = %d", D);
     }
     SF_LAUNCH_CHECK("sf_layer_norm_bwd");
     if (pw) {
-        hipLaunchKernelGGL(norm_fold_kernel, dim3(ceil_div(2LL * D, 32)), dim3(NT), 0, st, pw, nparts, D, dw, db);
+        hipLaunchKernelGGL(norm_fold_kernel, dim3(ceil_div(2LL * D, 32)), dim3(1024), 0, st, pw, nparts, D, dw, db);
         SF_LAUNCH_CHECK("sf_layer_norm_bwd (fold)");
     }
     return SF_OK;
