@@ -10,11 +10,11 @@ from .baselines import AttentionGRUModel, LightweightCNNReducer, PureBPModel, Pu
 from .dataset import ResidentStreamflowDataset, window_shards
 from .evaluation import Evaluator, calculate_metrics, calculate_psnr, calculate_ssim, merge_partials
 from .functional import compute_dtype, set_compute_dtype
-from .modules import (CNNEncoder, CombinedLoss, GANLoss, ImageLoss, LayerNorm, LSTMModule, PatchDiscriminator,
+from .modules import (CNNEncoder, CombinedLoss, DifferentialAttention, GANLoss, ImageLoss, LayerNorm, LSTMModule, PatchDiscriminator,
                       PositionalEncoding, SimpleUpsamplingDecoder, StationLoss, StreamflowPredictionModel,
                       TransformerModule)
 
-__all__ = ["ops", "AttentionGRUModel", "LightweightCNNReducer", "PureBPModel", "PureLSTMModel", "build_baseline_model", "ResidentStreamflowDataset", "window_shards", "compute_dtype", "set_compute_dtype", "CNNEncoder", "CombinedLoss", "GANLoss", "ImageLoss", "LayerNorm",
+__all__ = ["ops", "AttentionGRUModel", "LightweightCNNReducer", "PureBPModel", "PureLSTMModel", "build_baseline_model", "ResidentStreamflowDataset", "window_shards", "compute_dtype", "set_compute_dtype", "CNNEncoder", "CombinedLoss", "DifferentialAttention", "GANLoss", "ImageLoss", "LayerNorm",
            "LSTMModule", "PatchDiscriminator", "PositionalEncoding", "SimpleUpsamplingDecoder", "StationLoss",
            "StreamflowPredictionModel", "TransformerModule", "Evaluator", "calculate_metrics", "calculate_psnr",
            "calculate_ssim", "merge_partials"]

@@ -48,8 +48,8 @@ template <int G> __device__ __forceinline__ float row_sum(float v, float* sm) {
 // Columns of piece c of lane q: V elements from `col`.  The last piece of a row whose width V does not
 // divide is moved back to end with the row; its first `skip` elements belong to the piece before it and
 // are left out of the sums (their outputs are written twice, with the same bits).  A lane without a piece
-// works on piece 0 of the row with everything skipped.  FULL: G * NC * V is the width, nothing is ever skipped (the
-// selects that skip cost the backward pass of 4096 columns 16 us of 132).
+// works on piece 0 of the row with everything skipped.  FULL: G * NC * V is the width, nothing is ever skipped (without
+// the selects, and with dsum loaded early, the backward pass of 16384 x 4096 bf16 went from 136 to 110 us).
 template <int G, int NC, int V, bool FULL> struct Cols {
     int col[NC], skip[NC];
     bool live[NC];
@@ -347,7 +347,8 @@ __global__ __launch_bounds__(1024) void norm_fold_kernel(const float* __restrict
 
 // Which lanes hold a row of D elements: G lanes with NC pieces of V elements each, at most 32 elements per
 // lane (more and the backward pass, with four arrays of them, spills).  A wave or less while that is
-// enough, a workgroup up to D = 8192, wide = true beyond.
+// enough (a workgroup for 16 elements per lane and more was slower: bf16 rows of 2048 backward 61 us against 51), a
+// workgroup up to D = 8192, wide = true beyond.
 struct RowPlan { int G, NC, V; bool wide; };
 RowPlan row_plan(int D, int dtype) {
     const int V = D >= (dtype == SF_BF16 ? 8 : 4) ? (dtype == SF_BF16 ? 8 : 4) : 1;
@@ -355,8 +356,8 @@ RowPlan row_plan(int D, int dtype) {
     int G = 8;
     while (G < 64 && G < pieces) G *= 2;
     if (pieces > 64 * (32 / V)) G = NT;
-    int NC = 1;
-    while (NC * G < pieces) NC *= 2;
+    int NC = (pieces + G - 1) / G;
+    if (NC == 5 || NC == 7) ++NC;
     return {G, NC, V, NC * V > 32};
 }
 
@@ -381,10 +382,11 @@ template <typename T, typename F> bool with_plan(const RowPlan& p, int D, F&& f)
         return true;                                                                                                        \
     }
     SF_PLAN(8, 1, 1)
-    SF_PLAN(8, 1, V) SF_PLAN(16, 1, V) SF_PLAN(32, 1, V) SF_PLAN(64, 1, V) SF_PLAN(64, 2, V) SF_PLAN(64, 4, V)
-    SF_PLAN(NT, 4, V)
+    SF_PLAN(8, 1, V) SF_PLAN(16, 1, V) SF_PLAN(32, 1, V)
+    SF_PLAN(64, 1, V) SF_PLAN(64, 2, V) SF_PLAN(64, 3, V) SF_PLAN(64, 4, V)
+    SF_PLAN(NT, 3, V) SF_PLAN(NT, 4, V)
     if constexpr (V == 8) { SF_PLAN(NT, 2, V) }
-    if constexpr (V == 4) { SF_PLAN(64, 8, V) SF_PLAN(NT, 8, V) }
+    if constexpr (V == 4) { SF_PLAN(64, 6, V) SF_PLAN(64, 8, V) SF_PLAN(NT, 6, V) SF_PLAN(NT, 8, V) }
 #undef SF_PLAN
     return false;
 }

@@ -226,6 +226,54 @@ class LayerNorm(nn.Module):
         return SF.layer_norm(x, self.weight, self.bias, self.eps, None if residual is None else residual.to(x.dtype))
 
 
+class DifferentialAttention(nn.Module):
+    """Self-attention of [B, T, embed_dim] tokens with the difference of two softmax maps per head, for sequences of
+    any length (TransformerModule's fused layers hold at most 8 steps):
+
+        o_h = (softmax(q1 k1^T / sqrt(d)) - lam_h softmax(q2 k2^T / sqrt(d))) v,   d = embed_dim / (2 num_heads)
+        lam_h = exp(lambda_q1 . lambda_k1) - exp(lambda_q2 . lambda_k2) + lambda_init  (vectors of d values per head)
+
+    The heads' results go through a LayerNorm over their 2 d values (shared by the heads), are scaled by 1 -
+    lambda_init, as is usual to keep their size that of one softmax map's, and projected.  num_kv_heads < num_heads: groups of
+    query heads share a key / value head.  `lengths` int32 [B]: tokens of each sample, the others are not attended
+    to.  Computes in bf16 inside torch.autocast('cuda'), else in f32; the result is f32 as from the other modules."""
+
+    def __init__(self, embed_dim: int, num_heads: int, num_kv_heads: Optional[int] = None, causal: bool = False,
+                 lambda_init: float = 0.8):
+        super().__init__()
+        kv = num_heads if num_kv_heads is None else num_kv_heads
+        if embed_dim % (16 * num_heads) or embed_dim // (2 * num_heads) > 64:
+            raise NotImplementedError("DifferentialAttention: embed_dim / (2 num_heads) must be a multiple of 8 up to 64")
+        if kv < 1 or num_heads % kv:
+            raise ValueError(f"DifferentialAttention: {num_heads} heads cannot share {kv} key / value heads")
+        self.embed_dim, self.num_heads, self.num_kv_heads = embed_dim, num_heads, kv
+        self.head_dim, self.causal, self.lambda_init = embed_dim // (2 * num_heads), bool(causal), float(lambda_init)
+        width = 2 * self.head_dim
+        self.in_proj = nn.Linear(embed_dim, (num_heads + 2 * kv) * width)
+        self.out_proj = nn.Linear(num_heads * width, embed_dim)
+        self.norm = LayerNorm(width)
+        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+            self.register_parameter(name, nn.Parameter(0.1 * torch.randn(num_heads, self.head_dim)))
+
+    def lam(self) -> torch.Tensor:
+        """The weight of the second map, one per head."""
+        return (torch.exp((self.lambda_q1 * self.lambda_k1).sum(-1)) - torch.exp((self.lambda_q2 * self.lambda_k2).sum(-1))
+                + self.lambda_init)
+
+    def forward(self, x: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+        _need_cuda(x, "DifferentialAttention")
+        if x.dim() != 3 or x.shape[-1] != self.embed_dim:
+            raise RuntimeError(f"DifferentialAttention: [B, T, {self.embed_dim}] tokens, not {tuple(x.shape)}")
+        B, T, _ = x.shape
+        H, kv, d, dt = self.num_heads, self.num_kv_heads, self.head_dim, SF.compute_dtype()
+        qkv = SF.linear(x.reshape(B * T, -1), self.in_proj, dt).to(dt).view(B, T, -1)
+        q, k, v = torch.split(qkv, [H * 2 * d, kv * 2 * d, kv * 2 * d], dim=-1)
+        o = SF.diff_attention(q.view(B, T, H, 2, d), k.view(B, T, kv, 2, d), v.view(B, T, kv, 2 * d), self.lam(), self.causal,
+                              lengths=lengths)
+        o = self.norm(o) * (1.0 - self.lambda_init)
+        return SF.linear(o.reshape(B * T, -1), self.out_proj, dt).view(B, T, self.embed_dim)
+
+
 # ------------------------------------------------------------------------------ decoder
 class SimpleUpsamplingDecoder(nn.Module):
     """Mirror of src/model/decoder.py:125-177."""

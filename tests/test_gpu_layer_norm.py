@@ -98,7 +98,7 @@ def compare(sf, x, res, w, b, dy, ds, eps=1e-5):
 
 # widths around every change of layout: below one piece, pieces that end inside the row, one lane group to the
 # next, a wave's registers to a workgroup's, beyond a workgroup's registers
-WIDTHS = [1, 3, 7, 8, 9, 64, 65, 128, 129, 255, 257, 513, 1000, 1024, 2047, 2049, 4095, 8192, 8195]
+WIDTHS = [1, 3, 7, 8, 9, 64, 65, 128, 129, 255, 257, 513, 768, 1000, 1024, 1100, 1300, 1536, 2047, 2049, 4095, 4096, 5000, 6144, 8192, 8195]
 
 
 @pytest.mark.gpu
