@@ -251,6 +251,12 @@ __device__ __forceinline__ int wave_max_i(int v) {
     return __builtin_amdgcn_readfirstlane(v);
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
 // stores 4 consecutive padded columns (c a multiple of 4) of a [2, d] row
 template <typename T, int DP> __device__ __forceinline__ void store_cols(T* row, int c, int d, float x0, float x1, float x2, float x3) {
     const int half = c / DP, j = c % DP;
@@ -498,29 +504,27 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_join_k
     if (row >= rows) return;
     const int b = bh / a.Hk, t = (int)(row / group), hq = bh % a.Hk * group + (int)(row % group);
     const long long at0 = (long long)tail * a.parts * rb + id % rb;
+    // lane s holds the state of part s (there are at most 64)
     const float* const pm = a.part + (long long)items * a.parts * rb * (4 * DP);
-    float m[2] = {-1e30f, -1e30f};
-    for (int s = 0; s < a.parts; ++s) {
-        const float4 v = *reinterpret_cast<const float4*>(pm + (at0 + (long long)s * rb) * 4);
-        m[0] = fmaxf(m[0], v.x);
-        m[1] = fmaxf(m[1], v.z);
-    }
+    float4 v{-1e30f, 0.f, -1e30f, 0.f};
+    if (lane < a.parts) v = *reinterpret_cast<const float4*>(pm + (at0 + (long long)lane * rb) * 4);
+    const float m[2] = {wave_max(v.x), wave_max(v.z)};
+    const float f1 = exp2f(v.x - m[0]), f2 = exp2f(v.z - m[1]);
+    const float l[2] = {wave_sum(v.y * f1), wave_sum(v.w * f2)};
     constexpr int NCOL = (2 * DP + 63) / 64;
-    float l[2] = {0.f, 0.f}, acc[2][NCOL];
+    float acc[2][NCOL];
 #pragma unroll
     for (int n = 0; n < NCOL; ++n) acc[0][n] = acc[1][n] = 0.f;
+#pragma unroll 4
     for (int s = 0; s < a.parts; ++s) {
-        const long long at = at0 + (long long)s * rb;
-        const float4 v = *reinterpret_cast<const float4*>(pm + at * 4);
-        const float f[2] = {exp2f(v.x - m[0]), exp2f(v.z - m[1])};
-        l[0] += v.y * f[0];
-        l[1] += v.w * f[1];
+        const float* const po = a.part + (at0 + (long long)s * rb) * (4 * DP);
+        const float w1 = __shfl(f1, s, 64), w2 = __shfl(f2, s, 64);
 #pragma unroll
         for (int n = 0; n < NCOL; ++n) {
             const int c = n * 64 + lane;
             if (c < 2 * DP) {
-                acc[0][n] += a.part[at * (4 * DP) + c] * f[0];
-                acc[1][n] += a.part[at * (4 * DP) + 2 * DP + c] * f[1];
+                acc[0][n] += po[c] * w1;
+                acc[1][n] += po[2 * DP + c] * w2;
             }
         }
     }
@@ -587,11 +591,9 @@ __global__ __launch_bounds__(1024) void attn_dlam_kernel(const float* __restrict
     __shared__ double sm[16];
     const int h = blockIdx.x;
     double s = 0.0;
-    for (int b = 0; b < B; ++b) {
-        const float* const p = stat + (((long long)b * H + h) * 4 + 3) * Tp;
-#pragma unroll 4
-        for (int t = threadIdx.x; t < Tp; t += 1024) s += (double)p[t];
-    }
+    const long long n = (long long)B * Tp;
+#pragma unroll 8
+    for (long long i = threadIdx.x; i < n; i += 1024) s += (double)stat[((i / Tp * H + h) * 4 + 3) * Tp + i % Tp];
     s = wave_sum_d(s);
     if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -994,8 +996,8 @@ int check_align(const void* const* ps, int n, const char* who) {
 
 // How a launch's work items are cut.  The chip runs `slots` workgroups at a time; items beyond a whole number of rounds
 // would leave most of it idle in the last one.  Those are cut into the number of parts for which the last rounds take
-// the least time, counted in quarters of an inner tile (64 keys or 32 .. 64 query rows: about 1 us in bf16, 3 to 10 us in f32,
-// whose matrix rate is a sixteenth): what a part costs by itself, and about 10 us for the launch that joins them.
+// the least time, counted in quarters of an inner tile (about 1 us in bf16, 2 to 6 us in f32, whose matrix rate is a
+// sixteenth): what a part costs by itself, and about 10 us for the launch that joins them.
 // Causal items that fill the chip are not cut: they come longest first, the last ones are short.
 struct Cut { int full, tail, parts; };
 Cut cut_items(long long items, int slots, int tiles, bool f32, bool causal) {
@@ -1005,7 +1007,7 @@ Cut cut_items(long long items, int slots, int tiles, bool f32, bool causal) {
     int parts = 0;
     for (int p = 1; p <= 64 && (p == 1 || tiles / p >= 2); ++p) {
         const long long rounds = (tail * p + slots - 1) / slots;
-        const long long cost = rounds * (4 * ((tiles + p - 1) / p) + (f32 ? 1 : 4)) + (p > 1 ? (f32 ? 8 : 32) : 0);
+        const long long cost = rounds * (4 * ((tiles + p - 1) / p) + (f32 ? 2 : 4)) + (p > 1 ? (f32 ? 16 : 32) : 0);
         if (!parts || cost < best) { best = cost; parts = p; }
     }
     if (parts == 1) return {(int)items, 0, 1};
