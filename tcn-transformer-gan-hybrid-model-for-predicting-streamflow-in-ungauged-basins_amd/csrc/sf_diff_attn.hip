@@ -188,6 +188,10 @@ template <typename T> __device__ __forceinline__ Frag<T> global_piece(const T* r
     return f;
 }
 
+// a row's reference point before it has seen a key: every finite score is far above it, and it is itself finite, so that its
+// differences with masked scores (-inf) and with other reference points are never NaN
+constexpr float NO_SCORE = -3e38f;
+
 struct Strides { long long b, t, h; };      // elements
 template <typename T> struct Args {
     const T* q; const T* k; const T* v;
@@ -311,7 +315,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
     float m[2], l[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        m[i] = -1e30f;
+        m[i] = NO_SCORE;
         l[i] = 0.f;
 #pragma unroll
         for (int n = 0; n < DT; ++n) acc[i][n] = zero16();
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             // The reference point m of the exponentials only has to keep them in range: it moves when a lane's 16 of them
-            // add up to more than 2^12 (always at a row's first visible key, m being -1e30 before), then to the row's
+            // add up to more than 2^12 (always at a row's first visible key, m being NO_SCORE before), then to the row's
             // maximum.  The usual tile so needs no maximum, no exchange between lanes and no rescaling.
             float p[16];
             float sum = exponentials(p, s[i], m[i]);
@@ -506,7 +510,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_join_k
     const long long at0 = (long long)tail * a.parts * rb + id % rb;
     // lane s holds the state of part s (there are at most 64)
     const float* const pm = a.part + (long long)items * a.parts * rb * (4 * DP);
-    float4 v{-1e30f, 0.f, -1e30f, 0.f};
+    float4 v{NO_SCORE, 0.f, NO_SCORE, 0.f};
     if (lane < a.parts) v = *reinterpret_cast<const float4*>(pm + (at0 + (long long)lane * rb) * 4);
     const float m[2] = {wave_max(v.x), wave_max(v.z)};
     const float f1 = exp2f(v.x - m[0]), f2 = exp2f(v.z - m[1]);
@@ -986,7 +990,7 @@ int check_desc(const sf_diff_attn_desc* p, const char* who) {
         SF_REQUIRE(i % 3 != 1 || (s >= 2 * p->d && s < (1 << 22)), "%s: token stride %lld (a head has %d values)", who, s, 2 * p->d);
     }
     const double groups = (double)p->B * p->Hk * (((double)p->H / p->Hk * p->Tq + 31) / 32 + (p->Tk + 127) / 128);
-    SF_REQUIRE(groups < 1e8 && (double)p->B * p->Tq * p->H < 2e9, "%s: too many rows", who);
+    SF_REQUIRE(groups < 1e8 && (double)p->B * ((p->Tq + 63) / 64 * 64) * p->H < 2e9, "%s: too many rows", who);
     return SF_OK;
 }
 int check_align(const void* const* ps, int n, const char* who) {

@@ -10,6 +10,7 @@ import warnings
 from typing import List, Optional, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -834,6 +835,7 @@ class LayerNormFn(torch.autograd.Function):
         return (y, s) if residual is not None else y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, ds=None):
         s, w, stats = ctx.saved_tensors
         if dy is None:              # only the sum was used
@@ -848,7 +850,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
     """y = weight * (s - mean(s)) / sqrt(var(s) + eps) + bias over the last axis, for f32 or bf16 x of any
     leading shape (statistics in f32); weight and bias [D] or None.  Without a residual s = x and the result is y; with
     one, s = x + residual, rounded to x's dtype as the next layer will read it, and the result is
-    (y, s).  Differentiable in all four; the gradient of x is also that of the residual."""
+    (y, s).  Differentiable once in all four; the gradient of x is also that of the residual."""
     if not x.is_cuda:
         raise RuntimeError("layer_norm: GPU tensors only (no CPU path exists)")
     if x.dtype not in (torch.float32, torch.bfloat16):
@@ -880,6 +882,7 @@ class DiffAttentionFn(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         q, k, v, lam, lengths, maps, lse = ctx.saved_tensors
         if ctx.desc is None:
@@ -898,7 +901,7 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     the last query sees the last key.  lengths: int32 [B] on the device, the keys each sample has (the values
     are clamped to [0, Tk]; what lies behind them is never read).  A query that sees no key gives zeros.
     Sums and softmax statistics are f32; in bf16 the probabilities are rounded once for the second product.
-    Differentiable in q, k, v and lam; no atomics: equal inputs give equal bits.  Slices of one projection are
+    Differentiable once in q, k, v and lam; no atomics: equal inputs give equal bits.  Slices of one projection are
     read in place where their steps are whole 16 bytes, other layouts are copied."""
     if not (q.is_cuda and k.is_cuda and v.is_cuda and lam.is_cuda):
         raise RuntimeError("diff_attention: GPU tensors only (no CPU path exists)")
@@ -939,7 +942,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     step whose found_inf[0] is not zero changes nothing but the second count.  lr and weight_decay: one
     number, or one per tensor.  seed: of the stochastic rounding of 8-bit moments.  shadows: bf16 copies
     of the parameters to refresh (entries may be None).  The parameters are written behind torch's
-    back: copies the package derives from them (packed weights, shadows) are marked stale here."""
+    back (a graph that saved them before the step would read the new values): copies the package derives from
+    them (packed weights, shadows) are marked stale here."""
     if not state.is_cuda:
         raise RuntimeError("adamw_step: GPU tensors only (no CPU path exists)")
     with ops.device_guard(state):

@@ -1411,8 +1411,6 @@ def adamw_step(ps, gs, ms, vs, state, lr, beta1, beta2, eps, weight_decay, seed=
             raise RuntimeError(f"adamw_step: gradient {i} of {g.numel()} elements on {g.device} does not fit its parameter of {k} on "
                                f"GPU {index}, or is not contiguous")
         g_at.append(g.data_ptr())
-    if len(set(p_at)) != n and len({a for a, k in zip(p_at, numels) if k}) != sum(1 for k in numels if k):
-        raise RuntimeError("adamw_step: the same parameter is listed twice")
     sh_at = None
     if shadows is not None:
         sh_at = [None if s is None else _flat_addresses([s], [k], index, f"adamw_step: shadow {i},", torch.bfloat16)[0]
@@ -1421,6 +1419,9 @@ def adamw_step(ps, gs, ms, vs, state, lr, beta1, beta2, eps, weight_decay, seed=
     v_at, ve_at = _moment_addresses(vs, numels, index, "adamw_step: second moment")
     if (me_at is None) != (ve_at is None):
         raise TypeError("adamw_step: f32 and 8-bit moments cannot be mixed in one call")
+    written = [a for at in (p_at, m_at, v_at) for a, k in zip(at, numels) if k]
+    if len(set(written)) != len(written):
+        raise RuntimeError("adamw_step: the same parameter or moment is listed twice")
     if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and eps >= 0.0):
         raise ValueError(f"adamw_step: betas ({beta1}, {beta2}) must lie in [0, 1), eps ({eps}) must not be negative")
     if step_offsets is not None and any(o > 0 for o in step_offsets):

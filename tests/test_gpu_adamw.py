@@ -504,6 +504,9 @@ def test_gpu_refusals():
     p = z()
     with pytest.raises(RuntimeError, match="twice"):
         step([p, p], [z(), z()], [z(), z()], [z(), z()], state, 1e-3)
+    with pytest.raises(RuntimeError, match="twice"):
+        m = z()
+        step([p, z()], [z(), z()], [m, m], [z(), z()], state, 1e-3)
     with pytest.raises(RuntimeError, match="gradient 0"):
         step([p], [z(5)], [z()], [z()], state, 1e-3)
     with pytest.raises(RuntimeError, match="moment"):

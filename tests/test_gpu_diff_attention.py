@@ -197,6 +197,35 @@ def test_large_scores(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_scores_near_the_end_of_the_range(Tq):
+    """All of a row's scores are hugely negative, or hugely positive: the softmax only knows their differences.  Scores
+    of -+ 2^110 and -+ 2^111 exactly: one key takes all, in bf16 and in f32, forward and backward."""
+    sf = load_pkg()
+    for dtype in (BF, F):
+        for sign in (-1.0, 1.0):
+            q = torch.zeros(1, Tq, 1, 2, 8)
+            k = torch.zeros(1, 300, 1, 2, 8)
+            q[..., 0], k[..., 0] = sign * 2.0 ** 55, 2.0 ** 56
+            best = 77 if sign < 0 else 211
+            k[:, best, :, :, 0] = 2.0 ** 55 if sign < 0 else 2.0 ** 57
+            v = torch.randn(1, 300, 1, 16)
+            q, k, v = (t.to(dtype) for t in (q, k, v))
+            o, g = run(sf, q, k, v, torch.tensor([0.25]), torch.ones(1, Tq, 1, 16).to(dtype), scale=1.0)
+            want = (0.75 * v[:, best:best + 1].double()).expand(1, Tq, 1, 16)
+            assert bool(((o.detach().double().cpu() - want).abs() <= 2.0 ** -8 * want.abs()).all())
+            dv = g["dv"].double().cpu()
+            assert bool((dv[:, best] == 0.75 * Tq).all()) and float(dv.abs().sum()) == 0.75 * Tq * 16
+            # P is one-hot, so dP - delta is 0 in exact numbers.  In f32 both are sums of the same 16 products dO V, in orders of
+            # their own: each is off by at most 16 half steps of 2^-24 of sum |V|, their difference by 32, and two more for
+            # its own rounding and its rounding to the operand type (2^-8 of it).  It is multiplied by the key (dq) or, over
+            # the Tq rows, by the query (dk).
+            off = 34 * 2.0 ** -24 * float(v[0, best].double().abs().sum())
+            assert float(g["dq"].abs().max()) <= off * float(k[0, best].double().abs().max())
+            assert float(g["dk"].abs().max()) <= off * Tq * float(q.double().abs().max())
+
+
+@pytest.mark.gpu
 def test_lam_zero_one_negative_and_types():
     sf = load_pkg()
     q, k, v, _, do = make(2, 60, 60, 4, 4, 16, BF, seed=2)
@@ -338,6 +367,46 @@ def test_captured_forward_replays(shape):
         torch.cuda.synchronize()
         want = sf.functional.diff_attention(q, k, v, lam, lengths=lengths)
         assert torch.equal(outs[i % 2], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 100, 100, 4, 2, 64), (1, 260, 300, 2, 2, 16)], ids=str)
+def test_captured_training_pass_replays(shape):
+    """Forward and backward in one graph, replayed with other inputs, against the eager pass."""
+    sf = load_pkg()
+    for dtype in (BF, F):
+        q, k, v, lam, do = (t.cuda() for t in make(*shape, dtype, seed=12))
+
+        def passes():
+            xs = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+            o = sf.functional.diff_attention(*xs, causal=True)
+            return (o.detach(), *torch.autograd.grad(o, xs, do))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            passes()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = passes()
+        for i in range(4):
+            for t in (q, k, v, do):
+                t.copy_(torch.randn_like(t) * (1 + i))
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, y in zip(got, passes()):
+                assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_second_derivative_is_refused():
+    sf = load_pkg()
+    q, k, v, lam, do = (t.cuda() for t in make(1, 9, 9, 1, 1, 8, F))
+    q.requires_grad_(True)
+    g, = torch.autograd.grad(sf.functional.diff_attention(q, k, v, lam), q, do, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), q)
 
 
 def test_refusals():
