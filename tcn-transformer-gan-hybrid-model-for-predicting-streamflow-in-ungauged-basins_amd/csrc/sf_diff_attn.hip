@@ -68,7 +68,7 @@ __device__ __forceinline__ constexpr int acc_row(int r, int h) { return 8 * (r /
 // (pad) and the pieces of a row XORed (x), so that both 16 rows at one piece and 4 rows at 64 bytes cover the 256-byte
 // bank window once.  XOR and shift touch few bits on purpose: the rest of an address is a constant of the instruction,
 // and a lane needs 4 address registers for its row pieces and 4 for its column pieces (a full XOR of the piece index takes
-// 8 and 8, which the key gradient kernel does not have).
+// 8 and 8), or 2 and 2 from which one instruction makes each of the four (Lane).
 template <typename T, int DP> struct Tile {
     static constexpr int EPC = 16 / (int)sizeof(T);       // elements per 16-byte piece
     static constexpr int NCH = 2 * DP / EPC;
@@ -82,40 +82,46 @@ template <typename T, int DP> struct Tile {
     static __host__ __device__ __forceinline__ constexpr int pad(int g) { return NCH >= 16 ? g * 16 : NCH == 8 ? g * 32 : 0; }
     static __host__ __device__ __forceinline__ constexpr int row_off(int row) { return row * ROWB + pad(row / GROUP); }
     static constexpr int bytes(int rows) { return row_off(rows); }
-    // byte offset of piece c_const + c_lane (no common bits) of row r_const + r_lane (r_const a multiple of 16)
-    static __device__ __forceinline__ int at(int r_const, int r_lane, int c_const, int c_lane) {
-        const int lane_part = row_off(r_lane) + ((c_lane & ~XM) << 4);
-        const int mixed = ((c_const & XM) ^ ((c_lane & XM) ^ x(r_lane))) << 4;
-        return (lane_part + mixed) + (row_off(r_const) + ((c_const & ~XM) << 4));
+    // A lane's share of the byte offset of piece c_const + c_lane of row r_const + r_lane (rows and pieces: no common bits of the
+    // two, the shift and the XOR of the sum are those of its terms)
+    struct Lane { int part, mix; };
+    static __device__ __forceinline__ Lane lane_at(int r_lane, int c_lane, int byte) {
+        return {row_off(r_lane) + ((c_lane & ~XM) << 4) + byte, ((c_lane & XM) ^ x(r_lane)) << 4};
     }
-    // columns 16 n + 8 h .. + 7 of row r_const + r_lane
-    static __device__ __forceinline__ Frag<T> row_piece(lds_cptr t, int r_const, int r_lane, int n, int h) {
+    static __device__ __forceinline__ int at(Lane l, int r_const, int c_const) {
+        return (l.part + (l.mix ^ (((c_const & XM) ^ x(r_const)) << 4))) + (row_off(r_const) + ((c_const & ~XM) << 4));
+    }
+    static __device__ __forceinline__ Lane row_lane(int lane) { return lane_at(lane & 31, (lane >> 5) * (8 / EPC), 0); }
+    static __device__ __forceinline__ Lane col_lane(int lane) {
+        const int h = lane >> 5, i = lane & 15;
+        if constexpr (sizeof(T) == 2) return lane_at(4 * h + (i >> 2), 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), (i & 1) * 8);
+        else return lane_at(4 * h, (lane & 31) >> 2, (lane & 3) * 4);
+    }
+    // columns 16 n + 8 h .. + 7 of row r_const + lane % 32, h = lane / 32 (r_const a multiple of 32)
+    static __device__ __forceinline__ Frag<T> row_piece(lds_cptr t, Lane l, int r_const, int n) {
         Frag<T> f;
         if constexpr (sizeof(T) == 2) {
-            f.v = *(const SF_LDS bf16x8*)(t + at(r_const, r_lane, 2 * n, h));
+            f.v = *(const SF_LDS bf16x8*)(t + at(l, r_const, 2 * n));
         } else {
-            const f32x4 lo = *(const SF_LDS f32x4*)(t + at(r_const, r_lane, 4 * n, 2 * h));
-            const f32x4 hi = *(const SF_LDS f32x4*)(t + at(r_const, r_lane, 4 * n + 1, 2 * h));
-            #pragma unroll
+            const f32x4 lo = *(const SF_LDS f32x4*)(t + at(l, r_const, 4 * n));
+            const f32x4 hi = *(const SF_LDS f32x4*)(t + at(l, r_const, 4 * n + 1));
+#pragma unroll
             for (int j = 0; j < 4; ++j) { f.v[j] = lo[j]; f.v[4 + j] = hi[j]; }
         }
         return f;
     }
-    // column 32 n + lane % 32 of rows r_const + acc_row(0..7, lane / 32): the reduction axis is the rows, in the order the
-    // accumulators hold them
-    static __device__ __forceinline__ Frag<T> col_piece(lds_cptr t, int r_const, int n, int lane) {
-        const int h = lane >> 5;
+    // column 32 n + lane % 32 of rows r_const + acc_row(0..7, lane / 32) (r_const a multiple of 16): the reduction axis is the
+    // rows, in the order the accumulators hold them
+    static __device__ __forceinline__ Frag<T> col_piece(lds_cptr t, Lane l, int r_const, int n) {
         Frag<T> f;
         if constexpr (sizeof(T) == 2) {
-            const int i = lane & 15, row = 4 * h + (i >> 2), piece = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), byte = (i & 1) * 8;
-            const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((SF_LDS bf16x4*)(t + at(r_const, row, 4 * n, piece) + byte));
-            const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((SF_LDS bf16x4*)(t + at(r_const, row + 8, 4 * n, piece) + byte));
+            const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((SF_LDS bf16x4*)(t + at(l, r_const, 4 * n)));
+            const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((SF_LDS bf16x4*)(t + at(l, r_const + 8, 4 * n)));
 #pragma unroll
             for (int j = 0; j < 4; ++j) { f.v[j] = a[j]; f.v[4 + j] = b[j]; }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                f.v[j] = *(const SF_LDS float*)(t + at(r_const, acc_row(j, h), 8 * n, (lane & 31) >> 2) + (lane & 3) * 4);
+            for (int j = 0; j < 8; ++j) f.v[j] = *(const SF_LDS float*)(t + at(l, r_const + acc_row(j, 0), 8 * n));
         }
         return f;
     }
@@ -191,6 +197,10 @@ template <typename T> __device__ __forceinline__ Frag<T> global_piece(const T* r
 // a row's reference point before it has seen a key: every finite score is far above it, and it is itself finite, so that its
 // differences with masked scores (-inf) and with other reference points are never NaN
 constexpr float NO_SCORE = -3e38f;
+
+// waves per SIMD that a kernel's registers have to leave room for: two, so that one computes while the other loads, but where the
+// accumulators and f32 operands of 2 x 64 columns alone are more than half of them
+template <typename T, int DP> constexpr int WAVES = sizeof(T) == 4 && DP == 64 ? 1 : 2;
 
 struct Strides { long long b, t, h; };      // elements
 template <typename T> struct Args {
@@ -276,7 +286,7 @@ template <typename T, int DP> __device__ __forceinline__ void store_cols(T* row,
 // all keys of the tile.  KEYS_SPLIT true (at most 32 rows, single tokens): all waves take the same 32 rows and wave w
 // the keys 32 w .. of the tile; the waves' results are joined through LDS at the end.
 template <typename T, int DP, int NW, bool KEYS_SPLIT, int KT>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(Args<T> a) {
+__global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<T> a) {
     using L = Tile<T, DP>;
     constexpr int KS = DP / 16, DT = 2 * DP / 32;
     constexpr int RB = KEYS_SPLIT ? 32 : 32 * NW;
@@ -326,6 +336,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
     lds_ptr const buf0 = (lds_ptr)smem;
     lds_ptr const buf1 = buf0 + 2 * TB;
 
+    const typename L::Lane rl = L::row_lane(lane), cl = L::col_lane(lane);
+
     auto exponentials = [&](float* p, const f32x16& s, float ref) {
         float sum = 0.f;
 #pragma unroll
@@ -342,7 +354,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
         for (int n = 0; n < KS; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                s[i] = mma(L::row_piece(kt, sub, lane & 31, i * KS + n, h2), qf[i][n], s[i]);
+                s[i] = mma(L::row_piece(kt, rl, sub, i * KS + n), qf[i][n], s[i]);
         if (key0 + 32 > vmin) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -381,7 +393,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kern
         for (int n = 0; n < DT; ++n)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const Frag<T> vf = L::col_piece(vt, sub + 16 * u, n, lane);
+                const Frag<T> vf = L::col_piece(vt, cl, sub + 16 * u, n);
                 acc[0][n] = mma(vf, pf[0][u], acc[0][n]);
                 acc[1][n] = mma(vf, pf[1][u], acc[1][n]);
             }
@@ -610,7 +622,7 @@ __global__ __launch_bounds__(1024) void attn_dlam_kernel(const float* __restrict
 
 // Gradient of the queries: as the forward pass, 32 rows per wave, the keys tile by tile.
 template <typename T, int DP, int KT>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Args<T> a) {
+__global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a) {
     using L = Tile<T, DP>;
     constexpr int NW = 4, RB = 32 * NW, KS = DP / 16, VS = 2 * DP / 16;
     constexpr int NA = DP == 16 ? 2 : 2 * DP / 32;         // accumulators: 32 columns each (DP = 16: both halves in each)
@@ -657,6 +669,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Ar
     const Copy<T, DP, KT, NW> kc(a.ks.t, a.d), vc(a.vs.t, a.d);
     lds_ptr const buf0 = (lds_ptr)smem;
     lds_ptr const buf1 = buf0 + 2 * TB;
+    const typename L::Lane rl = L::row_lane(lane), cl = L::col_lane(lane);
 
     auto sub_tile = [&](lds_cptr kt, lds_cptr vt, int sub, int key0) {
         if (key0 >= vmax) return;
@@ -665,9 +678,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Ar
         for (int n = 0; n < KS; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                s[i] = mma(L::row_piece(kt, sub, lane & 31, i * KS + n, h2), qf[i][n], s[i]);
+                s[i] = mma(L::row_piece(kt, rl, sub, i * KS + n), qf[i][n], s[i]);
 #pragma unroll
-        for (int n = 0; n < VS; ++n) dp = mma(L::row_piece(vt, sub, lane & 31, n, h2), gf[n], dp);
+        for (int n = 0; n < VS; ++n) dp = mma(L::row_piece(vt, rl, sub, n), gf[n], dp);
         if (key0 + 32 > vmin) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -690,7 +703,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Ar
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int map = DP == 16 ? n : 32 * n / DP;
-                acc[n] = mma(L::col_piece(kt, sub + 16 * u, DP == 16 ? 0 : n, lane), df[map][u], acc[n]);
+                acc[n] = mma(L::col_piece(kt, cl, sub + 16 * u, DP == 16 ? 0 : n), df[map][u], acc[n]);
             }
     };
     auto step = [&](int i, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill) {
@@ -731,14 +744,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(Ar
 }
 
 // Gradients of the keys and values: a wave owns 32 keys, the workgroup's 128 keys meet the query rows of every head of the
-// group tile by tile.  PAIRED (bf16 heads of 2 x 64): eight waves, two for the same keys on alternate 32 rows of a 64-row tile,
-// keys and values both in LDS (one workgroup per CU); the pairs' sums are joined through LDS at the end.  With the keys in
-// registers, four waves and two workgroups per CU the 128 accumulators leave too few: the kernel spills, and a reload
-// waits for the copies under way (2 x 5120 tokens, 8 heads: KVTIME).  Not PAIRED: four waves, keys in registers.
-template <typename T, int DP, bool PAIRED>
-__global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(Args<T> a) {
+// group tile by tile.  The wave's keys stay in registers, the values in LDS.  bf16 heads of 2 x 64: with 128 accumulators and
+// 32 registers of keys little is left of the 256 that two waves per SIMD have, and a spilled one is reloaded behind the copies
+// under way.  So a lane keeps two address registers for its row pieces and two for its column pieces and makes the
+// others where it uses them (fresh), and the maps come one after the other: no spill in the loop (2 x 5120 tokens, 8 heads:
+// 725 us with 13 spills, 592 us without; eight waves in pairs, with the keys in LDS too, 635 us).
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a) {
     using L = Tile<T, DP>;
-    constexpr int NW = PAIRED ? 8 : 4, KB = 128, QT = PAIRED ? 64 : 32, KS = DP / 16, VS = 2 * DP / 16, DT = 2 * DP / 32;
+    constexpr int NW = 4, KB = 128, QT = 32, KS = DP / 16, VS = 2 * DP / 16, DT = 2 * DP / 32;
     constexpr int NA = DP == 16 ? 2 : DT;
     constexpr int TB = L::bytes(QT), SB = 1024;            // query / gradient tile; row statistics (16 QT bytes, copied by a wave)
     constexpr int BUF = 2 * TB + SB;
@@ -750,11 +764,10 @@ __global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void at
     int bh, x;
     locate(w.item, a.B * a.Hk, tiles, a.causal, bh, x);
     const int b = bh / a.Hk, hk = bh % a.Hk, k0 = x * KB;
-    const int kw = wave & 3, rows0 = PAIRED ? (wave >> 2) * 32 : 0;        // the wave's 32 keys, and its rows of a query tile
-    const int key = k0 + kw * 32 + (lane & 31);
+        const int key = k0 + wave * 32 + (lane & 31);
     const int kend = keys_of(a, b), reach = a.Tk - a.Tq;
     const int t_min = key >= kend ? 1 << 30 : a.causal ? key - reach : 0;  // the key is seen by queries from t_min on
-    const int w_first = k0 + kw * 32;                                    // the wave's first key
+    const int w_first = k0 + wave * 32;                                    // the wave's first key
     const int w_tmax = a.causal ? w_first + 31 - reach : 0;                // queries from here on see all keys of the wave
     const int q_first = a.causal ? max(0, k0 - reach) / QT : 0;            // first query tile that sees a key of the workgroup
     const int q_tiles = (a.Tq + QT - 1) / QT;
@@ -765,7 +778,6 @@ __global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void at
     lds_ptr const buf0 = (lds_ptr)smem;                                    // (the buffers first: their addresses fit the offset fields)
     lds_ptr const buf1 = buf0 + BUF;
     lds_ptr const vmem = buf0 + 2 * BUF;                                   // [KB] value rows
-    lds_ptr const kmem = vmem + L::bytes(KB);                              // [KB] key rows (PAIRED)
     const T* const kbase = a.k + b * a.ks.b + hk * a.ks.h;
     const T* const vbase = a.v + b * a.vs.b + hk * a.vs.h;
     f32x16 dv[DT], dk[NA];
@@ -774,7 +786,7 @@ __global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void at
 #pragma unroll
     for (int n = 0; n < NA; ++n) dk[n] = zero16();
 
-    const Copy<T, DP, QT, NW> qc(a.qs.t, a.d), gc((long long)a.H * 2 * a.d, a.d);
+    const Copy<T, DP, QT, NW> q_copy(a.qs.t, a.d), g_copy((long long)a.H * 2 * a.d, a.d);
     const long long gstride = (long long)a.H * 2 * a.d;
     // the next tile to copy: (head, query tile) and where it lies
     struct Pos { int head, tile; const T* q; const T* g; const float* stat; } pos{};
@@ -786,8 +798,8 @@ __global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void at
     if (first < last) go_to(first / per_head, q_first + first % per_head);
     auto issue = [&](lds_ptr dst) {
         const int have = a.Tq - pos.tile * QT;
-        qc.issue(pos.q, have, dst);
-        gc.issue(pos.g, have, dst + TB);
+        q_copy.issue(pos.q, have, dst);
+        g_copy.issue(pos.g, have, dst + TB);
         if (wave == 0) {
             const __amdgpu_buffer_rsrc_t rs =
                 __builtin_amdgcn_make_buffer_rsrc((void*)pos.stat, 0, (unsigned)(3 * a.Tp + QT) * 4u, 0x00020000);
@@ -804,35 +816,37 @@ __global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void at
     };
     // `cur` holds the tile of (head, tile), the next one goes to `fill`
     int head = pos.head, tile = pos.tile;
-    Frag<T> kf[2][PAIRED ? 1 : KS];
-    auto step = [&](bool more, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill, lds_cptr __restrict__ vals) {
-        const int t0 = tile * QT + rows0, hq = hk * group + head;
+    Frag<T> kf[2][KS];
+    const typename L::Lane rl = L::row_lane(lane), cl = L::col_lane(lane);
+    // the lane's addresses, as values that the compiler cannot prove equal to those of the last use and keep
+    auto fresh = [](typename L::Lane l, int off) {
+        asm volatile("" : "+v"(l.mix), "+s"(off));
+        return typename L::Lane{l.part + off, l.mix};
+    };
+    auto step = [&](bool more, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill) {
+        const int t0 = tile * QT, hq = hk * group + head;
         if (++tile == q_tiles) { tile = q_first; ++head; }
         if (more) issue(fill);
         if (w_first >= kend || (a.causal && t0 + 31 + reach < w_first)) return;     // nothing of this wave is seen
         const float lam = lam_of(a.lam, a.lam_bf16, hq);
-        lds_cptr const qt = cur + L::row_off(rows0);
-        lds_cptr const gt = qt + TB;
-        lds_cptr const keys = vals + L::bytes(KB);
-        const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB) + rows0;    // [lse_1, delta_1, lse_2, delta_2][QT]
+        lds_cptr const gt = cur + TB;
+        const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB);            // [lse_1, delta_1, lse_2, delta_2][QT]
         const bool edge = w_first + 32 > kend || (a.causal && t0 < w_tmax);
         f32x16 dp = zero16();
+        const typename L::Lane gl = fresh(rl, 0), vl = fresh(rl, L::row_off(wave * 32));
 #pragma unroll
         for (int n = 0; n < VS; ++n) {
             if (n && n % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-            dp = mma(L::row_piece(gt, 0, lane & 31, n, h2), L::row_piece(vals, 0, lane & 31, n, h2), dp);
+            dp = mma(L::row_piece(gt, gl, 0, n), L::row_piece(vmem, vl, 0, n), dp);
         }
         f32x16 p = zero16();            // P_1 - lam P_2
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             __builtin_amdgcn_sched_barrier(0);          // (one map after the other: fewer operands in flight)
             f32x16 s = zero16();
+            const typename L::Lane ql = fresh(rl, 0);
 #pragma unroll
-            for (int n = 0; n < KS; ++n) {
-                const Frag<T> qp = L::row_piece(qt, 0, lane & 31, i * KS + n, h2);
-                if constexpr (PAIRED) s = mma(qp, L::row_piece(keys, 0, lane & 31, i * KS + n, h2), s);
-                else s = mma(qp, kf[i][n], s);
-            }
+            for (int n = 0; n < KS; ++n) s = mma(L::row_piece(cur, ql, 0, i * KS + n), kf[i][n], s);
             if (edge) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = t0 + acc_row(r, h2) >= t_min ? s[r] : -INFINITY;
@@ -856,11 +870,12 @@ __global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void at
                 }
                 pack(df[u], ds);
             }
+            const typename L::Lane qc = fresh(cl, 0);
 #pragma unroll
             for (int n = 0; n < NA / 2; ++n)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
-                    dk[i * (NA / 2) + n] = mma(L::col_piece(qt, 16 * u, DP == 16 ? 0 : i * (NA / 2) + n, lane), df[u], dk[i * (NA / 2) + n]);
+                    dk[i * (NA / 2) + n] = mma(L::col_piece(cur, qc, 16 * u, DP == 16 ? 0 : i * (NA / 2) + n), df[u], dk[i * (NA / 2) + n]);
         }
         Frag<T> pf[2];
 #pragma unroll
@@ -870,56 +885,29 @@ __global__ __launch_bounds__(PAIRED ? 512 : 256, sizeof(T) == 2 ? 2 : 1) void at
             for (int j = 0; j < 8; ++j) x[j] = p[8 * u + j];
             pack(pf[u], x);
         }
+        const typename L::Lane gc = fresh(cl, 0);
 #pragma unroll
         for (int n = 0; n < DT; ++n)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) dv[n] = mma(L::col_piece(gt, 16 * u, n, lane), pf[u], dv[n]);
+            for (int u = 0; u < 2; ++u) dv[n] = mma(L::col_piece(gt, gc, 16 * u, n), pf[u], dv[n]);
     };
     if (first < last) {
         const Copy<T, DP, KB, NW> vc(a.vs.t, a.d);
         vc.issue(vbase + k0 * a.vs.t, kend - k0, vmem);
-        if constexpr (PAIRED) Copy<T, DP, KB, NW>(a.ks.t, a.d).issue(kbase + k0 * a.ks.t, kend - k0, kmem);
-        lds_cptr const vals = vmem + L::row_off(kw * 32);
         issue(buf0);
-        if constexpr (!PAIRED) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    kf[i][s] = global_piece<T>(kbase + (key < kend ? (long long)key * a.ks.t : 0), i, s * 16 + 8 * h2, a.d, key < kend);
-        }
+            for (int s = 0; s < KS; ++s)
+                kf[i][s] = global_piece<T>(kbase + (key < kend ? (long long)key * a.ks.t : 0), i, s * 16 + 8 * h2, a.d, key < kend);
         for (int i = first;;) {
             stage_sync();
-            step(i + 1 < last, buf0, buf1, vals);
+            step(i + 1 < last, buf0, buf1);
             if (++i >= last) break;
             stage_sync();
-            step(i + 1 < last, buf1, buf0, vals);
+            step(i + 1 < last, buf1, buf0);
             if (++i >= last) break;
         }
-    }
-    if constexpr (PAIRED) {
-        // the second wave of each pair hands its sums over, 64 floats of every lane at a time
-        SF_LDS float* const box = (SF_LDS float*)smem + (kw * 128) * 64 + lane;
-        static_assert((DT + NA) * 16 <= 128, "one box per pair");
-        __syncthreads();
-        if (wave >= 4) {
-#pragma unroll
-            for (int n = 0; n < DT; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    box[(n * 16 + r) * 64] = dv[n][r];
-                    box[((DT + n) * 16 + r) * 64] = dk[n][r];
-                }
-        }
-        __syncthreads();
-        if (wave >= 4) return;
-#pragma unroll
-        for (int n = 0; n < DT; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                dv[n][r] += box[(n * 16 + r) * 64];
-                dk[n][r] += box[((DT + n) * 16 + r) * 64];
-            }
     }
     if (key >= a.Tk) return;
     const long long out = (((long long)b * a.Tk + key) * a.Hk + hk) * (2 * a.d);
@@ -1011,7 +999,7 @@ Cut cut_items(long long items, int slots, int tiles, bool f32, bool causal) {
     int parts = 0;
     for (int p = 1; p <= 64 && (p == 1 || tiles / p >= 2); ++p) {
         const long long rounds = (tail * p + slots - 1) / slots;
-        const long long cost = rounds * (4 * ((tiles + p - 1) / p) + (f32 ? 2 : 4)) + (p > 1 ? (f32 ? 16 : 32) : 0);
+        const long long cost = rounds * (4 * ((tiles + p - 1) / p) + 4) + (p > 1 ? (f32 ? 16 : 32) : 0);
         if (!parts || cost < best) { best = cost; parts = p; }
     }
     if (parts == 1) return {(int)items, 0, 1};
@@ -1020,7 +1008,7 @@ Cut cut_items(long long items, int slots, int tiles, bool f32, bool causal) {
 // workgroups that share a CU: what the kernels' registers (forward pass of single tokens: LDS) leave room for
 enum Pass { FWD, FWD_KEYS, DQ, DKV };
 int slots_of(const sf_diff_attn_desc* p, Pass pass) {
-    static const int bf16_[4][3] = {{4, 3, 2}, {4, 2, 2}, {4, 3, 2}, {3, 2, 1}}, f32_[4][3] = {{2, 1, 1}, {2, 1, 1}, {2, 2, 1}, {2, 2, 1}};
+    static const int bf16_[4][3] = {{4, 3, 2}, {4, 2, 2}, {4, 3, 2}, {3, 2, 2}}, f32_[4][3] = {{4, 2, 1}, {2, 1, 1}, {3, 2, 1}, {3, 2, 1}};
     const int w = p->d <= 16 ? 0 : p->d <= 32 ? 1 : 2;
     return 256 * (p->dtype == SF_F32 ? f32_ : bf16_)[pass][w];
 }
@@ -1042,8 +1030,7 @@ Cut dq_cut(const sf_diff_attn_desc* p) {
     return cut_items((rows + 127) / 128 * p->B * p->Hk, slots_of(p, DQ), (p->Tk + 63) / 64, p->dtype == SF_F32, p->causal);
 }
 Cut dkv_cut(const sf_diff_attn_desc* p) {
-    const int qt = p->dtype == SF_BF16 && padded(p->d) == 64 ? 64 : 32;
-    return cut_items((long long)((p->Tk + 127) / 128) * p->B * p->Hk, slots_of(p, DKV), (p->Tq + qt - 1) / qt * (p->H / p->Hk),
+    return cut_items((long long)((p->Tk + 127) / 128) * p->B * p->Hk, slots_of(p, DKV), (p->Tq + 31) / 32 * (p->H / p->Hk),
                      p->dtype == SF_F32, p->causal);
 }
 
@@ -1108,10 +1095,8 @@ template <typename T, int DP> int launch_bwd(Args<T> a, const Cut& cq, const Cut
     constexpr int KT = sizeof(T) == 4 ? 32 : 64;
     hipLaunchKernelGGL((attn_delta_kernel<T>), dim3(ceil_div(n, 16)), dim3(256), 0, st, a);
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (delta)");
-    constexpr bool paired = sizeof(T) == 2 && DP == 64;
     constexpr int lds_q = 4 * L::bytes(KT);
-    constexpr int lds_k = (paired ? 2 : 1) * L::bytes(128) + 2 * (2 * L::bytes(paired ? 64 : 32) + 1024);
-    static_assert(!paired || lds_k >= 4 * 128 * 64 * 4, "the pairs' boxes");
+    constexpr int lds_k = L::bytes(128) + 2 * (2 * L::bytes(32) + 1024);
     SF_LDS_ONCE((attn_dq_kernel<T, DP, KT>), lds_q);
     a.full = cq.full;
     a.parts = cq.parts;
@@ -1121,10 +1106,10 @@ template <typename T, int DP> int launch_bwd(Args<T> a, const Cut& cq, const Cut
         hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, false>), dim3(cq.tail * 32), dim3(256), 0, st, a, cq.tail);
         SF_LAUNCH_CHECK("sf_diff_attn_bwd (queries, join)");
     }
-    SF_LDS_ONCE((attn_dkv_kernel<T, DP, paired>), lds_k);
+    SF_LDS_ONCE((attn_dkv_kernel<T, DP>), lds_k);
     a.full = ck.full;
     a.parts = ck.parts;
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, paired>), dim3(ck.full + ck.tail * ck.parts), dim3(paired ? 512 : 256), lds_k, st, a);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(ck.full + ck.tail * ck.parts), dim3(256), lds_k, st, a);
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (keys)");
     if (ck.tail) {
         hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, true>), dim3(ck.tail * 32), dim3(256), 0, st, a, ck.tail);
