@@ -565,9 +565,13 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_join_k
 }
 
 // ------------------------------------------------------------------------------ backward
-// stat = lse_1, delta_1, lse_2, delta_2 of every row, delta_i = do . O_i.  16 lanes per row.  O_1 and O_2 are kept in f32: the
-// gradients of the scores are differences dP - delta, and with bf16 maps their rounding would be most of the error of dq, dk
-// and dlam (measured on 32 x 365 tokens: relative error of dq 3.6e-3, against 2.0e-3 so).
+constexpr int STATS = 5;                // values of a row
+
+// stat = lse_1, -delta_1, lse_2, lam (delta_2 - delta_1), delta_2 of every row; delta_i = do . O_i.  16 lanes per row.  What the two
+// gradient kernels would compute for every score is in them: -delta_1 starts the accumulators of dP, so that
+// dP - delta_1 costs nothing, and -lam (dP - delta_2) is one multiply-add from it (2 x 5120 tokens: dq 384 to 372 us, dk and dv 597 to 589).  O_1 and O_2 are
+// kept in f32: the gradients of the scores are differences dP - delta, and rounding the maps to bf16 as well raises the
+// relative error of dq from 2.9e-3 to 3.6e-3 (32 x 365 tokens).
 template <typename T> __global__ __launch_bounds__(256) void attn_delta_kernel(Args<T> a) {
     const long long id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);       // (b, t, h), t up to Tp
     const int q = threadIdx.x & 15, h = (int)(id % a.H), t = (int)(id / a.H % a.Tp);
@@ -595,10 +599,10 @@ template <typename T> __global__ __launch_bounds__(256) void attn_delta_kernel(A
         d1 += __shfl_xor(d1, o, 64);
         d2 += __shfl_xor(d2, o, 64);
     }
-    if (q >= 4) return;
-    float v = q == 1 ? d1 : d2;
-    if ((q & 1) == 0) v = t < a.Tq ? a.lse_in[((b * a.H + h) * a.Tq + t) * 2 + (q >> 1)] : 0.f;
-    a.stat[((b * a.H + h) * 4 + q) * a.Tp + t] = v;
+    if (q >= STATS) return;
+    float v = q == 1 ? -d1 : q == 3 ? lam_of(a.lam, a.lam_bf16, h) * (d2 - d1) : d2;
+    if (q == 0 || q == 2) v = t < a.Tq ? a.lse_in[((b * a.H + h) * a.Tq + t) * 2 + (q >> 1)] : 0.f;
+    a.stat[((b * a.H + h) * STATS + q) * a.Tp + t] = v;
 }
 
 // dlam[h] = -sum over the rows of head h of delta_2, in 64 bits and a fixed order
@@ -609,7 +613,7 @@ __global__ __launch_bounds__(1024) void attn_dlam_kernel(const float* __restrict
     double s = 0.0;
     const long long n = (long long)B * Tp;
 #pragma unroll 8
-    for (long long i = threadIdx.x; i < n; i += 1024) s += (double)stat[((i / Tp * H + h) * 4 + 3) * Tp + i % Tp];
+    for (long long i = threadIdx.x; i < n; i += 1024) s += (double)stat[((i / Tp * H + h) * STATS + 4) * Tp + i % Tp];
     s = wave_sum_d(s);
     if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -659,8 +663,11 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a)
         gf[s] = global_piece<T>(a.dout + out, 0, s * 16 + 8 * h2, a.d, true);
         gf[KS + s] = global_piece<T>(a.dout + out, 1, s * 16 + 8 * h2, a.d, true);
     }
-    const float* const stat = a.stat + ((long long)b * a.H + hq) * 4 * a.Tp + t;
-    const float lse[2] = {stat[0], stat[2 * a.Tp]}, delta[2] = {stat[a.Tp], stat[3 * a.Tp]};
+    const float* const stat = a.stat + ((long long)b * a.H + hq) * STATS * a.Tp + t;
+    const float lse[2] = {stat[0], stat[2 * a.Tp]}, apart = stat[3 * a.Tp], lam = lam_of(a.lam, a.lam_bf16, hq);
+    f32x16 start;                                          // of dP - delta_1
+#pragma unroll
+    for (int r = 0; r < 16; ++r) start[r] = stat[a.Tp];
     f32x16 acc[NA];
 #pragma unroll
     for (int n = 0; n < NA; ++n) acc[n] = zero16();
@@ -673,7 +680,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a)
 
     auto sub_tile = [&](lds_cptr kt, lds_cptr vt, int sub, int key0) {
         if (key0 >= vmax) return;
-        f32x16 s[2] = {zero16(), zero16()}, dp = zero16();
+        f32x16 s[2] = {zero16(), zero16()}, dp = start;
 #pragma unroll
         for (int n = 0; n < KS; ++n)
 #pragma unroll
@@ -694,7 +701,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a)
         for (int i = 0; i < 2; ++i) {
             float ds[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(s[i][r] * a.c - lse[i]) * (dp[r] - delta[i]);
+            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(s[i][r] * a.c - lse[i]) * (i ? fmaf(-lam, dp[r], apart) : dp[r]);
             pack(df[i][0], ds);
             pack(df[i][1], ds + 8);
         }
@@ -727,15 +734,13 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a)
         }
     }
     if (!have) return;
-    const float f1 = a.scale, f2 = -a.scale * lam_of(a.lam, a.lam_bf16, hq);
 #pragma unroll
     for (int n = 0; n < NA; ++n)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const int col = (DP == 16 ? 0 : 32 * n) + acc_row(r, h2), map = DP == 16 ? n : 32 * n / DP;
-            const float f = map ? f2 : f1;
             if (col / DP != map) continue;
-            const float4 y{acc[n][r] * f, acc[n][r + 1] * f, acc[n][r + 2] * f, acc[n][r + 3] * f};
+            const float4 y{acc[n][r] * a.scale, acc[n][r + 1] * a.scale, acc[n][r + 2] * a.scale, acc[n][r + 3] * a.scale};
             if (w.parts > 1)
                 *reinterpret_cast<float4*>(a.part + (((long long)w.tail * w.parts + w.part) * RB + (row - r0)) * (2 * DP) + col) = y;
             else
@@ -793,7 +798,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
     auto go_to = [&](int head, int tile) {
         const int hq = hk * group + head, t = tile * QT;
         pos = {head, tile, a.q + b * a.qs.b + hq * a.qs.h + t * a.qs.t, a.dout + ((long long)b * a.Tq + t) * gstride + hq * (2 * a.d),
-               a.stat + ((long long)b * a.H + hq) * 4 * a.Tp + t};
+               a.stat + ((long long)b * a.H + hq) * STATS * a.Tp + t};
     };
     if (first < last) go_to(first / per_head, q_first + first % per_head);
     auto issue = [&](lds_ptr dst) {
@@ -830,9 +835,15 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
         if (w_first >= kend || (a.causal && t0 + 31 + reach < w_first)) return;     // nothing of this wave is seen
         const float lam = lam_of(a.lam, a.lam_bf16, hq);
         lds_cptr const gt = cur + TB;
-        const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB);            // [lse_1, delta_1, lse_2, delta_2][QT]
+        const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB);            // [STATS - 1][QT]
         const bool edge = w_first + 32 > kend || (a.causal && t0 < w_tmax);
-        f32x16 dp = zero16();
+        f32x16 dp;                      // dP - delta_1
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const f32x4 dl = *(const SF_LDS f32x4*)(stat + QT + acc_row(r, h2));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[r + e] = dl[e];
+        }
         const typename L::Lane gl = fresh(rl, 0), vl = fresh(rl, L::row_off(wave * 32));
 #pragma unroll
         for (int n = 0; n < VS; ++n) {
@@ -859,13 +870,13 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
                 for (int k = 0; k < 8; k += 4) {
                     const int r = 8 * u + k;
                     const f32x4 lv = *(const SF_LDS f32x4*)(stat + 2 * QT * i + acc_row(r, h2));
-                    const f32x4 dl = *(const SF_LDS f32x4*)(stat + 2 * QT * i + QT + acc_row(r, h2));
+                    f32x4 apart{};
+                    if (i) apart = *(const SF_LDS f32x4*)(stat + 3 * QT + acc_row(r, h2));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float y = __builtin_amdgcn_exp2f(s[r + e] * a.c - lv[e]);
-                        if (i) y *= -lam;
-                        p[r + e] = i ? p[r + e] + y : y;
-                        ds[k + e] = y * (dp[r + e] - dl[e]);
+                        const float y = __builtin_amdgcn_exp2f(s[r + e] * a.c - lv[e]);
+                        p[r + e] = i ? fmaf(-lam, y, p[r + e]) : y;
+                        ds[k + e] = y * (i ? fmaf(-lam, dp[r + e], apart[e]) : dp[r + e]);
                     }
                 }
                 pack(df[u], ds);
@@ -1008,7 +1019,7 @@ Cut cut_items(long long items, int slots, int tiles, bool f32, bool causal) {
 // workgroups that share a CU: what the kernels' registers (forward pass of single tokens: LDS) leave room for
 enum Pass { FWD, FWD_KEYS, DQ, DKV };
 int slots_of(const sf_diff_attn_desc* p, Pass pass) {
-    static const int bf16_[4][3] = {{4, 3, 2}, {4, 2, 2}, {4, 3, 2}, {3, 2, 2}}, f32_[4][3] = {{4, 2, 1}, {2, 1, 1}, {3, 2, 1}, {3, 2, 1}};
+    static const int bf16_[4][3] = {{4, 3, 2}, {4, 2, 2}, {3, 3, 2}, {3, 2, 2}}, f32_[4][3] = {{4, 2, 1}, {2, 1, 1}, {3, 2, 1}, {3, 2, 1}};
     const int w = p->d <= 16 ? 0 : p->d <= 32 ? 1 : 2;
     return 256 * (p->dtype == SF_F32 ? f32_ : bf16_)[pass][w];
 }
@@ -1126,7 +1137,7 @@ template <typename T> int fwd(const sf_diff_attn_desc* p, const void* q, const v
     const int dp = padded(p->d);
     return dp == 16 ? launch_fwd<T, 16>(a, f, st) : dp == 32 ? launch_fwd<T, 32>(a, f, st) : launch_fwd<T, 64>(a, f, st);
 }
-size_t stat_bytes(const sf_diff_attn_desc* p) { return (size_t)p->B * p->H * ((p->Tq + 63) / 64 * 64) * 4 * sizeof(float); }
+size_t stat_bytes(const sf_diff_attn_desc* p) { return (size_t)p->B * p->H * ((p->Tq + 63) / 64 * 64) * STATS * sizeof(float); }
 template <typename T> int bwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
                               const int* lengths, const float* maps, const float* lse, const void* dout, void* dq, void* dk,
                               void* dv, void* dlam, char* ws, hipStream_t st) {
