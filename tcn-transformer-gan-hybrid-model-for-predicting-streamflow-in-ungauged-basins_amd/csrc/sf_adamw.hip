@@ -17,6 +17,10 @@
 // for ever: codes are rounded stochastically, with 16 bits of an integer hash of (seed, step, tensor,
 // element), which keeps the moments unbiased and a run reproducible.  A second moment is never rounded to
 // zero (its square root divides).  The update of p uses the moments before they are rounded.
+//
+// Measured on 68.3 M elements in 39 tensors (a copy of 1 GiB runs at 5.05 TB/s on the same card): f32 gradients and moments 360 us,
+// 1.91 GB, 5.3 TB/s; bf16 gradients and 8-bit moments 196 us, 0.96 GB, 4.9 TB/s, and their values as bf16 (adamw_moments) 82 us,
+// 0.41 GB, 5.0 TB/s.  16 tensors with 2.8 M elements: 13 us, and the launch around it costs the host more.
 #include "sf_common.h"
 #include "../../include/sfhip.h"
 

@@ -9,8 +9,9 @@
 // The score matrices never exist in memory: tiles of 32 keys x 32 queries live in registers and the softmax runs
 // online (running maximum and sum per row and map, f32; exponents in base 2).  All products are 32 x 32
 // matrix instructions with f32 accumulation; probabilities and score gradients are rounded to the inputs' type to
-// enter the second product (bf16: half a step of 2^-8 of each probability, the size of the inputs' own
-// rounding).  The f32 form runs through the same code with f32 matrix instructions and rounds nothing.
+// enter the second product (bf16: at most half a step, 2^-8 of each, the size of the inputs' own rounding; relative to
+// its norm the output is then 2.2e-3 off and the gradients of q and k 2.6e-3 to 2.9e-3, where rounding the exact result to bf16
+// costs 1.7e-3).  The f32 form runs through the same code with f32 matrix instructions and rounds nothing.
 //
 // Layout.  Heads are [.., 2, d] rows (v and o: [.., 2 d], treated as two halves as well), d <= 64 a multiple of 8,
 // padded to DP = 16, 32 or 64 columns per half inside a tile.  A tile in LDS is [row][2 DP] and is read in two ways: 32 rows
@@ -285,6 +286,10 @@ template <typename T, int DP> __device__ __forceinline__ void store_cols(T* row,
 // one copy of the keys serves the whole group.  KEYS_SPLIT false: wave w takes rows 32 w .. of the workgroup's 128 and
 // all keys of the tile.  KEYS_SPLIT true (at most 32 rows, single tokens): all waves take the same 32 rows and wave w
 // the keys 32 w .. of the tile; the waves' results are joined through LDS at the end.
+// Measured, bf16 heads of 2 x 64: 8 heads, 2 x 5120 tokens: 340 to 375 us, 322 GFLOP, 0.9 PFLOP/s (a library product reaches 1.28);
+// the matrix pipe is busy 48 % of the time and the vector unit (32 exponentials a lane and tile of 32 x 32) nearly as long, hardly
+// at the same time, at a clock that power holds at 1.75 GHz.  1 x 8191 tokens, causal: 262 to 280 us, 206 GFLOP.  Single tokens,
+// 16 samples, 4 key heads, 8192 keys: 30 us, 134 MB, 4.4 TB/s, bound by HBM.
 template <typename T, int DP, int NW, bool KEYS_SPLIT, int KT>
 __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<T> a) {
     using L = Tile<T, DP>;
@@ -507,7 +512,8 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
     }
 }
 
-// joins the parts of the forward items that were cut: one wave per query row
+// joins the parts of the forward items that were cut: one wave per query row (2 x 5120 tokens, two parts for a fifth of the rows:
+// 18 us; single tokens of 64 key heads, four parts: 6 us)
 template <typename T, int DP> __global__ __launch_bounds__(256) void attn_join_kernel(Args<T> a, int rb, int items) {
     const int lane = threadIdx.x & 63;
     const int group = a.H / a.Hk;
@@ -569,9 +575,10 @@ constexpr int STATS = 5;                // values of a row
 
 // stat = lse_1, -delta_1, lse_2, lam (delta_2 - delta_1), delta_2 of every row; delta_i = do . O_i.  16 lanes per row.  What the two
 // gradient kernels would compute for every score is in them: -delta_1 starts the accumulators of dP, so that
-// dP - delta_1 costs nothing, and -lam (dP - delta_2) is one multiply-add from it (2 x 5120 tokens: dq 384 to 372 us, dk and dv 597 to 589).  O_1 and O_2 are
-// kept in f32: the gradients of the scores are differences dP - delta, and rounding the maps to bf16 as well raises the
-// relative error of dq from 2.9e-3 to 3.6e-3 (32 x 365 tokens).
+// dP - delta_1 costs nothing, and -lam (dP - delta_2) is one multiply-add from it (2 x 5120 tokens, 8 heads: dq 384 to
+// 372 us, dk and dv 597 to 589).  O_1 and O_2 are kept in f32: the gradients of the scores are differences dP - delta,
+// and rounding the maps to bf16 as well raises the relative error of dq from 2.9e-3 to 3.6e-3 (32 x 365 tokens).  Bound by HBM:
+// 22 us for the 210 MB of 2 x 5120 tokens and 8 heads of 2 x 64, most of it the maps.
 template <typename T> __global__ __launch_bounds__(256) void attn_delta_kernel(Args<T> a) {
     const long long id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);       // (b, t, h), t up to Tp
     const int q = threadIdx.x & 15, h = (int)(id % a.H), t = (int)(id / a.H % a.Tp);
@@ -605,7 +612,7 @@ template <typename T> __global__ __launch_bounds__(256) void attn_delta_kernel(A
     a.stat[((b * a.H + h) * STATS + q) * a.Tp + t] = v;
 }
 
-// dlam[h] = -sum over the rows of head h of delta_2, in 64 bits and a fixed order
+// dlam[h] = -sum over the rows of head h of delta_2, in 64 bits and a fixed order (10240 rows a head: 6 us, latency)
 __global__ __launch_bounds__(1024) void attn_dlam_kernel(const float* __restrict__ stat, void* __restrict__ dlam, int lam_bf16,
                                                          int B, int H, int Tp) {
     __shared__ double sm[16];
@@ -624,7 +631,8 @@ __global__ __launch_bounds__(1024) void attn_dlam_kernel(const float* __restrict
     }
 }
 
-// Gradient of the queries: as the forward pass, 32 rows per wave, the keys tile by tile.
+// Gradient of the queries: as the forward pass, 32 rows per wave, the keys tile by tile.  (8 bf16 heads of 2 x 64, 2 x 5120 tokens:
+// 347 to 380 us, 322 GFLOP, 0.88 PFLOP/s; bound as the forward pass.)
 template <typename T, int DP, int KT>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a) {
     using L = Tile<T, DP>;
@@ -753,7 +761,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a)
 // 32 registers of keys little is left of the 256 that two waves per SIMD have, and a spilled one is reloaded behind the copies
 // under way.  So a lane keeps two address registers for its row pieces and two for its column pieces and makes the
 // others where it uses them (fresh), and the maps come one after the other: no spill in the loop (2 x 5120 tokens, 8 heads:
-// 725 us with 13 spills, 592 us without; eight waves in pairs, with the keys in LDS too, 635 us).
+// 725 us with 13 spills, 592 us without; eight waves in pairs, with the keys in LDS too, 635 us).  539 to 600 us now, 429 GFLOP,
+// 0.75 PFLOP/s: the matrix pipe is busy 38 % of the time, LDS reads 34 %, and no registers are left to fetch operands ahead.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a) {
     using L = Tile<T, DP>;
