@@ -900,6 +900,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     query heads share a key / value head).  scale defaults to 1 / sqrt(d).  causal: query t sees keys up to t + Tk - Tq, so that
     the last query sees the last key.  lengths: int32 [B] on the device, the keys each sample has (the values
     are clamped to [0, Tk]; what lies behind them is never read).  A query that sees no key gives zeros.
+    Keys that only the causal order hides have weight zero: an infinity or NaN among their values shows in
+    a query close before them, as in a plain product.
     Sums and softmax statistics are f32; in bf16 the probabilities are rounded once for the second product.
     Differentiable once in q, k, v and lam; no atomics: equal inputs give equal bits.  Slices of one projection are
     read in place where their steps are whole 16 bytes, other layouts are copied."""

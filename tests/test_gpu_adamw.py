@@ -528,3 +528,26 @@ def test_gpu_refusals():
     with pytest.raises(RuntimeError, match="state"):
         step([p], [z()], [z()], [z()], z(3, torch.int32), 1e-3)
     assert state.tolist() == [0, 0]
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """A tensor of 2^30 + 5001 elements (4.3 GB each of values, gradients and f32 moments), between two small ones: its last
+    elements take the step that they take alone."""
+    sf = load_pkg()
+    n, k = (1 << 30) + 5001, 7001
+    big = [torch.full((n,), x, device="cuda") for x in (0.5, 0.25, 0.125, 0.0625)]
+    for t in big:
+        t[-k:].normal_()
+    big[3].abs_()
+    alone = [t[-k:].clone() for t in big]
+    lists = [[torch.ones(5, device="cuda"), t, torch.ones(3, device="cuda")] for t in big]
+    for xs in (lists, [[t] for t in alone]):
+        state = torch.zeros(2, device="cuda", dtype=torch.int32)
+        sf.functional.adamw_step(*xs, state, 1e-2)
+    for t, a in zip(big, alone):
+        assert torch.equal(t[-k:], a)
+    head = [torch.full((100,), x, device="cuda") for x in (0.5, 0.25, 0.125, 0.0625)]
+    sf.functional.adamw_step(*([t] for t in head), torch.zeros(2, device="cuda", dtype=torch.int32), 1e-2)
+    for t, a in zip(big, head):
+        assert bool((t[:-k] == a[0]).all())

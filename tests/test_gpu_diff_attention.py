@@ -285,6 +285,36 @@ def test_strides(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("Tq", [1, 300])
+def test_offsets_beyond_32_bits(Tq, dtype):
+    """Tokens and samples so far apart that their byte offsets pass 2^32 (a long cache): the same bits as packed ones."""
+    sf = load_pkg()
+    q, k, v, lam, do = (t.cuda() for t in make(2, Tq, 700, 2, 1, 64, dtype, seed=14))
+    step = (1 << 22) - 64                               # elements between two tokens, just below what the kernels take
+
+    def far(t, n):
+        buf = torch.empty(n, device="cuda", dtype=dtype)
+        gap = t.shape[1] * step                         # between the samples
+        strides = (gap, step, *t.contiguous().stride()[2:])
+        x = buf.as_strided(t.shape, strides)
+        x.copy_(t)
+        return x
+    xs = [far(t, 2 * t.shape[1] * step) for t in (q, k, v)]
+    if Tq > 1:
+        assert all(t.stride(0) * t.element_size() > 1 << 31 for t in xs)
+    assert all(2 * t.shape[1] * step * t.element_size() > 1 << 32 for t in xs[1:])
+    assert all(sf.ops.kernel_layout(t) is t for t in xs)
+    o, g = run(sf, q, k, v, lam, do, causal=True)
+    leaves = [t.requires_grad_(True) for t in (*xs, lam)]
+    of = sf.functional.diff_attention(*leaves, causal=True)
+    gf = torch.autograd.grad(of, leaves, do)
+    assert torch.equal(of, o)
+    for x, n in zip(gf, ("dq", "dk", "dv", "dlam")):
+        assert torch.equal(x, g[n])
+
+
+@pytest.mark.gpu
 def test_shared_heads_gradient_is_the_sum():
     """Shared key / value heads against the same call with the heads repeated: gradients add up over the group."""
     sf = load_pkg()

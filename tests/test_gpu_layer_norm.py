@@ -313,3 +313,45 @@ def test_gpu_refusals():
         ln(x, None, torch.ones(4))
     with pytest.raises(RuntimeError, match="no axis"):
         ln(torch.zeros(3, 0, device="cuda"), None, None)
+
+
+@pytest.mark.gpu
+def test_captured_training_pass_replays():
+    sf = load_pkg()
+    x, res, w, b, dy, ds = cuda(*make(700, 200, BF, True, seed=7))
+
+    def passes():
+        xs = [t.detach().requires_grad_(True) for t in (x, res, w, b)]
+        y, s = sf.functional.layer_norm(*xs[:1], *xs[2:], residual=xs[1])
+        return (y.detach(), s.detach(), *torch.autograd.grad([y, s], xs, [dy, ds]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        passes()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = passes()
+    for k in range(4):
+        for t in (x, res, dy, ds):
+            t.copy_(torch.randn_like(t) + k)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(got, passes()):
+            assert torch.equal(a, e)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """2^20 + 3 rows of 2056 bf16 values, 4.3 GB: a row's result does not depend on the rows before it, so the last ones have
+    the bits that they have alone."""
+    sf = load_pkg()
+    x = torch.empty((1 << 20) + 3, 2056, device="cuda", dtype=BF).normal_().requires_grad_(True)
+    w = torch.randn(2056, device="cuda")
+    y = sf.functional.layer_norm(x, w, None)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    tail = x.detach()[-1000:].clone().requires_grad_(True)
+    yt = sf.functional.layer_norm(tail, w, None)
+    dt, = torch.autograd.grad(yt, tail, tail.detach())
+    assert torch.equal(y[-1000:], yt) and torch.equal(dx[-1000:], dt)
