@@ -878,6 +878,7 @@ class DiffAttentionFn(torch.autograd.Function):
         o, saved = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need)
         if need:
             ctx.desc, maps, lse = saved or (None, None, None)       # (no query or no key: nothing to save)
+            ctx.strides = (q.stride(), k.stride(), v.stride())
             ctx.save_for_backward(q, k, v, lam, lengths, maps, lse)
         return o
 
@@ -887,7 +888,12 @@ class DiffAttentionFn(torch.autograd.Function):
         q, k, v, lam, lengths, maps, lse = ctx.saved_tensors
         if ctx.desc is None:
             return (*(torch.zeros(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, lam)), None, None, None)
-        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, ctx.desc, maps, lse, do.contiguous(), ctx.needs_input_grad[3])
+        desc = ctx.desc
+        if ctx.strides != (q.stride(), k.stride(), v.stride()) or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+            # hooks on saved tensors (torch.autograd.graph.save_on_cpu) give back copies of another layout
+            q, k, v = ops.kernel_layout(q), ops.kernel_layout(k), ops.kernel_layout(v)
+            desc = ops.diff_attn_desc(q, k, v, lam, desc.causal, desc.scale)
+        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, desc, maps, lse, do.contiguous(), ctx.needs_input_grad[3])
         return (*grads, None, None, None)
 
 

@@ -266,7 +266,7 @@ class DifferentialAttention(nn.Module):
             raise RuntimeError(f"DifferentialAttention: [B, T, {self.embed_dim}] tokens, not {tuple(x.shape)}")
         B, T, _ = x.shape
         H, kv, d, dt = self.num_heads, self.num_kv_heads, self.head_dim, SF.compute_dtype()
-        qkv = SF.linear(x.reshape(B * T, -1), self.in_proj, dt).to(dt).view(B, T, -1)
+        qkv = SF.linear(x.reshape(B * T, self.embed_dim), self.in_proj, dt).to(dt).view(B, T, -1)
         q, k, v = torch.split(qkv, [H * 2 * d, kv * 2 * d, kv * 2 * d], dim=-1)
         o = SF.diff_attention(q.view(B, T, H, 2, d), k.view(B, T, kv, 2, d), v.view(B, T, kv, 2 * d), self.lam(), self.causal,
                               lengths=lengths)

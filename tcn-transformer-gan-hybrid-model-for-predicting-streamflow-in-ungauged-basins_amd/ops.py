@@ -1178,7 +1178,7 @@ def kernel_layout(t: torch.Tensor) -> torch.Tensor:
     return t if _token_strides(t) is not None else t.clone(memory_format=torch.contiguous_format)
 
 
-def _diff_attn_desc(q, k, v, lam, causal, scale):
+def diff_attn_desc(q, k, v, lam, causal, scale):
     B, Tq, H, _, d = q.shape
     qs, ks, vs = _token_strides(q), _token_strides(k), _token_strides(v)
     if qs is None or ks is None or vs is None:
@@ -1193,7 +1193,7 @@ def diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need_save=False):
     o = torch.empty((B, Tq, H, 2 * d), device=q.device, dtype=q.dtype)
     if o.numel() == 0 or k.numel() == 0:        # no query, or no key for anyone
         return o.zero_(), None
-    desc = _diff_attn_desc(q, k, v, lam, causal, scale)
+    desc = diff_attn_desc(q, k, v, lam, causal, scale)
     at = ctypes.addressof(desc)
     maps = lse = None
     if need_save:
@@ -1207,8 +1207,9 @@ def diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need_save=False):
 
 
 def diff_attn_bwd(q, k, v, lam, lengths, desc, maps, lse, do, need_dlam=True):
-    """(dq, dk, dv, dlam), contiguous; desc, maps, lse: what diff_attn_fwd saved for the same q, k, v, lam, lengths."""
-    _dev(maps, lse, do, dtypes=[torch.float32, torch.float32, q.dtype])
+    """(dq, dk, dv, dlam), contiguous; maps, lse: what diff_attn_fwd saved for the same q, k, v, lam, lengths; desc: the one it
+    saved, if their layouts are still the same."""
+    _dev(lam, lengths, maps, lse, do, dtypes=[None, torch.int32, torch.float32, torch.float32, q.dtype])
     dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
     dlam = torch.empty_like(lam) if need_dlam else None
     at = ctypes.addressof(desc)
@@ -1400,8 +1401,8 @@ def adamw_step(ps, gs, ms, vs, state, lr, beta1, beta2, eps, weight_decay, seed=
             raise RuntimeError(f"adamw_step: {len(seq)} {name} for {n} parameters")
     _dev(state, found_inf, dtypes=[torch.int32, torch.int32])
     index = state.get_device()
-    if state.numel() != 2 or (found_inf is not None and found_inf.get_device() != index):
-        raise RuntimeError("adamw_step: state is int32 [2]: steps taken, steps skipped; found_inf lies on the same device")
+    if state.numel() != 2 or (found_inf is not None and (found_inf.get_device() != index or found_inf.numel() < 1)):
+        raise RuntimeError("adamw_step: state is int32 [2]: steps taken, steps skipped; found_inf is int32 [1] on the same device")
     numels = [p.numel() for p in ps]
     p_at = _flat_addresses(ps, numels, index, "adamw_step: parameter")
     codes, g_at = [], []

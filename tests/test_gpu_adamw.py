@@ -504,6 +504,8 @@ def test_gpu_refusals():
     p = z()
     with pytest.raises(RuntimeError, match="twice"):
         step([p, p], [z(), z()], [z(), z()], [z(), z()], state, 1e-3)
+    with pytest.raises(RuntimeError, match="found_inf"):
+        step([p], [z()], [z()], [z()], state, 1e-3, found_inf=torch.zeros(0, device="cuda", dtype=torch.int32))
     with pytest.raises(RuntimeError, match="twice"):
         m = z()
         step([p, z()], [z(), z()], [m, m], [z(), z()], state, 1e-3)

@@ -430,6 +430,26 @@ def test_captured_training_pass_replays(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_saved_tensors_in_another_layout(dtype):
+    """Slices of one projection, saved on the host meanwhile: what comes back for the backward pass is contiguous, and
+    the gradients have the same bits."""
+    sf = load_pkg()
+    x = torch.randn(2, 70, 3 * 2 * 32, device="cuda").to(dtype)
+    lam, do = torch.tensor([0.3, 0.6], device="cuda"), torch.randn(2, 70, 2, 32, device="cuda").to(dtype)
+
+    def grads():
+        leaf = x.clone().requires_grad_(True)
+        q, k, v = (t.view(2, 70, 2, 32) for t in leaf.split(64, -1))
+        q, k = q.view(2, 70, 2, 2, 16), k.view(2, 70, 2, 2, 16)
+        assert all(sf.ops.kernel_layout(t) is t and not t.is_contiguous() for t in (q, k, v))
+        return torch.autograd.grad(sf.functional.diff_attention(q, k, v, lam, causal=True), leaf, do)[0]
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        assert torch.equal(grads(), want)
+
+
+@pytest.mark.gpu
 def test_second_derivative_is_refused():
     sf = load_pkg()
     q, k, v, lam, do = (t.cuda() for t in make(1, 9, 9, 1, 1, 8, F))
