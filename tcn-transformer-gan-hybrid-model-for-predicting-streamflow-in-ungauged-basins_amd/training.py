@@ -455,17 +455,17 @@ class Trainer:
                 self._stale_master = False
 
     def _make_optimizer(self, net: nn.Module, lr: float, betas, big: int, shadow_big: bool) -> "FlatAdam":
-        """train.optimizer (an extension; the reference always uses Adam, src/train.py:80-91): "Adam" (default) or
-        "AdamW" with train.weight_decay (default 0.01) and train.optimizer_state_bits (32 or 8)."""
+        """train.optimizer (an extension; the reference always uses Adam, src/train.py:80-91, and reads no such key):
+        "AdamW" with train.weight_decay (default 0.01) and train.optimizer_state_bits (32 or 8); Adam without it."""
         tcfg = self.config.get("train", {})
         kind = str(tcfg.get("optimizer", "Adam")).lower()
-        if kind == "adam":
-            return FlatAdam(net, lr, betas=betas, big_numel=big, shadow_big=shadow_big)
         if kind == "adamw":
             return FlatAdamW(net, lr, betas=betas, big_numel=big, shadow_big=shadow_big,
                              weight_decay=float(tcfg.get("weight_decay", 0.01)),
                              state_bits=int(tcfg.get("optimizer_state_bits", 32)))
-        raise ValueError(f"train.optimizer: Adam or AdamW, not {tcfg.get('optimizer')!r}")
+        if kind != "adam":
+            self.logger.warning(f"train.optimizer {tcfg['optimizer']!r} is neither Adam nor AdamW: Adam is used")
+        return FlatAdam(net, lr, betas=betas, big_numel=big, shadow_big=shadow_big)
 
     # ---- data parallel ------------------------------------------------------------------
     def _broadcast_initial_state(self):

@@ -441,6 +441,18 @@ def test_trainer_option(bits, tmp_path):
         other.load_checkpoint(str(tmp_path / "c.pt"))
 
 
+@pytest.mark.gpu
+def test_trainer_without_the_option(caplog):
+    """Adam as before, with any other value of a key that was not read before."""
+    sf = load_pkg()
+    training = importlib.import_module(sf.__name__ + ".training")
+    for value, warns in ((None, False), ("adam", False), ("SGD", True)):
+        caplog.clear()
+        tr = training.Trainer(tiny_config(**({} if value is None else {"optimizer": value})), device="cuda:0")
+        assert type(tr.opt_g) is training.FlatAdam and type(tr.opt_d) is training.FlatAdam
+        assert any("neither Adam nor AdamW" in r.getMessage() for r in caplog.records) == warns
+
+
 def test_hash_spreads():
     """The rounding bits over 2^16 consecutive elements, per tensor and step: each half's mean and variance are
     those of a uniform number to 5 standard deviations, and different steps, tensors and halves do not correlate."""
