@@ -1007,51 +1007,67 @@ int check_align(const void* const* ps, int n, const char* who) {
 }
 
 // How a launch's work items are cut.  The chip runs `slots` workgroups at a time; items beyond a whole number of rounds
-// would leave most of it idle in the last one.  Those are cut into the number of parts for which the last rounds take
-// the least time, counted in quarters of an inner tile (about 1 us in bf16, 2 to 6 us in f32, whose matrix rate is a
-// sixteenth): what a part costs by itself, and about 10 us for the launch that joins them.
-// Causal items that fill the chip are not cut: they come longest first, the last ones are short.
-struct Cut { int full, tail, parts; };
-Cut cut_items(long long items, int slots, int tiles, bool f32, bool causal) {
+// would leave most of it idle in the last one.  Those are cut into the number of parts for which the launch takes the
+// least time, counted in quarters of a tile of 128 rows and 64 (f32: 32) keys, 0.5 to 1.5 us: `unit` for a step, `fixed` for what a
+// part costs by itself, `join` for the launch that joins them (from sweeps of 22 shapes for each type and width).  The time is
+// that of whole rounds of the longest item.  In f32 a round is 256 workgroups: one keeps a CU's matrix pipes busy, others on the
+// same CU share them.  There narrow causal items, which have on average a `share` of the longest one's steps and come
+// longest first, take the time of the longest or of all the work, whichever is more.
+// Items of unequal length that fill the chip are not cut: they come longest first, the last ones are short.
+struct Cut { int full, tail, parts; double cost; };
+int width_of(const sf_diff_attn_desc* p) { return p->d <= 16 ? 0 : p->d <= 32 ? 1 : 2; }
+Cut cut_items(const sf_diff_attn_desc* p, long long items, int slots, int steps, int unit, int fixed) {
+    static const int joins[2][3] = {{48, 32, 32}, {32, 16, 16}};
+    const bool f32 = p->dtype == SF_F32;
+    const int join = joins[f32][width_of(p)];
+    const double share = !p->causal ? 1 : p->Tq <= p->Tk ? 1 - (p->Tq - 1) / (2.0 * p->Tk) : (p->Tk + 1) / (2.0 * p->Tq);
+    const bool rounds = !f32 || p->d > 32 || share >= 0.9;
+    const int round = f32 ? 256 : slots;
+    auto time = [&](long long n, int len) {
+        const double one = (double)unit * len + fixed, all = n / 256.0 * (unit * len * share + fixed);
+        return rounds ? (n + round - 1) / round * one : all > one ? all : one;
+    };
     const long long full = items / slots * slots, tail = items - full;
-    if (!tail || (causal && full)) return {(int)items, 0, 1};
-    long long best = 0;
-    int parts = 0;
-    for (int p = 1; p <= 64 && (p == 1 || tiles / p >= 2); ++p) {
-        const long long rounds = (tail * p + slots - 1) / slots;
-        const long long cost = rounds * (4 * ((tiles + p - 1) / p) + 4) + (p > 1 ? (f32 ? 16 : 32) : 0);
-        if (!parts || cost < best) { best = cost; parts = p; }
+    Cut best{(int)items, 0, 1, time(items, steps)};
+    if (!tail || (full && share < 0.9)) return best;
+    const double before = full ? time(full, steps) : 0;
+    for (int n = 2; n <= 64 && steps / n >= 2; ++n) {
+        const double cost = before + time(tail * n, (steps + n - 1) / n) + join;
+        if (cost < best.cost) best = {(int)full, (int)tail, n, cost};
     }
-    if (parts == 1) return {(int)items, 0, 1};
-    return {(int)full, (int)tail, parts};
+    return best;
 }
-// workgroups that share a CU: what the kernels' registers (forward pass of single tokens: LDS) leave room for
+// workgroups that share a CU: what the kernels' registers (forward pass with split keys: LDS) leave room for
 enum Pass { FWD, FWD_KEYS, DQ, DKV };
 int slots_of(const sf_diff_attn_desc* p, Pass pass) {
     static const int bf16_[4][3] = {{4, 3, 2}, {4, 2, 2}, {3, 3, 2}, {3, 2, 2}}, f32_[4][3] = {{4, 2, 1}, {2, 1, 1}, {3, 2, 1}, {3, 2, 1}};
-    const int w = p->d <= 16 ? 0 : p->d <= 32 ? 1 : 2;
-    return 256 * (p->dtype == SF_F32 ? f32_ : bf16_)[pass][w];
+    return 256 * (p->dtype == SF_F32 ? f32_ : bf16_)[pass][width_of(p)];
 }
-// Up to 32 query rows per key/value head the waves of a workgroup share out the keys of a tile, beyond that the rows.
+int fixed_of(const sf_diff_attn_desc* p) { return p->dtype == SF_F32 && p->d > 32 ? 8 : 4; }
+// Up to 32 query rows per key/value head (single tokens) the waves of a workgroup share out the keys of a tile; beyond that the
+// rows, or the keys where the items are too few for the chip: four times the items, and the parts are joined in LDS
+// instead of by another launch.  (Forward, us, rows | keys: bf16 4 x 777 tokens, 4 heads on 2, causal, 2 x 16: 27 | 12, 2 x 64:
+// 34 | 24; 1 x 4096, 4 heads, 2 x 64: 78 | 102; f32 2 x 32: 4 x 777: 54 | 42, 1 x 4096: 224 | 245.)
 struct FwdPlan { bool keys; int kt, rb; Cut cut; };
 FwdPlan fwd_plan(const sf_diff_attn_desc* p) {
-    const long long rows = (long long)(p->H / p->Hk) * p->Tq;
+    const long long rows = (long long)(p->H / p->Hk) * p->Tq, heads = (long long)p->B * p->Hk;
     const bool f32 = p->dtype == SF_F32;
-    FwdPlan f;
-    f.keys = rows <= 32;
-    f.kt = f.keys ? (padded(p->d) == 64 ? 64 : 128) : f32 ? 32 : 64;
-    f.rb = f.keys ? 32 : 128;
-    f.cut = cut_items((rows + f.rb - 1) / f.rb * p->B * p->Hk, slots_of(p, f.keys ? FWD_KEYS : FWD), (p->Tk + f.kt - 1) / f.kt, f32,
-                      p->causal && !f.keys);
-    return f;
+    static const int fixed[2][3] = {{14, 14, 14}, {6, 12, 24}};
+    const int kt = padded(p->d) == 64 ? 64 : 128;
+    const FwdPlan keys{true, kt, 32, cut_items(p, (rows + 31) / 32 * heads, slots_of(p, FWD_KEYS), (p->Tk + kt - 1) / kt,
+                                               f32 ? 4 : 2, fixed[f32][width_of(p)])};
+    if (rows <= 32) return keys;
+    const int rt = f32 ? 32 : 64;
+    const FwdPlan split{false, rt, 128, cut_items(p, (rows + 127) / 128 * heads, slots_of(p, FWD), (p->Tk + rt - 1) / rt, 4, fixed_of(p))};
+    return keys.cut.cost < split.cut.cost ? keys : split;
 }
 Cut dq_cut(const sf_diff_attn_desc* p) {
     const long long rows = (long long)(p->H / p->Hk) * p->Tq;
-    return cut_items((rows + 127) / 128 * p->B * p->Hk, slots_of(p, DQ), (p->Tk + 63) / 64, p->dtype == SF_F32, p->causal);
+    const int kt = p->dtype == SF_F32 ? 32 : 64;
+    return cut_items(p, (rows + 127) / 128 * p->B * p->Hk, slots_of(p, DQ), (p->Tk + kt - 1) / kt, 4, fixed_of(p));
 }
 Cut dkv_cut(const sf_diff_attn_desc* p) {
-    return cut_items((long long)((p->Tk + 127) / 128) * p->B * p->Hk, slots_of(p, DKV), (p->Tq + 31) / 32 * (p->H / p->Hk),
-                     p->dtype == SF_F32, p->causal);
+    return cut_items(p, (long long)((p->Tk + 127) / 128) * p->B * p->Hk, slots_of(p, DKV), (p->Tq + 31) / 32 * (p->H / p->Hk), 4, fixed_of(p));
 }
 
 template <typename T> Args<T> make_args(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
