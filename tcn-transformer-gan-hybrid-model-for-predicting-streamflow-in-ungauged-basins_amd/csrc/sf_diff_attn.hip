@@ -631,12 +631,33 @@ __global__ __launch_bounds__(1024) void attn_dlam_kernel(const float* __restrict
     }
 }
 
-// Gradient of the queries: as the forward pass, 32 rows per wave, the keys tile by tile.  (8 bf16 heads of 2 x 64, 2 x 5120 tokens:
+// adds the accumulators of waves 1 .. NW - 1 to those of wave 0, one wave after the other, through LDS (N * 1024 floats)
+template <int NW, int N> __device__ __forceinline__ void join_waves(f32x16 (&acc)[N], float* box, int wave, int lane) {
+#pragma unroll 1
+    for (int u = 1; u < NW; ++u) {
+        __syncthreads();
+        if (wave == u) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) box[(n * 16 + r) * 64 + lane] = acc[n][r];
+        }
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[n][r] += box[(n * 16 + r) * 64 + lane];
+        }
+    }
+}
+
+// Gradient of the queries: as the forward pass, rows (32 per wave) or the keys of a tile shared out.  (8 bf16 heads of 2 x 64, 2 x 5120 tokens:
 // 347 to 380 us, 322 GFLOP, 0.88 PFLOP/s; bound as the forward pass.)
-template <typename T, int DP, int KT>
-__global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a) {
+template <typename T, int DP, int NW, bool KEYS_SPLIT, int KT>
+__global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a) {
     using L = Tile<T, DP>;
-    constexpr int NW = 4, RB = 32 * NW, KS = DP / 16, VS = 2 * DP / 16;
+    constexpr int RB = KEYS_SPLIT ? 32 : 32 * NW, KS = DP / 16, VS = 2 * DP / 16;
     constexpr int NA = DP == 16 ? 2 : 2 * DP / 32;         // accumulators: 32 columns each (DP = 16: both halves in each)
     constexpr int TB = L::bytes(KT);
     extern __shared__ __align__(16) char smem[];
@@ -649,7 +670,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a)
     locate(w.item, a.B * a.Hk, tiles, a.causal, bh, x);
     const int rt = tiles - 1 - x;
     const int b = bh / a.Hk, hk = bh % a.Hk;
-    const long long r0 = (long long)rt * RB, row = r0 + wave * 32 + (lane & 31);
+    const long long r0 = (long long)rt * RB, row = r0 + (KEYS_SPLIT ? 0 : wave * 32) + (lane & 31);
     const bool have = row < rows;
     const long long rr = have ? row : rows - 1;
     const int t = (int)(rr / group), hq = hk * group + (int)(rr % group);
@@ -726,8 +747,12 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a)
             kc.issue(kbase + (i + 1) * KT * a.ks.t, kend - (i + 1) * KT, fill);
             vc.issue(vbase + (i + 1) * KT * a.vs.t, kend - (i + 1) * KT, fill + TB);
         }
+        if constexpr (KEYS_SPLIT) {
+            sub_tile(cur, cur + TB, wave * 32, i * KT + wave * 32);
+        } else {
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) sub_tile(cur, cur + TB, u * 32, i * KT + u * 32);
+            for (int u = 0; u < KT / 32; ++u) sub_tile(cur, cur + TB, u * 32, i * KT + u * 32);
+        }
     };
     if (first < last) {
         kc.issue(kbase + first * KT * a.ks.t, kend - first * KT, buf0);
@@ -740,6 +765,10 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a)
             step(i, buf1, buf0);
             if (++i >= last) break;
         }
+    }
+    if constexpr (KEYS_SPLIT) {
+        join_waves<NW>(acc, (float*)smem, wave, lane);
+        if (wave != 0) return;
     }
     if (!have) return;
 #pragma unroll
@@ -953,8 +982,8 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
 }
 
 // adds the parts of the gradient items that were cut, in order: one wave per row (KEYS false: dq) or key (KEYS true: dv and dk)
-template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void attn_join_grad_kernel(Args<T> a, int items) {
-    constexpr int RB = 128, W = KEYS ? 4 * DP : 2 * DP;
+template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void attn_join_grad_kernel(Args<T> a, int items, int RB) {
+    constexpr int W = KEYS ? 4 * DP : 2 * DP;
     const int lane = threadIdx.x & 63, group = a.H / a.Hk;
     const long long rows = KEYS ? a.Tk : (long long)group * a.Tq, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int tail = (int)(id / RB), tiles = (int)((rows + RB - 1) / RB);
@@ -1037,10 +1066,11 @@ Cut cut_items(const sf_diff_attn_desc* p, long long items, int slots, int steps,
     }
     return best;
 }
-// workgroups that share a CU: what the kernels' registers (forward pass with split keys: LDS) leave room for
-enum Pass { FWD, FWD_KEYS, DQ, DKV };
+// workgroups that share a CU: what the kernels' registers (with split keys: LDS) leave room for
+enum Pass { FWD, FWD_KEYS, DQ, DQ_KEYS, DKV };
 int slots_of(const sf_diff_attn_desc* p, Pass pass) {
-    static const int bf16_[4][3] = {{4, 3, 2}, {4, 2, 2}, {3, 3, 2}, {3, 2, 2}}, f32_[4][3] = {{4, 2, 1}, {2, 1, 1}, {3, 2, 1}, {3, 2, 1}};
+    static const int bf16_[5][3] = {{4, 3, 2}, {4, 2, 2}, {3, 3, 2}, {3, 2, 2}, {3, 2, 2}},
+                     f32_[5][3] = {{4, 2, 1}, {2, 1, 1}, {3, 2, 1}, {2, 1, 1}, {3, 2, 1}};
     return 256 * (p->dtype == SF_F32 ? f32_ : bf16_)[pass][width_of(p)];
 }
 int fixed_of(const sf_diff_attn_desc* p) { return p->dtype == SF_F32 && p->d > 32 ? 8 : 4; }
@@ -1048,24 +1078,21 @@ int fixed_of(const sf_diff_attn_desc* p) { return p->dtype == SF_F32 && p->d > 3
 // rows, or the keys where the items are too few for the chip: four times the items, and the parts are joined in LDS
 // instead of by another launch.  (Forward, us, rows | keys: bf16 4 x 777 tokens, 4 heads on 2, causal, 2 x 16: 27 | 12, 2 x 64:
 // 34 | 24; 1 x 4096, 4 heads, 2 x 64: 78 | 102; f32 2 x 32: 4 x 777: 54 | 42, 1 x 4096: 224 | 245.)
-struct FwdPlan { bool keys; int kt, rb; Cut cut; };
-FwdPlan fwd_plan(const sf_diff_attn_desc* p) {
+struct RowPlan { bool keys; int kt, rb; Cut cut; };
+RowPlan row_plan(const sf_diff_attn_desc* p, Pass rows_pass, Pass keys_pass) {
     const long long rows = (long long)(p->H / p->Hk) * p->Tq, heads = (long long)p->B * p->Hk;
     const bool f32 = p->dtype == SF_F32;
     static const int fixed[2][3] = {{14, 14, 14}, {6, 12, 24}};
     const int kt = padded(p->d) == 64 ? 64 : 128;
-    const FwdPlan keys{true, kt, 32, cut_items(p, (rows + 31) / 32 * heads, slots_of(p, FWD_KEYS), (p->Tk + kt - 1) / kt,
+    const RowPlan keys{true, kt, 32, cut_items(p, (rows + 31) / 32 * heads, slots_of(p, keys_pass), (p->Tk + kt - 1) / kt,
                                                f32 ? 4 : 2, fixed[f32][width_of(p)])};
     if (rows <= 32) return keys;
     const int rt = f32 ? 32 : 64;
-    const FwdPlan split{false, rt, 128, cut_items(p, (rows + 127) / 128 * heads, slots_of(p, FWD), (p->Tk + rt - 1) / rt, 4, fixed_of(p))};
+    const RowPlan split{false, rt, 128, cut_items(p, (rows + 127) / 128 * heads, slots_of(p, rows_pass), (p->Tk + rt - 1) / rt, 4, fixed_of(p))};
     return keys.cut.cost < split.cut.cost ? keys : split;
 }
-Cut dq_cut(const sf_diff_attn_desc* p) {
-    const long long rows = (long long)(p->H / p->Hk) * p->Tq;
-    const int kt = p->dtype == SF_F32 ? 32 : 64;
-    return cut_items(p, (rows + 127) / 128 * p->B * p->Hk, slots_of(p, DQ), (p->Tk + kt - 1) / kt, 4, fixed_of(p));
-}
+RowPlan fwd_plan(const sf_diff_attn_desc* p) { return row_plan(p, FWD, FWD_KEYS); }
+RowPlan dq_plan(const sf_diff_attn_desc* p) { return row_plan(p, DQ, DQ_KEYS); }
 Cut dkv_cut(const sf_diff_attn_desc* p) {
     return cut_items(p, (long long)((p->Tk + 127) / 128) * p->B * p->Hk, slots_of(p, DKV), (p->Tq + 31) / 32 * (p->H / p->Hk), 4, fixed_of(p));
 }
@@ -1101,7 +1128,7 @@ template <typename K> int allow_lds(K kernel, int bytes) {
         }                                                             \
     } while (0)
 
-template <typename T, int DP> int launch_fwd(Args<T> a, const FwdPlan& f, hipStream_t st) {
+template <typename T, int DP> int launch_fwd(Args<T> a, const RowPlan& f, hipStream_t st) {
     const int grid = f.cut.full + f.cut.tail * f.cut.parts;
     using L = Tile<T, DP>;
     a.full = f.cut.full;
@@ -1125,21 +1152,28 @@ template <typename T, int DP> int launch_fwd(Args<T> a, const FwdPlan& f, hipStr
     return SF_OK;
 }
 
-template <typename T, int DP> int launch_bwd(Args<T> a, const Cut& cq, const Cut& ck, hipStream_t st) {
+template <typename T, int DP> int launch_bwd(Args<T> a, const RowPlan& f, const Cut& ck, hipStream_t st) {
     const long long n = (long long)a.B * a.Tp * a.H;
     using L = Tile<T, DP>;
-    constexpr int KT = sizeof(T) == 4 ? 32 : 64;
     hipLaunchKernelGGL((attn_delta_kernel<T>), dim3(ceil_div(n, 16)), dim3(256), 0, st, a);
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (delta)");
-    constexpr int lds_q = 4 * L::bytes(KT);
     constexpr int lds_k = L::bytes(128) + 2 * (2 * L::bytes(32) + 1024);
-    SF_LDS_ONCE((attn_dq_kernel<T, DP, KT>), lds_q);
+    const Cut& cq = f.cut;
     a.full = cq.full;
     a.parts = cq.parts;
-    hipLaunchKernelGGL((attn_dq_kernel<T, DP, KT>), dim3(cq.full + cq.tail * cq.parts), dim3(256), lds_q, st, a);
+    if (f.keys) {
+        constexpr int NW = DP == 64 ? 2 : 4, KT = 32 * NW, box = (DP == 16 ? 2 : 2 * DP / 32) * 4096;
+        constexpr int lds = 4 * L::bytes(KT) > box ? 4 * L::bytes(KT) : box;
+        SF_LDS_ONCE((attn_dq_kernel<T, DP, NW, true, KT>), lds);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, NW, true, KT>), dim3(cq.full + cq.tail * cq.parts), dim3(64 * NW), lds, st, a);
+    } else {
+        constexpr int KT = sizeof(T) == 4 ? 32 : 64, lds = 4 * L::bytes(KT);
+        SF_LDS_ONCE((attn_dq_kernel<T, DP, 4, false, KT>), lds);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, 4, false, KT>), dim3(cq.full + cq.tail * cq.parts), dim3(256), lds, st, a);
+    }
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (queries)");
     if (cq.tail) {
-        hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, false>), dim3(cq.tail * 32), dim3(256), 0, st, a, cq.tail);
+        hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, false>), dim3(cq.tail * f.rb / 4), dim3(256), 0, st, a, cq.tail, f.rb);
         SF_LAUNCH_CHECK("sf_diff_attn_bwd (queries, join)");
     }
     SF_LDS_ONCE((attn_dkv_kernel<T, DP>), lds_k);
@@ -1148,7 +1182,7 @@ template <typename T, int DP> int launch_bwd(Args<T> a, const Cut& cq, const Cut
     hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(ck.full + ck.tail * ck.parts), dim3(256), lds_k, st, a);
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (keys)");
     if (ck.tail) {
-        hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, true>), dim3(ck.tail * 32), dim3(256), 0, st, a, ck.tail);
+        hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, true>), dim3(ck.tail * 32), dim3(256), 0, st, a, ck.tail, 128);
         SF_LAUNCH_CHECK("sf_diff_attn_bwd (keys, join)");
     }
     return SF_OK;
@@ -1158,7 +1192,7 @@ template <typename T> int fwd(const sf_diff_attn_desc* p, const void* q, const v
                               const int* lengths, void* o, float* maps, float* lse, float* part, hipStream_t st) {
     Args<T> a = make_args<T>(p, q, k, v, lam, lengths);
     a.o = (T*)o; a.maps = maps; a.lse = lse; a.part = part;
-    const FwdPlan f = fwd_plan(p);
+    const RowPlan f = fwd_plan(p);
     const int dp = padded(p->d);
     return dp == 16 ? launch_fwd<T, 16>(a, f, st) : dp == 32 ? launch_fwd<T, 32>(a, f, st) : launch_fwd<T, 64>(a, f, st);
 }
@@ -1172,7 +1206,8 @@ template <typename T> int bwd(const sf_diff_attn_desc* p, const void* q, const v
     a.part = (float*)(ws + stat_bytes(p));
     a.dq = (T*)dq; a.dk = (T*)dk; a.dv = (T*)dv;
     const int dp = padded(p->d);
-    const Cut cq = dq_cut(p), ck = dkv_cut(p);
+    const RowPlan cq = dq_plan(p);
+    const Cut ck = dkv_cut(p);
     if (int rc = dp == 16 ? launch_bwd<T, 16>(a, cq, ck, st) : dp == 32 ? launch_bwd<T, 32>(a, cq, ck, st) : launch_bwd<T, 64>(a, cq, ck, st))
         return rc;
     if (dlam) {
@@ -1186,7 +1221,7 @@ template <typename T> int bwd(const sf_diff_attn_desc* p, const void* q, const v
 
 extern "C" size_t sf_diff_attn_fwd_workspace_bytes(const sf_diff_attn_desc* p) {
     if (check_desc(p, "sf_diff_attn_fwd_workspace_bytes")) return 0;
-    const FwdPlan f = fwd_plan(p);
+    const RowPlan f = fwd_plan(p);
     return (size_t)f.cut.tail * f.cut.parts * f.rb * (4 * padded(p->d) + 4) * sizeof(float);
 }
 
@@ -1205,9 +1240,10 @@ extern "C" int sf_diff_attn_fwd(const sf_diff_attn_desc* p, const void* q, const
 
 extern "C" size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* p) {
     if (check_desc(p, "sf_diff_attn_bwd_workspace_bytes")) return 0;
-    const Cut cq = dq_cut(p), ck = dkv_cut(p);
-    const size_t q = (size_t)cq.tail * cq.parts * 2, k = (size_t)ck.tail * ck.parts * 4;      // (one after the other in the same place)
-    return stat_bytes(p) + (q > k ? q : k) * 128 * padded(p->d) * sizeof(float);
+    const RowPlan f = dq_plan(p);
+    const Cut ck = dkv_cut(p);
+    const size_t q = (size_t)f.cut.tail * f.cut.parts * f.rb * 2, k = (size_t)ck.tail * ck.parts * 128 * 4;
+    return stat_bytes(p) + (q > k ? q : k) * padded(p->d) * sizeof(float);        // (one after the other in the same place)
 }
 
 extern "C" int sf_diff_attn_bwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
