@@ -212,9 +212,9 @@ template <typename T> struct Args {
     T* o; float* maps; float* lse;          // maps f32 [B,Tq,H,2,2d] = O_1, O_2; lse f32 [B,H,Tq,2] (base 2): for the backward pass
     float* part;                            // partial results of the work items that are cut
     const T* dout; const float* maps_in; const float* lse_in;
-    float* stat;                            // [B,H,4,Tp]: lse_1, delta_1, lse_2, delta_2; zeros from Tq to Tp
+    float* stat;                            // [B,H,STATS,Tp], see attn_delta_kernel; zeros from Tq to Tp
     T* dq; T* dk; T* dv;
-    int lam_bf16, B, Tq, Tp, Tk, H, Hk, d, causal;        // Tp: Tq rounded up to 64
+    int lam_bf16, B, Tq, Tp, Tk, H, Hk, d, causal;        // Tp: Tq rounded up to whole tiles of any kernel
     int full, parts;                        // see Cut
     float scale, c;                         // c = scale * log2(e)
 };
@@ -786,18 +786,18 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
 }
 
 // Gradients of the keys and values: a wave owns 32 keys, the workgroup's 128 keys meet the query rows of every head of the
-// group tile by tile.  The wave's keys stay in registers, the values in LDS.  bf16 heads of 2 x 64: with 128 accumulators and
+// group tile by tile.  SPLIT: the workgroup has 32 keys and the waves share out the rows of a tile; joined through LDS at the end.  The wave's keys stay in registers, the values in LDS.  bf16 heads of 2 x 64: with 128 accumulators and
 // 32 registers of keys little is left of the 256 that two waves per SIMD have, and a spilled one is reloaded behind the copies
 // under way.  So a lane keeps two address registers for its row pieces and two for its column pieces and makes the
 // others where it uses them (fresh), and the maps come one after the other: no spill in the loop (2 x 5120 tokens, 8 heads:
 // 725 us with 13 spills, 592 us without; eight waves in pairs, with the keys in LDS too, 635 us).  539 to 600 us now, 429 GFLOP,
 // 0.75 PFLOP/s: the matrix pipe is busy 38 % of the time, LDS reads 34 %, and no registers are left to fetch operands ahead.
-template <typename T, int DP>
-__global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a) {
+template <typename T, int DP, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a) {
     using L = Tile<T, DP>;
-    constexpr int NW = 4, KB = 128, QT = 32, KS = DP / 16, VS = 2 * DP / 16, DT = 2 * DP / 32;
+    constexpr int KB = SPLIT ? 32 : 32 * NW, QT = SPLIT ? 32 * NW : 32, KS = DP / 16, VS = 2 * DP / 16, DT = 2 * DP / 32;
     constexpr int NA = DP == 16 ? 2 : DT;
-    constexpr int TB = L::bytes(QT), SB = 1024;            // query / gradient tile; row statistics (16 QT bytes, copied by a wave)
+    constexpr int TB = L::bytes(QT), SB = QT <= 64 ? 1024 : 16 * QT;     // query / gradient tile; row statistics (copies of 1 KB)
     constexpr int BUF = 2 * TB + SB;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h2 = lane >> 5;
@@ -807,10 +807,11 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
     int bh, x;
     locate(w.item, a.B * a.Hk, tiles, a.causal, bh, x);
     const int b = bh / a.Hk, hk = bh % a.Hk, k0 = x * KB;
-        const int key = k0 + wave * 32 + (lane & 31);
+        const int kw = SPLIT ? 0 : wave * 32, rows0 = SPLIT ? wave * 32 : 0;       // the wave's keys, and its rows of a tile
+    const int key = k0 + kw + (lane & 31);
     const int kend = keys_of(a, b), reach = a.Tk - a.Tq;
     const int t_min = key >= kend ? 1 << 30 : a.causal ? key - reach : 0;  // the key is seen by queries from t_min on
-    const int w_first = k0 + wave * 32;                                    // the wave's first key
+    const int w_first = k0 + kw;                                    // the wave's first key
     const int w_tmax = a.causal ? w_first + 31 - reach : 0;                // queries from here on see all keys of the wave
     const int q_first = a.causal ? max(0, k0 - reach) / QT : 0;            // first query tile that sees a key of the workgroup
     const int q_tiles = (a.Tq + QT - 1) / QT;
@@ -843,10 +844,11 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
         const int have = a.Tq - pos.tile * QT;
         q_copy.issue(pos.q, have, dst);
         g_copy.issue(pos.g, have, dst + TB);
-        if (wave == 0) {
+        if (wave * 64 < QT) {
             const __amdgpu_buffer_rsrc_t rs =
                 __builtin_amdgcn_make_buffer_rsrc((void*)pos.stat, 0, (unsigned)(3 * a.Tp + QT) * 4u, 0x00020000);
-            copy_piece(rs, dst + 2 * TB, lane < QT ? lane / (QT / 4) * a.Tp * 4 + lane % (QT / 4) * 16 : (int)0x80000000, 0);
+            const int piece = wave * 64 + lane;
+            copy_piece(rs, dst + 2 * TB + wave * 1024, piece < QT ? piece / (QT / 4) * a.Tp * 4 + piece % (QT / 4) * 16 : (int)0x80000000, 0);
         }
         if (pos.tile + 1 == q_tiles) {
             go_to(pos.head + 1, q_first);       // (behind the last head nothing is read any more)
@@ -867,13 +869,13 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
         return typename L::Lane{l.part + off, l.mix};
     };
     auto step = [&](bool more, lds_cptr __restrict__ cur, lds_ptr __restrict__ fill) {
-        const int t0 = tile * QT, hq = hk * group + head;
+        const int t0 = tile * QT + rows0, hq = hk * group + head;
         if (++tile == q_tiles) { tile = q_first; ++head; }
         if (more) issue(fill);
         if (w_first >= kend || (a.causal && t0 + 31 + reach < w_first)) return;     // nothing of this wave is seen
         const float lam = lam_of(a.lam, a.lam_bf16, hq);
         lds_cptr const gt = cur + TB;
-        const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB);            // [STATS - 1][QT]
+        const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB) + rows0;            // [STATS - 1][QT]
         const bool edge = w_first + 32 > kend || (a.causal && t0 < w_tmax);
         f32x16 dp;                      // dP - delta_1
 #pragma unroll
@@ -882,7 +884,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
 #pragma unroll
             for (int e = 0; e < 4; ++e) dp[r + e] = dl[e];
         }
-        const typename L::Lane gl = fresh(rl, 0), vl = fresh(rl, L::row_off(wave * 32));
+        const typename L::Lane gl = fresh(rl, L::row_off(rows0)), vl = fresh(rl, L::row_off(kw));
 #pragma unroll
         for (int n = 0; n < VS; ++n) {
             if (n && n % 4 == 0) __builtin_amdgcn_sched_barrier(0);
@@ -893,7 +895,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
         for (int i = 0; i < 2; ++i) {
             __builtin_amdgcn_sched_barrier(0);          // (one map after the other: fewer operands in flight)
             f32x16 s = zero16();
-            const typename L::Lane ql = fresh(rl, 0);
+            const typename L::Lane ql = fresh(rl, L::row_off(rows0));
 #pragma unroll
             for (int n = 0; n < KS; ++n) s = mma(L::row_piece(cur, ql, 0, i * KS + n), kf[i][n], s);
             if (edge) {
@@ -919,7 +921,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
                 }
                 pack(df[u], ds);
             }
-            const typename L::Lane qc = fresh(cl, 0);
+            const typename L::Lane qc = fresh(cl, L::row_off(rows0));
 #pragma unroll
             for (int n = 0; n < NA / 2; ++n)
 #pragma unroll
@@ -934,7 +936,7 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
             for (int j = 0; j < 8; ++j) x[j] = p[8 * u + j];
             pack(pf[u], x);
         }
-        const typename L::Lane gc = fresh(cl, 0);
+        const typename L::Lane gc = fresh(cl, L::row_off(rows0));
 #pragma unroll
         for (int n = 0; n < DT; ++n)
 #pragma unroll
@@ -957,6 +959,11 @@ __global__ __launch_bounds__(256, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a
             step(i + 1 < last, buf1, buf0);
             if (++i >= last) break;
         }
+    }
+    if constexpr (SPLIT) {
+        join_waves<NW>(dv, (float*)smem, wave, lane);
+        join_waves<NW>(dk, (float*)smem, wave, lane);
+        if (wave != 0) return;
     }
     if (key >= a.Tk) return;
     const long long out = (((long long)b * a.Tk + key) * a.Hk + hk) * (2 * a.d);
@@ -1007,6 +1014,7 @@ template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void 
 }
 
 // ------------------------------------------------------------------------------ host side
+int padded_rows(const sf_diff_attn_desc* p) { return (p->Tq + 127) / 128 * 128; }
 int padded(int d) { return d <= 16 ? 16 : d <= 32 ? 32 : 64; }
 
 int check_desc(const sf_diff_attn_desc* p, const char* who) {
@@ -1027,7 +1035,7 @@ int check_desc(const sf_diff_attn_desc* p, const char* who) {
         SF_REQUIRE(i % 3 != 1 || (s >= 2 * p->d && s < (1 << 22)), "%s: token stride %lld (a head has %d values)", who, s, 2 * p->d);
     }
     const double groups = (double)p->B * p->Hk * (((double)p->H / p->Hk * p->Tq + 31) / 32 + (p->Tk + 127) / 128);
-    SF_REQUIRE(groups < 1e8 && (double)p->B * ((p->Tq + 63) / 64 * 64) * p->H < 2e9, "%s: too many rows", who);
+    SF_REQUIRE(groups < 1e8 && (double)p->B * padded_rows(p) * p->H < 2e9, "%s: too many rows", who);
     return SF_OK;
 }
 int check_align(const void* const* ps, int n, const char* who) {
@@ -1067,10 +1075,10 @@ Cut cut_items(const sf_diff_attn_desc* p, long long items, int slots, int steps,
     return best;
 }
 // workgroups that share a CU: what the kernels' registers (with split keys: LDS) leave room for
-enum Pass { FWD, FWD_KEYS, DQ, DQ_KEYS, DKV };
+enum Pass { FWD, FWD_KEYS, DQ, DQ_KEYS, DKV, DKV_SPLIT };
 int slots_of(const sf_diff_attn_desc* p, Pass pass) {
-    static const int bf16_[5][3] = {{4, 3, 2}, {4, 2, 2}, {3, 3, 2}, {3, 2, 2}, {3, 2, 2}},
-                     f32_[5][3] = {{4, 2, 1}, {2, 1, 1}, {3, 2, 1}, {2, 1, 1}, {3, 2, 1}};
+    static const int bf16_[6][3] = {{4, 3, 2}, {4, 2, 2}, {3, 3, 2}, {3, 2, 2}, {3, 2, 2}, {3, 2, 2}},
+                     f32_[6][3] = {{4, 2, 1}, {2, 1, 1}, {3, 2, 1}, {2, 1, 1}, {3, 2, 1}, {2, 1, 1}};
     return 256 * (p->dtype == SF_F32 ? f32_ : bf16_)[pass][width_of(p)];
 }
 int fixed_of(const sf_diff_attn_desc* p) { return p->dtype == SF_F32 && p->d > 32 ? 8 : 4; }
@@ -1093,8 +1101,19 @@ RowPlan row_plan(const sf_diff_attn_desc* p, Pass rows_pass, Pass keys_pass) {
 }
 RowPlan fwd_plan(const sf_diff_attn_desc* p) { return row_plan(p, FWD, FWD_KEYS); }
 RowPlan dq_plan(const sf_diff_attn_desc* p) { return row_plan(p, DQ, DQ_KEYS); }
-Cut dkv_cut(const sf_diff_attn_desc* p) {
-    return cut_items(p, (long long)((p->Tk + 127) / 128) * p->B * p->Hk, slots_of(p, DKV), (p->Tq + 31) / 32 * (p->H / p->Hk), 4, fixed_of(p));
+// The key gradients likewise: 128 keys, 32 for each wave, or 32 keys and the rows of a tile shared out.  (Backward pass, us, keys |
+// split: bf16 2 x 365 tokens, 4 heads, 2 x 16: 30 | 21, 2 x 64: 44 | 36; 1 x 512, 8 heads, 2 x 32: 36 | 25; f32 8 x 300, 4 heads,
+// causal, 2 x 16: 69 | 45.)
+struct KeyPlan { bool split; int kb, qt; Cut cut; };
+KeyPlan dkv_plan(const sf_diff_attn_desc* p) {
+    const bool f32 = p->dtype == SF_F32;
+    static const int fixed[2][3] = {{18, 18, 18}, {8, 14, 26}};
+    const int group = p->H / p->Hk, heads = p->B * p->Hk, qt = padded(p->d) == 64 ? 64 : 128, unit = f32 ? 4 : 3;
+    const KeyPlan split{true, 32, qt, cut_items(p, (long long)((p->Tk + 31) / 32) * heads, slots_of(p, DKV_SPLIT), (p->Tq + qt - 1) / qt * group,
+                                                unit, fixed[f32][width_of(p)])};
+    const KeyPlan keys{false, 128, 32, cut_items(p, (long long)((p->Tk + 127) / 128) * heads, slots_of(p, DKV), (p->Tq + 31) / 32 * group, unit,
+                                                 fixed_of(p))};
+    return split.cut.cost < keys.cut.cost ? split : keys;
 }
 
 template <typename T> Args<T> make_args(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
@@ -1105,7 +1124,7 @@ template <typename T> Args<T> make_args(const sf_diff_attn_desc* p, const void* 
     a.ks = {p->k_stride[0], p->k_stride[1], p->k_stride[2]};
     a.vs = {p->v_stride[0], p->v_stride[1], p->v_stride[2]};
     a.lam = lam; a.lam_bf16 = p->lam_dtype == SF_BF16; a.lengths = lengths;
-    a.B = p->B; a.Tq = p->Tq; a.Tp = (p->Tq + 63) / 64 * 64; a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.d = p->d; a.causal = p->causal != 0;
+    a.B = p->B; a.Tq = p->Tq; a.Tp = padded_rows(p); a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.d = p->d; a.causal = p->causal != 0;
     a.parts = 1;
     a.scale = p->scale;
     a.c = (float)((double)p->scale * 1.4426950408889634);
@@ -1152,12 +1171,11 @@ template <typename T, int DP> int launch_fwd(Args<T> a, const RowPlan& f, hipStr
     return SF_OK;
 }
 
-template <typename T, int DP> int launch_bwd(Args<T> a, const RowPlan& f, const Cut& ck, hipStream_t st) {
+template <typename T, int DP> int launch_bwd(Args<T> a, const RowPlan& f, const KeyPlan& g, hipStream_t st) {
     const long long n = (long long)a.B * a.Tp * a.H;
     using L = Tile<T, DP>;
     hipLaunchKernelGGL((attn_delta_kernel<T>), dim3(ceil_div(n, 16)), dim3(256), 0, st, a);
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (delta)");
-    constexpr int lds_k = L::bytes(128) + 2 * (2 * L::bytes(32) + 1024);
     const Cut& cq = f.cut;
     a.full = cq.full;
     a.parts = cq.parts;
@@ -1176,13 +1194,22 @@ template <typename T, int DP> int launch_bwd(Args<T> a, const RowPlan& f, const 
         hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, false>), dim3(cq.tail * f.rb / 4), dim3(256), 0, st, a, cq.tail, f.rb);
         SF_LAUNCH_CHECK("sf_diff_attn_bwd (queries, join)");
     }
-    SF_LDS_ONCE((attn_dkv_kernel<T, DP>), lds_k);
+    const Cut& ck = g.cut;
     a.full = ck.full;
     a.parts = ck.parts;
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(ck.full + ck.tail * ck.parts), dim3(256), lds_k, st, a);
+    if (g.split) {
+        constexpr int NW = DP == 64 ? 2 : 4, QT = 32 * NW, lds = L::bytes(32) + 2 * (2 * L::bytes(QT) + 16 * (QT < 64 ? 64 : QT));
+        static_assert(lds >= (2 * DP / 32 < 2 ? 2 : 2 * DP / 32) * 4096, "the waves' box");
+        SF_LDS_ONCE((attn_dkv_kernel<T, DP, NW, true>), lds);
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP, NW, true>), dim3(ck.full + ck.tail * ck.parts), dim3(64 * NW), lds, st, a);
+    } else {
+        constexpr int lds = L::bytes(128) + 2 * (2 * L::bytes(32) + 1024);
+        SF_LDS_ONCE((attn_dkv_kernel<T, DP, 4, false>), lds);
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP, 4, false>), dim3(ck.full + ck.tail * ck.parts), dim3(256), lds, st, a);
+    }
     SF_LAUNCH_CHECK("sf_diff_attn_bwd (keys)");
     if (ck.tail) {
-        hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, true>), dim3(ck.tail * 32), dim3(256), 0, st, a, ck.tail, 128);
+        hipLaunchKernelGGL((attn_join_grad_kernel<T, DP, true>), dim3(ck.tail * g.kb / 4), dim3(256), 0, st, a, ck.tail, g.kb);
         SF_LAUNCH_CHECK("sf_diff_attn_bwd (keys, join)");
     }
     return SF_OK;
@@ -1196,7 +1223,7 @@ template <typename T> int fwd(const sf_diff_attn_desc* p, const void* q, const v
     const int dp = padded(p->d);
     return dp == 16 ? launch_fwd<T, 16>(a, f, st) : dp == 32 ? launch_fwd<T, 32>(a, f, st) : launch_fwd<T, 64>(a, f, st);
 }
-size_t stat_bytes(const sf_diff_attn_desc* p) { return (size_t)p->B * p->H * ((p->Tq + 63) / 64 * 64) * STATS * sizeof(float); }
+size_t stat_bytes(const sf_diff_attn_desc* p) { return (size_t)p->B * p->H * padded_rows(p) * STATS * sizeof(float); }
 template <typename T> int bwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
                               const int* lengths, const float* maps, const float* lse, const void* dout, void* dq, void* dk,
                               void* dv, void* dlam, char* ws, hipStream_t st) {
@@ -1207,7 +1234,7 @@ template <typename T> int bwd(const sf_diff_attn_desc* p, const void* q, const v
     a.dq = (T*)dq; a.dk = (T*)dk; a.dv = (T*)dv;
     const int dp = padded(p->d);
     const RowPlan cq = dq_plan(p);
-    const Cut ck = dkv_cut(p);
+    const KeyPlan ck = dkv_plan(p);
     if (int rc = dp == 16 ? launch_bwd<T, 16>(a, cq, ck, st) : dp == 32 ? launch_bwd<T, 32>(a, cq, ck, st) : launch_bwd<T, 64>(a, cq, ck, st))
         return rc;
     if (dlam) {
@@ -1241,8 +1268,8 @@ extern "C" int sf_diff_attn_fwd(const sf_diff_attn_desc* p, const void* q, const
 extern "C" size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* p) {
     if (check_desc(p, "sf_diff_attn_bwd_workspace_bytes")) return 0;
     const RowPlan f = dq_plan(p);
-    const Cut ck = dkv_cut(p);
-    const size_t q = (size_t)f.cut.tail * f.cut.parts * f.rb * 2, k = (size_t)ck.tail * ck.parts * 128 * 4;
+    const KeyPlan g = dkv_plan(p);
+    const size_t q = (size_t)f.cut.tail * f.cut.parts * f.rb * 2, k = (size_t)g.cut.tail * g.cut.parts * g.kb * 4;
     return stat_bytes(p) + (q > k ? q : k) * padded(p->d) * sizeof(float);        // (one after the other in the same place)
 }
 
