@@ -654,6 +654,8 @@ template <int NW, int N> __device__ __forceinline__ void join_waves(f32x16 (&acc
 
 // Gradient of the queries: as the forward pass, rows (32 per wave) or the keys of a tile shared out.  (8 bf16 heads of 2 x 64, 2 x 5120 tokens:
 // 347 to 380 us, 322 GFLOP, 0.88 PFLOP/s; bound as the forward pass.)
+// bf16: delta_2 comes out of here again, as the sum of P_2 dP in f32, for dlam alone: over all the rows little is left of the terms of
+// dlam, and with the delta_2 of the forward pass's bf16 probabilities it was off by 2e-3 to 4.5e-3 of itself.
 template <typename T, int DP, int NW, bool KEYS_SPLIT, int KT>
 __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T> a) {
     using L = Tile<T, DP>;
@@ -700,6 +702,8 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
     f32x16 acc[NA];
 #pragma unroll
     for (int n = 0; n < NA; ++n) acc[n] = zero16();
+    constexpr bool SUM = sizeof(T) == 2;
+    float p2dp = 0.f;                                      // sum of P_2 (dP - delta_1)
     const T* const kbase = a.k + b * a.ks.b + hk * a.ks.h;
     const T* const vbase = a.v + b * a.vs.b + hk * a.vs.h;
     const Copy<T, DP, KT, NW> kc(a.ks.t, a.d), vc(a.vs.t, a.d);
@@ -730,7 +734,11 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
         for (int i = 0; i < 2; ++i) {
             float ds[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(s[i][r] * a.c - lse[i]) * (i ? fmaf(-lam, dp[r], apart) : dp[r]);
+            for (int r = 0; r < 16; ++r) {
+                const float y = __builtin_amdgcn_exp2f(s[i][r] * a.c - lse[i]);
+                if (SUM && i) p2dp = fmaf(y, dp[r], p2dp);
+                ds[r] = y * (i ? fmaf(-lam, dp[r], apart) : dp[r]);
+            }
             pack(df[i][0], ds);
             pack(df[i][1], ds + 8);
         }
@@ -768,9 +776,23 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
     }
     if constexpr (KEYS_SPLIT) {
         join_waves<NW>(acc, (float*)smem, wave, lane);
+        if constexpr (SUM) {
+            float* const box = (float*)smem;
+            __syncthreads();
+            box[wave * 64 + lane] = p2dp;
+            __syncthreads();
+            for (int u = 1; u < NW; ++u)
+                if (wave == 0) p2dp += box[u * 64 + lane];
+        }
         if (wave != 0) return;
     }
+    if constexpr (SUM) p2dp += __shfl_xor(p2dp, 32, 64);
     if (!have) return;
+    if (SUM && h2 == 0) {
+        const long long at = ((long long)w.tail * w.parts + w.part) * RB + (row - r0);
+        if (w.parts > 1) a.part[(long long)(gridDim.x - a.full) * RB * (2 * DP) + at] = p2dp;
+        else a.stat[(((long long)b * a.H + hq) * STATS + 4) * a.Tp + t] = p2dp - start[0];
+    }
 #pragma unroll
     for (int n = 0; n < NA; ++n)
 #pragma unroll
@@ -1003,6 +1025,12 @@ template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void 
     const long long out = KEYS ? (((long long)b * a.Tk + row) * a.Hk + hk) * (2 * a.d)
                                : (((long long)b * a.Tq + row / group) * a.H + hk * group + row % group) * (2 * a.d);
     const float* const p = a.part + ((long long)tail * a.parts * RB + id % RB) * W;
+    if (!KEYS && sizeof(T) == 2) {          // (there are at most 64 parts)
+        const float* const sums = a.part + (long long)items * a.parts * RB * W + (long long)tail * a.parts * RB + id % RB;
+        const float sum = wave_sum(lane < a.parts ? sums[(long long)lane * RB] : 0.f);
+        float* const stat = a.stat + ((long long)b * a.H + hk * group + row % group) * STATS * a.Tp + row / group;
+        if (lane == 0) stat[4LL * a.Tp] = sum - stat[a.Tp];
+    }
     for (int c = lane; c < W; c += 64) {
         const int half = c / DP & 1, j = c % DP;
         if (j >= a.d) continue;
@@ -1269,8 +1297,8 @@ extern "C" size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* p) {
     if (check_desc(p, "sf_diff_attn_bwd_workspace_bytes")) return 0;
     const RowPlan f = dq_plan(p);
     const KeyPlan g = dkv_plan(p);
-    const size_t q = (size_t)f.cut.tail * f.cut.parts * f.rb * 2, k = (size_t)g.cut.tail * g.cut.parts * g.kb * 4;
-    return stat_bytes(p) + (q > k ? q : k) * padded(p->d) * sizeof(float);        // (one after the other in the same place)
+    const size_t q = (size_t)f.cut.tail * f.cut.parts * f.rb * (2 * padded(p->d) + 1), k = (size_t)g.cut.tail * g.cut.parts * g.kb * 4 * padded(p->d);
+    return stat_bytes(p) + (q > k ? q : k) * sizeof(float);        // (one after the other in the same place)
 }
 
 extern "C" int sf_diff_attn_bwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,

@@ -315,6 +315,19 @@ def test_offsets_beyond_32_bits(Tq, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 130, 300, 4, 2, 64), (1, 40, 3000, 1, 1, 32), (2, 1, 300, 6, 3, 8), (2, 700, 700, 2, 1, 16),
+                                   (1, 700, 900, 2, 2, 64)], ids=str)
+@pytest.mark.parametrize("causal", [False, True])
+def test_lam_gradient_in_bf16(shape, causal):
+    """dlam takes part in no rounding to bf16 but that of the inputs: its sums are of f32 probabilities and f32 dP, so it
+    meets the bound of the f32 form."""
+    q, k, v, lam, do = make(*shape, BF, seed=15)
+    _, g = run(load_pkg(), q, k, v, lam, do, causal=causal)
+    want, mag = oracle(q, k, v, lam, causal, None, q.shape[-1] ** -0.5, do)
+    check(g["dlam"], want["dlam"], mag["dlam"], F, "dlam")
+
+
+@pytest.mark.gpu
 def test_shared_heads_gradient_is_the_sum():
     """Shared key / value heads against the same call with the heads repeated: gradients add up over the group."""
     sf = load_pkg()
