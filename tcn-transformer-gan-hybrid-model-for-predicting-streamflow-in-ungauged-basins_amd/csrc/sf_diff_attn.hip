@@ -573,7 +573,8 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_join_k
 // ------------------------------------------------------------------------------ backward
 constexpr int STATS = 5;                // values of a row
 
-// stat = lse_1, -delta_1, lse_2, lam (delta_2 - delta_1), delta_2 of every row; delta_i = do . O_i.  16 lanes per row.  What the two
+// stat = lse_1, -delta_1, lse_2, lam (delta_2 - delta_1), delta_2 of every row; delta_i = do . O_i (the last one is for dlam alone,
+// and in bf16 the query gradients' kernel writes a better one).  16 lanes per row.  What the two
 // gradient kernels would compute for every score is in them: -delta_1 starts the accumulators of dP, so that
 // dP - delta_1 costs nothing, and -lam (dP - delta_2) is one multiply-add from it (2 x 5120 tokens, 8 heads: dq 384 to
 // 372 us, dk and dv 597 to 589).  O_1 and O_2 are kept in f32: the gradients of the scores are differences dP - delta,
@@ -653,7 +654,7 @@ template <int NW, int N> __device__ __forceinline__ void join_waves(f32x16 (&acc
 }
 
 // Gradient of the queries: as the forward pass, rows (32 per wave) or the keys of a tile shared out.  (8 bf16 heads of 2 x 64, 2 x 5120 tokens:
-// 347 to 380 us, 322 GFLOP, 0.88 PFLOP/s; bound as the forward pass.)
+// 350 to 390 us, 322 GFLOP, 0.86 PFLOP/s; bound as the forward pass.)
 // bf16: delta_2 comes out of here again, as the sum of P_2 dP in f32, for dlam alone: over all the rows little is left of the terms of
 // dlam, and with the delta_2 of the forward pass's bf16 probabilities it was off by 2e-3 to 4.5e-3 of itself.
 template <typename T, int DP, int NW, bool KEYS_SPLIT, int KT>
@@ -812,8 +813,8 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
 // 32 registers of keys little is left of the 256 that two waves per SIMD have, and a spilled one is reloaded behind the copies
 // under way.  So a lane keeps two address registers for its row pieces and two for its column pieces and makes the
 // others where it uses them (fresh), and the maps come one after the other: no spill in the loop (2 x 5120 tokens, 8 heads:
-// 725 us with 13 spills, 592 us without; eight waves in pairs, with the keys in LDS too, 635 us).  539 to 600 us now, 429 GFLOP,
-// 0.75 PFLOP/s: the matrix pipe is busy 38 % of the time, LDS reads 34 %, and no registers are left to fetch operands ahead.
+// 725 us with 13 spills, 592 us without; eight waves in pairs, with the keys in LDS too, 635 us).  540 to 600 us now, 429 GFLOP,
+// 0.75 PFLOP/s: the matrix pipe is busy 40 % of the time, LDS reads 35 %, and no registers are left to fetch operands ahead.
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a) {
     using L = Tile<T, DP>;
