@@ -873,9 +873,9 @@ class DiffAttentionFn(torch.autograd.Function):
     """(softmax(scale q1 k1^T) - lam softmax(scale q2 k2^T)) v, see diff_attention."""
 
     @staticmethod
-    def forward(ctx, q, k, v, lam, lengths, causal, scale):
+    def forward(ctx, q, k, v, lam, lengths, causal, scale, strides):
         need = any(ctx.needs_input_grad[:4])
-        o, saved = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need)
+        o, saved = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need, strides)
         if need:
             ctx.desc, maps, lse = saved or (None, None, None)       # (no query or no key: nothing to save)
             ctx.strides = (q.stride(), k.stride(), v.stride())
@@ -887,14 +887,14 @@ class DiffAttentionFn(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, lam, lengths, maps, lse = ctx.saved_tensors
         if ctx.desc is None:
-            return (*(torch.zeros(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, lam)), None, None, None)
+            return (*(torch.zeros(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, lam)), None, None, None, None)
         desc = ctx.desc
         if ctx.strides != (q.stride(), k.stride(), v.stride()) or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
             # hooks on saved tensors (torch.autograd.graph.save_on_cpu) give back copies of another layout
-            q, k, v = ops.kernel_layout(q), ops.kernel_layout(k), ops.kernel_layout(v)
-            desc = ops.diff_attn_desc(q, k, v, lam, desc.causal, desc.scale)
+            (q, k, v), strides = ops.kernel_layouts(q, k, v)
+            desc = ops.diff_attn_desc(q, k, v, lam, desc.causal, desc.scale, strides)
         grads = ops.diff_attn_bwd(q, k, v, lam, lengths, desc, maps, lse, do.contiguous(), ctx.needs_input_grad[3])
-        return (*grads, None, None, None)
+        return (*grads, None, None, None, None)
 
 
 def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, causal: bool = False,
@@ -930,14 +930,15 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
         raise RuntimeError(f"diff_attention: lam {tuple(lam.shape)} for {H} heads")
     if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
         raise RuntimeError(f"diff_attention: lengths is a contiguous int32 [{B}], not {lengths.dtype} {tuple(lengths.shape)}")
-    if any(t.device != q.device for t in (k, v, lam, *(() if lengths is None else (lengths,)))):
+    index = q.get_device()
+    if k.get_device() != index or v.get_device() != index or lam.get_device() != index or (lengths is not None and lengths.get_device() != index):
         raise RuntimeError("diff_attention: all tensors on one device")
     scale = d ** -0.5 if scale is None else float(scale)
-    q, k, v = ops.kernel_layout(q), ops.kernel_layout(k), ops.kernel_layout(v)
+    (q, k, v), strides = ops.kernel_layouts(q, k, v)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"diff_attention: scale must be positive, not {scale}")
     with ops.device_guard(q):
-        return DiffAttentionFn.apply(q, k, v, lam.contiguous(), lengths, bool(causal), scale)
+        return DiffAttentionFn.apply(q, k, v, lam.contiguous(), lengths, bool(causal), scale, strides)
 
 
 # ------------------------------------------------------------------------------ AdamW

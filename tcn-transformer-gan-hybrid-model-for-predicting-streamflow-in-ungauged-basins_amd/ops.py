@@ -1178,22 +1178,32 @@ def kernel_layout(t: torch.Tensor) -> torch.Tensor:
     return t if _token_strides(t) is not None else t.clone(memory_format=torch.contiguous_format)
 
 
-def diff_attn_desc(q, k, v, lam, causal, scale):
+def kernel_layouts(*ts):
+    """Each tensor as the attention kernels can read it, in place or a contiguous copy, and their strides."""
+    strides = [_token_strides(t) for t in ts]
+    if None in strides:
+        ts = [kernel_layout(t) for t in ts]
+        strides = [_token_strides(t) for t in ts]
+    return ts, strides
+
+
+def diff_attn_desc(q, k, v, lam, causal, scale, strides=None):
+    """strides: those of kernel_layouts(q, k, v), when they are at hand."""
     B, Tq, H, _, d = q.shape
-    qs, ks, vs = _token_strides(q), _token_strides(k), _token_strides(v)
+    qs, ks, vs = strides or (_token_strides(q), _token_strides(k), _token_strides(v))
     if qs is None or ks is None or vs is None:
         raise RuntimeError("diff_attention: a layout the kernels cannot read (see kernel_layout)")
     return DiffAttnDesc(code_of(q.dtype), code_of(lam.dtype), B, Tq, k.shape[1], H, k.shape[2], d, int(causal), scale, qs, ks, vs)
 
 
-def diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need_save=False):
+def diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need_save=False, strides=None):
     """q [B,Tq,H,2,d], k [B,Tk,Hk,2,d], v [B,Tk,Hk,2d], lam [H] -> (o [B,Tq,H,2d], saved): saved (what the
     backward pass needs) is None unless wanted."""
     B, Tq, H, _, d = q.shape
     o = torch.empty((B, Tq, H, 2 * d), device=q.device, dtype=q.dtype)
     if o.numel() == 0 or k.numel() == 0:        # no query, or no key for anyone
         return o.zero_(), None
-    desc = diff_attn_desc(q, k, v, lam, causal, scale)
+    desc = diff_attn_desc(q, k, v, lam, causal, scale, strides)
     at = ctypes.addressof(desc)
     maps = lse = None
     if need_save:
