@@ -633,7 +633,8 @@ int sf_layer_norm_bwd(const void* dy, const void* dsum, const void* s, const flo
  * NULL in inference); ws:
  * sf_diff_attn_fwd_workspace_bytes(desc) bytes (may be 0), any contents.  Backward: dlam [H] of lam's type, or NULL;
  * every output is overwritten; ws: sf_diff_attn_bwd_workspace_bytes(desc) bytes.  No atomics: equal calls give equal
- * results.  The workspace size functions return 0 for a descriptor that the call itself refuses. */
+ * results.  A call has less than 16 million tiles of 32 rows (of all the heads) or keys, a backward call less than 2^28 rows (B H Tq, Tq
+ * rounded up to 128).  The workspace size functions return 0 for a descriptor that the call itself refuses. */
 typedef struct sf_diff_attn_desc {
     int dtype, lam_dtype, B, Tq, Tk, H, Hk, d, causal;
     float scale;

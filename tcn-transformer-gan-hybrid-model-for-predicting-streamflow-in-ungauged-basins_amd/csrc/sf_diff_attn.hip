@@ -1063,8 +1063,14 @@ int check_desc(const sf_diff_attn_desc* p, const char* who) {
         SF_REQUIRE(s >= 0 && s % epc == 0, "%s: stride %lld is not a multiple of 16 bytes", who, s);
         SF_REQUIRE(i % 3 != 1 || (s >= 2 * p->d && s < (1 << 22)), "%s: token stride %lld (a head has %d values)", who, s, 2 * p->d);
     }
-    const double groups = (double)p->B * p->Hk * (((double)p->H / p->Hk * p->Tq + 31) / 32 + (p->Tk + 127) / 128);
-    SF_REQUIRE(groups < 1e8 && (double)p->B * padded_rows(p) * p->H < 2e9, "%s: too many rows", who);
+    // a launch has less than 2^32 threads: 256 for an item of 32 rows or keys, and the parts of the last ones
+    const double rows = ((double)p->H / p->Hk * p->Tq + 31) / 32, keys = (p->Tk + 31) / 32;
+    SF_REQUIRE((double)p->B * p->Hk * (rows > keys ? rows : keys) < 16e6, "%s: too many rows or keys for one call", who);
+    return SF_OK;
+}
+int check_bwd_desc(const sf_diff_attn_desc* p, const char* who) {
+    if (int rc = check_desc(p, who)) return rc;
+    SF_REQUIRE((double)p->B * padded_rows(p) * p->H < (1 << 28), "%s: too many rows for one call", who);     // (16 threads for a row)
     return SF_OK;
 }
 int check_align(const void* const* ps, int n, const char* who) {
@@ -1295,7 +1301,7 @@ extern "C" int sf_diff_attn_fwd(const sf_diff_attn_desc* p, const void* q, const
 }
 
 extern "C" size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* p) {
-    if (check_desc(p, "sf_diff_attn_bwd_workspace_bytes")) return 0;
+    if (check_bwd_desc(p, "sf_diff_attn_bwd_workspace_bytes")) return 0;
     const RowPlan f = dq_plan(p);
     const KeyPlan g = dkv_plan(p);
     const size_t q = (size_t)f.cut.tail * f.cut.parts * f.rb * (2 * padded(p->d) + 1), k = (size_t)g.cut.tail * g.cut.parts * g.kb * 4 * padded(p->d);
@@ -1305,7 +1311,7 @@ extern "C" size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* p) {
 extern "C" int sf_diff_attn_bwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
                                 const int* lengths, const float* maps, const float* lse, const void* dout, void* dq, void* dk,
                                 void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream) {
-    if (int rc = check_desc(p, "sf_diff_attn_bwd")) return rc;
+    if (int rc = check_bwd_desc(p, "sf_diff_attn_bwd")) return rc;
     const void* ps[] = {q, k, v, maps, dout, dq, dk, dv, lse};
     if (int rc = check_align(ps, 9, "sf_diff_attn_bwd")) return rc;
     const size_t need = sf_diff_attn_bwd_workspace_bytes(p);

@@ -510,6 +510,11 @@ def test_library_refusals():
     def bwd(ws=a, n=nb, do=a):
         return L.sf_diff_attn_bwd(ctypes.byref(desc()), a, a, a, a, None, a, a, do, a, a, a, a, ws, ctypes.c_size_t(n), None)
     assert bwd(ws=None) == -22 and bwd(n=nb - 1) == -22 and bwd(do=None) == -22
+    # more work than one launch has threads for
+    for many in (dict(B=1 << 23, H=4, Hk=2), dict(B=1 << 10, Tk=1 << 20), dict(B=1 << 12, H=8, Hk=1, Tq=1 << 16)):
+        assert fwd(desc(**many)) == -22, many
+    wide = desc(B=1 << 21, H=1, Hk=1)
+    assert int(L.sf_diff_attn_bwd_workspace_bytes(ctypes.byref(wide))) == 0
 
 
 @pytest.mark.gpu
