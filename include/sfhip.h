@@ -650,7 +650,7 @@ int sf_diff_attn_bwd(const sf_diff_attn_desc* desc, const void* q, const void* k
 
 /* ---- AdamW over many tensors -------------------------------------------------------------------- */
 /* One AdamW step (decoupled weight decay; the reference trains with Adam, src/train.py:80-91) of `count`
- * tensors in as few launches as their pointers fit (40 tensors each).  All array arguments are HOST
+ * tensors (of less than 2^36 elements) in as few launches as their pointers fit (some 40 tensors each).  All array arguments are HOST
  * arrays of `count` entries, read during the call: p f32 parameters, g gradients (g_dtype[i] f32 or bf16),
  * shadow_bf16 (NULL, or entries that may be NULL) copies of the updated parameters, n elements (0 allowed),
  * lr, weight_decay, step_offset (NULL = 0; see sf_adam_guarded).  Any element alignment; no two

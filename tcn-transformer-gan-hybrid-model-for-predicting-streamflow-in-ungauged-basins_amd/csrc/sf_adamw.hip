@@ -18,7 +18,7 @@
 // element), which keeps the moments unbiased and a run reproducible.  A second moment is never rounded to
 // zero (its square root divides).  The update of p uses the moments before they are rounded.
 //
-// Measured on 68.3 M elements in 39 tensors (a copy of 1 GiB runs at 5.05 TB/s on the same card): f32 gradients and moments 360 us,
+// Measured on 68.3 M elements in 40 tensors (a copy of 1 GiB runs at 5.05 TB/s on the same card): f32 gradients and moments 360 us,
 // 1.91 GB, 5.3 TB/s; bf16 gradients and 8-bit moments 196 us, 0.96 GB, 4.9 TB/s, and their values as bf16 (adamw_moments) 82 us,
 // 0.41 GB, 5.0 TB/s.  16 tensors with 2.8 M elements: 13 us, and the launch around it costs the host more.
 #include "sf_common.h"
@@ -29,7 +29,8 @@ namespace {
 constexpr int NT = 256;
 constexpr int CHUNK = 4096;        // elements of a workgroup: 16 per thread
 constexpr int BLOCK = SF_ADAMW_BLOCK;
-constexpr int MAX_TENSORS = 40;    // tensors of one launch: their table stays below 4 KB of kernel arguments
+constexpr long long MAX_GROUPS = (1 << 24) - 1;     // workgroups of one launch: less than 2^32 threads
+constexpr long long MAX_ELEMENTS = MAX_GROUPS * CHUNK;
 static_assert(BLOCK == 8 * 32 && CHUNK % (8 * NT) == 0, "32 lanes hold a block of moments");
 
 struct Tensor {
@@ -47,9 +48,11 @@ struct Tensor {
     int g_bf16;
     int first;                     // first workgroup
 };
-struct Table { Tensor t[MAX_TENSORS]; };
 struct Hyper { double beta1, beta2; float eps, grad_scale; unsigned seed_lo, seed_hi; int count; };
-static_assert(sizeof(Table) + sizeof(Hyper) + 16 <= 4096, "kernel arguments");
+// tensors of one launch: as many as 4 KB of kernel arguments hold beside two pointers and the 256 bytes that the compiler adds
+constexpr int MAX_TENSORS = (4096 - 256 - 16 - (int)sizeof(Hyper)) / (int)sizeof(Tensor);
+static_assert(MAX_TENSORS <= 64, "a lane for each");
+struct Table { Tensor t[MAX_TENSORS]; };
 
 // V elements at an address aligned to one element only: the hardware serves wide global accesses at any element alignment
 template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Some { T e[V]; };
@@ -282,14 +285,14 @@ __global__ __launch_bounds__(NT) void adamw_moments_kernel(Table tab, int count)
     else moments_chunk<false>(T, c0);
 }
 
-// splits the list into launches of at most MAX_TENSORS non-empty tensors and 2^30 workgroups
+// splits the list into launches of at most MAX_TENSORS non-empty tensors and MAX_GROUPS workgroups
 template <typename F, typename L> int over_tensors(int count, const long long* n, F&& fill, L&& launch) {
     Table tab;
     int used = 0;
     long long groups = 0;
     for (int i = 0; i <= count; ++i) {
         const long long need = i < count ? (n[i] + CHUNK - 1) / CHUNK : 0;
-        if (used && (i == count || used == MAX_TENSORS || groups + need > (1LL << 30))) {
+        if (used && (i == count || used == MAX_TENSORS || groups + need > MAX_GROUPS)) {
             launch(tab, used, (int)groups);
             used = 0;
             groups = 0;
@@ -317,7 +320,7 @@ extern "C" int sf_adamw_step(int count, float* const* p, const void* const* g, v
     SF_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "sf_adamw_step: betas must lie in [0, 1)");
     SF_REQUIRE(eps >= 0.f, "sf_adamw_step: eps must not be negative");
     for (int i = 0; i < count; ++i) {
-        SF_REQUIRE(n[i] >= 0 && n[i] <= (1LL << 41), "sf_adamw_step: tensor %d has %lld elements", i, n[i]);
+        SF_REQUIRE(n[i] >= 0 && n[i] <= MAX_ELEMENTS, "sf_adamw_step: tensor %d has %lld elements", i, n[i]);
         SF_REQUIRE(n[i] == 0 || (p[i] && g[i] && m[i] && v[i]), "sf_adamw_step: tensor %d has a null pointer", i);
         SF_REQUIRE(n[i] == 0 || state_bits == 32 || (m_exp[i] && v_exp[i]), "sf_adamw_step: tensor %d lacks its exponents", i);
         SF_REQUIRE(g_dtype[i] == SF_F32 || g_dtype[i] == SF_BF16, "sf_adamw_step: tensor %d has gradient dtype %d", i, g_dtype[i]);
@@ -346,7 +349,7 @@ extern "C" int sf_adamw_moments(int count, const void* const* m, const void* con
                                 const long long* n, void* stream) {
     SF_REQUIRE(count >= 0 && m && v && m_exp && v_exp && m_bf16 && v_bf16 && n, "sf_adamw_moments: null argument");
     for (int i = 0; i < count; ++i) {
-        SF_REQUIRE(n[i] >= 0 && n[i] <= (1LL << 41), "sf_adamw_moments: tensor %d has %lld elements", i, n[i]);
+        SF_REQUIRE(n[i] >= 0 && n[i] <= MAX_ELEMENTS, "sf_adamw_moments: tensor %d has %lld elements", i, n[i]);
         SF_REQUIRE(n[i] == 0 || (m[i] && v[i] && m_exp[i] && v_exp[i] && m_bf16[i] && v_bf16[i]),
                    "sf_adamw_moments: tensor %d has a null pointer", i);
     }

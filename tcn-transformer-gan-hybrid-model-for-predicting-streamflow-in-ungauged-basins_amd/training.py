@@ -200,7 +200,7 @@ class FlatAdam:
 
 class AdamW:
     """AdamW over a list of f32 parameters (or parameter groups: dicts with "params" and optionally "lr" and
-    "weight_decay"), every tensor updated from its own gradient (f32 or bf16) by one multi-tensor launch per 40
+    "weight_decay"), every tensor updated from its own gradient (f32 or bf16) by one multi-tensor launch per 43
     tensors: no flat copies, no launch per parameter.
 
     state_bits 32 keeps f32 moments; 8 keeps one byte per element and moment plus a byte per 256 elements
