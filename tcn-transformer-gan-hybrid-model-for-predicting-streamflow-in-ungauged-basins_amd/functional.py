@@ -955,8 +955,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     them (packed weights, shadows) are marked stale here."""
     if not state.is_cuda:
         raise RuntimeError("adamw_step: GPU tensors only (no CPU path exists)")
+    params = list(params)               # (an iterator is read once, and both calls below need it)
     with ops.device_guard(state):
-        ops.adamw_step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), state, lr, betas[0], betas[1], eps,
+        ops.adamw_step(params, list(grads), list(exp_avgs), list(exp_avg_sqs), state, lr, betas[0], betas[1], eps,
                        weight_decay, seed, found_inf, grad_scale, shadows, step_offsets)
         ops.touch(params)
 

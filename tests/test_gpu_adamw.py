@@ -565,3 +565,17 @@ def test_offsets_beyond_32_bits():
     sf.functional.adamw_step(*([t] for t in head), torch.zeros(2, device="cuda", dtype=torch.int32), 1e-2)
     for t, a in zip(big, head):
         assert bool((t[:-k] == a[0]).all())
+
+
+@pytest.mark.gpu
+def test_derived_copies_go_stale_for_an_iterator():
+    """The parameters may come as an iterator (module.parameters()), as any other list of the call."""
+    sf = load_pkg()
+    lin = torch.nn.Linear(16, 8).cuda()
+    shadow = sf.ops.weight_shadow(lin.weight).clone()
+    gs, ms, vs = ([torch.ones_like(p) for p in lin.parameters()] for _ in range(3))
+    state = torch.zeros(2, dtype=torch.int32, device="cuda")
+    sf.functional.adamw_step(lin.parameters(), iter(gs), iter(ms), iter(vs), state, 0.1)
+    assert sf.ops.shadow_if_current(lin.weight) is None
+    assert torch.equal(sf.ops.weight_shadow(lin.weight), lin.weight.detach().bfloat16())
+    assert not torch.equal(shadow, lin.weight.detach().bfloat16())
