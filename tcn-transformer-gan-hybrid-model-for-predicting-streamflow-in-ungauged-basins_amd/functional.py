@@ -893,7 +893,9 @@ class DiffAttentionFn(torch.autograd.Function):
             # hooks on saved tensors (torch.autograd.graph.save_on_cpu) give back copies of another layout
             (q, k, v), strides = ops.kernel_layouts(q, k, v)
             desc = ops.diff_attn_desc(q, k, v, lam, desc.causal, desc.scale, strides)
-        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, desc, maps, lse, do.contiguous(), ctx.needs_input_grad[3])
+        # (a contiguous gradient may start anywhere: the backward pass of a concatenation hands over slices of a flat buffer)
+        maps, lse, do = (ops.aligned(t) for t in (maps, lse, do))
+        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, desc, maps, lse, do, ctx.needs_input_grad[3])
         return (*grads, None, None, None, None)
 
 

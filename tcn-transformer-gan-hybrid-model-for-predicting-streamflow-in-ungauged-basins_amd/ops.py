@@ -1178,6 +1178,11 @@ def kernel_layout(t: torch.Tensor) -> torch.Tensor:
     return t if _token_strides(t) is not None else t.clone(memory_format=torch.contiguous_format)
 
 
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """t itself when it is contiguous and starts at a multiple of 16 bytes, else a copy that does."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def kernel_layouts(*ts):
     """Each tensor as the attention kernels can read it, in place or a contiguous copy, and their strides."""
     strides = [_token_strides(t) for t in ts]

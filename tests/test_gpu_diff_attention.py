@@ -552,3 +552,30 @@ def test_gpu_refusals():
         att(q, k, v, lam, scale=-1.0)
     with pytest.raises(RuntimeError, match="q \\["):
         att(q[0], k, v, lam)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_gradients_at_any_address(dtype):
+    """A contiguous gradient that starts between two 16-byte pieces (a slice of a flat buffer, what the backward pass of a concatenation
+    hands over) and saved tensors that come back at such an address: the same bits."""
+    sf = load_pkg()
+    x = make(2, 33, 50, 4, 2, 16, dtype, seed=16)
+    want = run(sf, *x)[1]
+    leaves = [t.cuda().requires_grad_(True) for t in x[:4]]
+    do = x[4].cuda()
+
+    def odd(t):
+        buf = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+        view = buf[1:].view(t.shape)
+        view.copy_(t)
+        return view
+    assert odd(do).is_contiguous() and odd(do).data_ptr() % 16
+    got = torch.autograd.grad(sf.functional.diff_attention(*leaves), leaves, odd(do))
+    assert all(torch.equal(a, want[n]) for a, n in zip(got, ("dq", "dk", "dv", "dlam")))
+    flat = torch.cat([torch.zeros(3, dtype=dtype, device="cuda"), sf.functional.diff_attention(*leaves).flatten()])
+    got = torch.autograd.grad(flat, leaves, torch.cat([torch.zeros(3, dtype=dtype, device="cuda"), do.flatten()]))
+    assert all(torch.equal(a, want[n]) for a, n in zip(got, ("dq", "dk", "dv", "dlam")))
+    with torch.autograd.graph.saved_tensors_hooks(odd, lambda t: t):
+        got = torch.autograd.grad(sf.functional.diff_attention(*leaves), leaves, do)
+    assert all(torch.equal(a, want[n]) for a, n in zip(got, ("dq", "dk", "dv", "dlam")))
