@@ -629,8 +629,9 @@ int sf_layer_norm_bwd(const void* dy, const void* dsum, const void* s, const flo
  * scale > 0.  lengths: int32 [B] on the device, keys of each sample (clamped to [0, Tk]), or NULL; keys from
  * there on are not read.  causal: query t sees keys up to t + Tk - Tq.  A query that sees no key gets zeros and has
  * no gradient.  All pointers 16-byte aligned; o, do, dq [B,Tq,H,2d] and dk, dv [B,Tk,Hk,2d] contiguous.
- * Forward: maps f32 [B,Tq,H,2,2d] (both softmax maps' results) and lse f32 [B,H,Tq,2] are kept for the backward pass (both
- * NULL in inference); ws:
+ * Scores may be of any finite size.
+ * Forward: maps f32 [B,Tq,H,2,2d] (both softmax maps' results) and sums f32 [B,H,Tq,2,2] (of each map the score that its exponentials
+ * are relative to, and their sum) are kept for the backward pass (both NULL in inference); ws:
  * sf_diff_attn_fwd_workspace_bytes(desc) bytes (may be 0), any contents.  Backward: dlam [H] of lam's type, or NULL;
  * every output is overwritten; ws: sf_diff_attn_bwd_workspace_bytes(desc) bytes.  No atomics: equal calls give equal
  * results.  A call has less than 16 million tiles of 32 rows (of all the heads) or keys, a backward call less than 2^28 rows (B H Tq, Tq
@@ -642,10 +643,10 @@ typedef struct sf_diff_attn_desc {
 } sf_diff_attn_desc;
 size_t sf_diff_attn_fwd_workspace_bytes(const sf_diff_attn_desc* desc);
 int sf_diff_attn_fwd(const sf_diff_attn_desc* desc, const void* q, const void* k, const void* v, const void* lam,
-                     const int* lengths, void* o, float* maps, float* lse, void* ws, size_t ws_bytes, void* stream);
+                     const int* lengths, void* o, float* maps, float* sums, void* ws, size_t ws_bytes, void* stream);
 size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* desc);
 int sf_diff_attn_bwd(const sf_diff_attn_desc* desc, const void* q, const void* k, const void* v, const void* lam,
-                     const int* lengths, const float* maps, const float* lse, const void* dout, void* dq, void* dk,
+                     const int* lengths, const float* maps, const float* sums, const void* dout, void* dq, void* dk,
                      void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- AdamW over many tensors -------------------------------------------------------------------- */

@@ -195,9 +195,41 @@ template <typename T> __device__ __forceinline__ Frag<T> global_piece(const T* r
     return f;
 }
 
-// a row's reference point before it has seen a key: every finite score is far above it, and it is itself finite, so that its
-// differences with masked scores (-inf) and with other reference points are never NaN
-constexpr float NO_SCORE = -3e38f;
+// Exponentials of a row are taken relative to a score `ref` that it has seen, and are 2^exponent(s), c being the scale in base 2.
+// Scores may be of any finite size, so nothing may depend on c s as such: rounded to f32 it is off by half a step, 0.004 at
+// 2^16, 1 at 2^24, 2^86 at 2^110.  While c ref is below FAR, the exponent is fma(s, c, -fl(c ref)), one rounding of its own
+// size; that c ref was rounded is a factor between 2^-1/2 and 2^1/2 that all of the row's terms and their sum share.
+// Beyond, no f32 lies near c ref any more, and the exponent is (s - ref) c: two roundings of its own size.  Which of
+// the two it is depends on `ref` alone, so equal scores have equal terms wherever they are formed.
+constexpr float FAR = 16777216.f;
+__device__ __forceinline__ float scaled(float ref, float c) {
+#pragma clang fp contract(off)
+    return ref * c;
+}
+__device__ __forceinline__ bool is_far(float ref, float c) { return !(fabsf(scaled(ref, c)) < FAR); }
+struct Exponent {
+    float sub, neg;
+    __device__ __forceinline__ Exponent(float ref, float c) {
+        const bool far = is_far(ref, c);
+        sub = far ? ref : 0.f;
+        neg = far ? 0.f : -scaled(ref, c);
+    }
+    __device__ __forceinline__ float operator()(float s, float c) const { return fmaf(s - sub, c, neg); }
+};
+// 2^this takes terms relative to `from` to terms relative to `to`
+__device__ __forceinline__ float change(float from, float to, float c) {
+#pragma clang fp contract(off)
+    const float far = -Exponent(from, c)(to, c), near = scaled(from, c) - scaled(to, c), between = fmaf(from, c, -scaled(to, c));
+    return is_far(to, c) ? far : is_far(from, c) ? between : near;
+}
+// The backward pass takes probabilities as 2^(c s - lse), lse = c ref + log2(sum) in one f32, where every |lse| of a tile is below
+// NEAR: off by 2^-18 of themselves at most.  Elsewhere as 2^(c (s - ref) - lg), one operation more; lg is log2(sum), less what the
+// rounding of c ref has left in the sum.
+constexpr float NEAR = 64.f;
+
+// a row's reference before it has seen a key: no finite score is below it, and it is itself finite, so that its differences
+// with masked scores (-inf) and with other references are never NaN
+constexpr float NO_SCORE = -3.4028234663852886e38f;
 
 // waves per SIMD that a kernel's registers have to leave room for: two, so that one computes while the other loads, but where the
 // accumulators and f32 operands of 2 x 64 columns alone are more than half of them
@@ -209,9 +241,9 @@ template <typename T> struct Args {
     Strides qs, ks, vs;
     const void* lam;
     const int* lengths;
-    T* o; float* maps; float* lse;          // maps f32 [B,Tq,H,2,2d] = O_1, O_2; lse f32 [B,H,Tq,2] (base 2): for the backward pass
+    T* o; float* maps; float* sums;         // maps f32 [B,Tq,H,2,2d] = O_1, O_2; sums f32 [B,H,Tq,2,2] = (ref, sum) of each map: for the backward pass
     float* part;                            // partial results of the work items that are cut
-    const T* dout; const float* maps_in; const float* lse_in;
+    const T* dout; const float* maps_in; const float* sums_in;
     float* stat;                            // [B,H,STATS,Tp], see attn_delta_kernel; zeros from Tq to Tp
     T* dq; T* dk; T* dv;
     int lam_bf16, B, Tq, Tp, Tk, H, Hk, d, causal;        // Tp: Tq rounded up to whole tiles of any kernel
@@ -290,8 +322,9 @@ template <typename T, int DP> __device__ __forceinline__ void store_cols(T* row,
 // the matrix pipe is busy 48 % of the time and the vector unit (32 exponentials a lane and tile of 32 x 32) nearly as long, hardly
 // at the same time, at a clock that power holds at 1.75 GHz.  1 x 8191 tokens, causal: 262 to 280 us, 206 GFLOP.  Single tokens,
 // 16 samples, 4 key heads, 8192 keys: 30 us, 134 MB, 4.4 TB/s, bound by HBM.
+// (narrow heads: four waves per SIMD, as many as slots_of counts on)
 template <typename T, int DP, int NW, bool KEYS_SPLIT, int KT>
-__global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<T> a) {
+__global__ __launch_bounds__(64 * NW, (DP == 16 && !KEYS_SPLIT ? 4 : WAVES<T, DP>)) void attn_fwd_kernel(Args<T> a) {
     using L = Tile<T, DP>;
     constexpr int KS = DP / 16, DT = 2 * DP / 32;
     constexpr int RB = KEYS_SPLIT ? 32 : 32 * NW;
@@ -327,10 +360,10 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
         for (int s = 0; s < KS; ++s) qf[i][s] = global_piece<T>(qrow, i, s * 16 + 8 * h2, a.d, true);
 
     f32x16 acc[2][DT];
-    float m[2], l[2];
+    float ref[2], l[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        m[i] = NO_SCORE;
+        ref[i] = NO_SCORE;
         l[i] = 0.f;
 #pragma unroll
         for (int n = 0; n < DT; ++n) acc[i][n] = zero16();
@@ -343,15 +376,6 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
 
     const typename L::Lane rl = L::row_lane(lane), cl = L::col_lane(lane);
 
-    auto exponentials = [&](float* p, const f32x16& s, float ref) {
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(s[r] * a.c - ref);
-            sum += p[r];
-        }
-        return sum;
-    };
     auto sub_tile = [&](lds_cptr kt, lds_cptr vt, int sub, int key0) {
         if (key0 >= vmax) return;
         f32x16 s[2] = {zero16(), zero16()};
@@ -371,24 +395,36 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
         Frag<T> pf[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            // The reference point m of the exponentials only has to keep them in range: it moves when a lane's 16 of them
-            // add up to more than 2^12 (always at a row's first visible key, m being NO_SCORE before), then to the row's
-            // maximum.  The usual tile so needs no maximum, no exchange between lanes and no rescaling.
-            float p[16];
-            float sum = exponentials(p, s[i], m[i]);
-            if (__any(sum > 4096.f)) {
+            // The reference of the exponentials only has to keep them in range: it moves when a lane's 16 of them add up to more
+            // than 2^12, then to the row's maximum.  The usual tile so needs no maximum, no exchange between lanes
+            // and no rescaling.  Where a row has seen no key yet, or its reference is far, the attempt does not count (it is made
+            // all the same: behind a branch it could not overlap with the products).
+            float p[16], sum = 0.f;
+            const float at = scaled(ref[i], a.c);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], a.c, -at));
+                sum += p[r];
+            }
+            if (__any((sum > 4096.f) | !(fabsf(at) < FAR))) {
                 float top = s[i][0];
 #pragma unroll
                 for (int r = 1; r < 16; ++r) top = fmaxf(top, s[i][r]);
-                top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
-                const float mn = fmaxf(m[i], top), f = exp2f(m[i] - mn);
-                m[i] = mn;
+                const float to = fmaxf(ref[i], fmaxf(top, __shfl_xor(top, 32, 64))), f = exp2f(change(ref[i], to, a.c));
+                ref[i] = to;
                 l[i] *= f;
 #pragma unroll
                 for (int n = 0; n < DT; ++n)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[i][n][r] *= f;
-                sum = exponentials(p, s[i], m[i]);
+                __builtin_amdgcn_sched_barrier(0);         // (fewer registers)
+                sum = 0.f;
+                const Exponent exponent(to, a.c);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    p[r] = __builtin_amdgcn_exp2f(exponent(s[i][r], a.c));
+                    sum += p[r];
+                }
             }
             l[i] += sum;
             pack(pf[i][0], p);
@@ -433,7 +469,7 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
 
     if constexpr (KEYS_SPLIT) {
         // the waves' states one after the other into LDS, wave 0 adds them up
-        float* const box = reinterpret_cast<float*>(smem);             // [2 DT 16][64] accumulators, then m, l
+        float* const box = reinterpret_cast<float*>(smem);             // [2 DT 16][64] accumulators, then ref, l
 #pragma unroll 1
         for (int u = 1; u < NW; ++u) {
             __syncthreads();
@@ -444,7 +480,7 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
                     for (int n = 0; n < DT; ++n)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) box[((i * DT + n) * 16 + r) * 64 + lane] = acc[i][n][r];
-                    box[(2 * DT * 16 + 2 * i) * 64 + lane] = m[i];
+                    box[(2 * DT * 16 + 2 * i) * 64 + lane] = ref[i];
                     box[(2 * DT * 16 + 2 * i + 1) * 64 + lane] = l[i];
                 }
             }
@@ -452,9 +488,9 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
             if (wave == 0) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float mo = box[(2 * DT * 16 + 2 * i) * 64 + lane], lo = box[(2 * DT * 16 + 2 * i + 1) * 64 + lane];
-                    const float mn = fmaxf(m[i], mo), f = exp2f(m[i] - mn), g = exp2f(mo - mn);
-                    m[i] = mn;
+                    const float other = box[(2 * DT * 16 + 2 * i) * 64 + lane], lo = box[(2 * DT * 16 + 2 * i + 1) * 64 + lane];
+                    const float to = fmaxf(ref[i], other), f = exp2f(change(ref[i], to, a.c)), g = exp2f(change(other, to, a.c));
+                    ref[i] = to;
                     l[i] = l[i] * f + lo * g;
 #pragma unroll
                     for (int n = 0; n < DT; ++n)
@@ -480,10 +516,10 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
                     *reinterpret_cast<float4*>(po + i * 2 * DP + 32 * n + acc_row(r, h2)) =
                         float4{acc[i][n][r], acc[i][n][r + 1], acc[i][n][r + 2], acc[i][n][r + 3]};
         if (h2 == 0)
-            *reinterpret_cast<float4*>(a.part + items * w.parts * RB * (4 * DP) + at * 4) = float4{m[0], l[0], m[1], l[1]};
+            *reinterpret_cast<float4*>(a.part + items * w.parts * RB * (4 * DP) + at * 4) = float4{ref[0], l[0], ref[1], l[1]};
         return;
     }
-    // a row that sees no key has l = 0: its output is zero, and its lse infinite, which makes its probabilities zero
+    // a row that sees no key has l = 0: its output is zero
     const float i1 = l[0] > 0.f || l[0] != l[0] ? 1.f / l[0] : 0.f, i2 = l[1] > 0.f || l[1] != l[1] ? 1.f / l[1] : 0.f;
     const float lam = lam_of(a.lam, a.lam_bf16, hq);
     const long long out = (((long long)b * a.Tq + t) * a.H + hq) * (2 * a.d);
@@ -505,11 +541,7 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_fwd_kernel(Args<
                 store_cols<float, DP>(a.maps + 2 * out + 2 * a.d, c, a.d, z[0], z[1], z[2], z[3]);
             }
         }
-    if (a.lse && h2 == 0) {
-        float* const p = a.lse + (((long long)b * a.H + hq) * a.Tq + t) * 2;
-        p[0] = l[0] > 0.f ? m[0] + __log2f(l[0]) : l[0] == 0.f ? INFINITY : l[0];
-        p[1] = l[1] > 0.f ? m[1] + __log2f(l[1]) : l[1] == 0.f ? INFINITY : l[1];
-    }
+    if (a.sums && h2 == 0) *reinterpret_cast<float4*>(a.sums + (((long long)b * a.H + hq) * a.Tq + t) * 4) = float4{ref[0], l[0], ref[1], l[1]};
 }
 
 // joins the parts of the forward items that were cut: one wave per query row (2 x 5120 tokens, two parts for a fifth of the rows:
@@ -530,8 +562,8 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_join_k
     const float* const pm = a.part + (long long)items * a.parts * rb * (4 * DP);
     float4 v{NO_SCORE, 0.f, NO_SCORE, 0.f};
     if (lane < a.parts) v = *reinterpret_cast<const float4*>(pm + (at0 + (long long)lane * rb) * 4);
-    const float m[2] = {wave_max(v.x), wave_max(v.z)};
-    const float f1 = exp2f(v.x - m[0]), f2 = exp2f(v.z - m[1]);
+    const float ref[2] = {wave_max(v.x), wave_max(v.z)};
+    const float f1 = exp2f(change(v.x, ref[0], a.c)), f2 = exp2f(change(v.z, ref[1], a.c));
     const float l[2] = {wave_sum(v.y * f1), wave_sum(v.w * f2)};
     constexpr int NCOL = (2 * DP + 63) / 64;
     float acc[2][NCOL];
@@ -564,22 +596,20 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void attn_join_k
             a.maps[2 * out + (2 + half) * a.d + j] = z;
         }
     }
-    if (a.lse && lane < 2) {
-        const float ll = lane ? l[1] : l[0], mm = lane ? m[1] : m[0];
-        a.lse[(((long long)b * a.H + hq) * a.Tq + t) * 2 + lane] = ll > 0.f ? mm + __log2f(ll) : ll == 0.f ? INFINITY : ll;
-    }
+    if (a.sums && lane == 0) *reinterpret_cast<float4*>(a.sums + (((long long)b * a.H + hq) * a.Tq + t) * 4) = float4{ref[0], l[0], ref[1], l[1]};
 }
 
 // ------------------------------------------------------------------------------ backward
-constexpr int STATS = 5;                // values of a row
+constexpr int STATS = 9;                // values of a row
 
-// stat = lse_1, -delta_1, lse_2, lam (delta_2 - delta_1), delta_2 of every row; delta_i = do . O_i (the last one is for dlam alone,
-// and in bf16 the query gradients' kernel writes a better one).  16 lanes per row.  What the two
+// stat = lse_1, -delta_1, lse_2, lam (delta_2 - delta_1), ref_1, lg_1, ref_2, lg_2, delta_2 of every row; delta_i = do . O_i
+// (the last one is for dlam alone, and in bf16 the query gradients' kernel writes a better one).  A row that saw no key gets infinite lse
+// and ref, which make its probabilities zero.  16 lanes per row.  What the two
 // gradient kernels would compute for every score is in them: -delta_1 starts the accumulators of dP, so that
 // dP - delta_1 costs nothing, and -lam (dP - delta_2) is one multiply-add from it (2 x 5120 tokens, 8 heads: dq 384 to
 // 372 us, dk and dv 597 to 589).  O_1 and O_2 are kept in f32: the gradients of the scores are differences dP - delta,
 // and rounding the maps to bf16 as well raises the relative error of dq from 2.9e-3 to 3.6e-3 (32 x 365 tokens).  Bound by HBM:
-// 22 us for the 210 MB of 2 x 5120 tokens and 8 heads of 2 x 64, most of it the maps.
+// 24 us for the 210 MB of 2 x 5120 tokens and 8 heads of 2 x 64, most of it the maps.
 template <typename T> __global__ __launch_bounds__(256) void attn_delta_kernel(Args<T> a) {
     const long long id = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);       // (b, t, h), t up to Tp
     const int q = threadIdx.x & 15, h = (int)(id % a.H), t = (int)(id / a.H % a.Tp);
@@ -609,7 +639,15 @@ template <typename T> __global__ __launch_bounds__(256) void attn_delta_kernel(A
     }
     if (q >= STATS) return;
     float v = q == 1 ? -d1 : q == 3 ? lam_of(a.lam, a.lam_bf16, h) * (d2 - d1) : d2;
-    if (q == 0 || q == 2) v = t < a.Tq ? a.lse_in[((b * a.H + h) * a.Tq + t) * 2 + (q >> 1)] : 0.f;
+    if (q != 1 && q != 3 && q != 8) {
+        v = 0.f;
+        if (t < a.Tq) {
+            const float* const p = a.sums_in + ((b * a.H + h) * a.Tq + t) * 4 + (q == 2 || q > 5 ? 2 : 0);
+            const float ref = p[0], sum = p[1], lg = sum > 0.f ? __log2f(sum) : sum;        // (0 stays 0, NaN NaN)
+            if (q > 3 && q & 1) v = is_far(ref, a.c) ? lg : lg - fmaf(ref, a.c, -scaled(ref, a.c));
+            else v = sum == 0.f ? INFINITY : q > 3 ? ref : scaled(ref, a.c) + lg;
+        }
+    }
     a.stat[((b * a.H + h) * STATS + q) * a.Tp + t] = v;
 }
 
@@ -621,7 +659,7 @@ __global__ __launch_bounds__(1024) void attn_dlam_kernel(const float* __restrict
     double s = 0.0;
     const long long n = (long long)B * Tp;
 #pragma unroll 8
-    for (long long i = threadIdx.x; i < n; i += 1024) s += (double)stat[((i / Tp * H + h) * STATS + 4) * Tp + i % Tp];
+    for (long long i = threadIdx.x; i < n; i += 1024) s += (double)stat[((i / Tp * H + h) * STATS + STATS - 1) * Tp + i % Tp];
     s = wave_sum_d(s);
     if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -696,7 +734,14 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
         gf[KS + s] = global_piece<T>(a.dout + out, 1, s * 16 + 8 * h2, a.d, true);
     }
     const float* const stat = a.stat + ((long long)b * a.H + hq) * STATS * a.Tp + t;
-    const float lse[2] = {stat[0], stat[2 * a.Tp]}, apart = stat[3 * a.Tp], lam = lam_of(a.lam, a.lam_bf16, hq);
+    float lse[2] = {stat[0], stat[2 * a.Tp]};              // or lg, with ref to be taken off the scores first
+    const float apart = stat[3 * a.Tp], lam = lam_of(a.lam, a.lam_bf16, hq);
+    const bool wide = __any(!(fmaxf(fabsf(lse[0]), fabsf(lse[1])) < NEAR));
+    const float ref[2] = {stat[4 * a.Tp], stat[6 * a.Tp]};
+    if (wide) {
+        lse[0] = stat[5 * a.Tp];
+        lse[1] = stat[7 * a.Tp];
+    }
     f32x16 start;                                          // of dP - delta_1
 #pragma unroll
     for (int r = 0; r < 16; ++r) start[r] = stat[a.Tp];
@@ -733,10 +778,14 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
         Frag<T> df[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+            if (wide) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] -= ref[i];
+            }
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float y = __builtin_amdgcn_exp2f(s[i][r] * a.c - lse[i]);
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[i][r], a.c, -lse[i]));
                 if (SUM && i) p2dp = fmaf(y, dp[r], p2dp);
                 ds[r] = y * (i ? fmaf(-lam, dp[r], apart) : dp[r]);
             }
@@ -792,7 +841,7 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
     if (SUM && h2 == 0) {
         const long long at = ((long long)w.tail * w.parts + w.part) * RB + (row - r0);
         if (w.parts > 1) a.part[(long long)(gridDim.x - a.full) * RB * (2 * DP) + at] = p2dp;
-        else a.stat[(((long long)b * a.H + hq) * STATS + 4) * a.Tp + t] = p2dp - start[0];
+        else a.stat[(((long long)b * a.H + hq) * STATS + STATS - 1) * a.Tp + t] = p2dp - start[0];
     }
 #pragma unroll
     for (int n = 0; n < NA; ++n)
@@ -820,7 +869,7 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<
     using L = Tile<T, DP>;
     constexpr int KB = SPLIT ? 32 : 32 * NW, QT = SPLIT ? 32 * NW : 32, KS = DP / 16, VS = 2 * DP / 16, DT = 2 * DP / 32;
     constexpr int NA = DP == 16 ? 2 : DT;
-    constexpr int TB = L::bytes(QT), SB = QT <= 64 ? 1024 : 16 * QT;     // query / gradient tile; row statistics (copies of 1 KB)
+    constexpr int TB = L::bytes(QT), SB = 32 * QT;         // query / gradient tile; row statistics, all but the last (copies of 1 KB)
     constexpr int BUF = 2 * TB + SB;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h2 = lane >> 5;
@@ -867,11 +916,12 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<
         const int have = a.Tq - pos.tile * QT;
         q_copy.issue(pos.q, have, dst);
         g_copy.issue(pos.g, have, dst + TB);
-        if (wave * 64 < QT) {
+        static_assert(2 * QT % 64 == 0 && 2 * QT <= 64 * NW, "whole waves copy the statistics");
+        if (wave * 64 < 2 * QT) {
             const __amdgpu_buffer_rsrc_t rs =
-                __builtin_amdgcn_make_buffer_rsrc((void*)pos.stat, 0, (unsigned)(3 * a.Tp + QT) * 4u, 0x00020000);
+                __builtin_amdgcn_make_buffer_rsrc((void*)pos.stat, 0, (unsigned)((STATS - 2) * a.Tp + QT) * 4u, 0x00020000);
             const int piece = wave * 64 + lane;
-            copy_piece(rs, dst + 2 * TB + wave * 1024, piece < QT ? piece / (QT / 4) * a.Tp * 4 + piece % (QT / 4) * 16 : (int)0x80000000, 0);
+            copy_piece(rs, dst + 2 * TB + wave * 1024, piece / (QT / 4) * a.Tp * 4 + piece % (QT / 4) * 16, 0);
         }
         if (pos.tile + 1 == q_tiles) {
             go_to(pos.head + 1, q_first);       // (behind the last head nothing is read any more)
@@ -900,6 +950,8 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<
         lds_cptr const gt = cur + TB;
         const SF_LDS float* const stat = (const SF_LDS float*)(cur + 2 * TB) + rows0;            // [STATS - 1][QT]
         const bool edge = w_first + 32 > kend || (a.causal && t0 < w_tmax);
+        const bool wide = __any(!(fmaxf(fabsf(stat[lane & 31]), fabsf(stat[2 * QT + (lane & 31)])) < NEAR));
+        const SF_LDS float* const lse = wide ? stat + 5 * QT : stat;            // or lg, with ref to be taken off the scores first
         f32x16 dp;                      // dP - delta_1
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
@@ -925,6 +977,14 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = t0 + acc_row(r, h2) >= t_min ? s[r] : -INFINITY;
             }
+            if (wide) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const f32x4 ref = *(const SF_LDS f32x4*)(stat + (4 + 2 * i) * QT + acc_row(r, h2));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[r + e] -= ref[e];
+                }
+            }
             Frag<T> df[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -932,12 +992,12 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<
 #pragma unroll
                 for (int k = 0; k < 8; k += 4) {
                     const int r = 8 * u + k;
-                    const f32x4 lv = *(const SF_LDS f32x4*)(stat + 2 * QT * i + acc_row(r, h2));
+                    const f32x4 lv = *(const SF_LDS f32x4*)(lse + 2 * QT * i + acc_row(r, h2));
                     f32x4 apart{};
                     if (i) apart = *(const SF_LDS f32x4*)(stat + 3 * QT + acc_row(r, h2));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float y = __builtin_amdgcn_exp2f(s[r + e] * a.c - lv[e]);
+                        const float y = __builtin_amdgcn_exp2f(fmaf(s[r + e], a.c, -lv[e]));
                         p[r + e] = i ? fmaf(-lam, y, p[r + e]) : y;
                         ds[k + e] = y * (i ? fmaf(-lam, dp[r + e], apart[e]) : dp[r + e]);
                     }
@@ -1030,7 +1090,7 @@ template <typename T, int DP, bool KEYS> __global__ __launch_bounds__(256) void 
         const float* const sums = a.part + (long long)items * a.parts * RB * W + (long long)tail * a.parts * RB + id % RB;
         const float sum = wave_sum(lane < a.parts ? sums[(long long)lane * RB] : 0.f);
         float* const stat = a.stat + ((long long)b * a.H + hk * group + row % group) * STATS * a.Tp + row / group;
-        if (lane == 0) stat[4LL * a.Tp] = sum - stat[a.Tp];
+        if (lane == 0) stat[(STATS - 1LL) * a.Tp] = sum - stat[a.Tp];
     }
     for (int c = lane; c < W; c += 64) {
         const int half = c / DP & 1, j = c % DP;
@@ -1233,7 +1293,7 @@ template <typename T, int DP> int launch_bwd(Args<T> a, const RowPlan& f, const 
     a.full = ck.full;
     a.parts = ck.parts;
     if (g.split) {
-        constexpr int NW = DP == 64 ? 2 : 4, QT = 32 * NW, lds = L::bytes(32) + 2 * (2 * L::bytes(QT) + 16 * (QT < 64 ? 64 : QT));
+        constexpr int NW = DP == 64 ? 2 : 4, QT = 32 * NW, lds = L::bytes(32) + 2 * (2 * L::bytes(QT) + 32 * QT);
         static_assert(lds >= (2 * DP / 32 < 2 ? 2 : 2 * DP / 32) * 4096, "the waves' box");
         SF_LDS_ONCE((attn_dkv_kernel<T, DP, NW, true>), lds);
         hipLaunchKernelGGL((attn_dkv_kernel<T, DP, NW, true>), dim3(ck.full + ck.tail * ck.parts), dim3(64 * NW), lds, st, a);
@@ -1251,19 +1311,19 @@ template <typename T, int DP> int launch_bwd(Args<T> a, const RowPlan& f, const 
 }
 
 template <typename T> int fwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
-                              const int* lengths, void* o, float* maps, float* lse, float* part, hipStream_t st) {
+                              const int* lengths, void* o, float* maps, float* sums, float* part, hipStream_t st) {
     Args<T> a = make_args<T>(p, q, k, v, lam, lengths);
-    a.o = (T*)o; a.maps = maps; a.lse = lse; a.part = part;
+    a.o = (T*)o; a.maps = maps; a.sums = sums; a.part = part;
     const RowPlan f = fwd_plan(p);
     const int dp = padded(p->d);
     return dp == 16 ? launch_fwd<T, 16>(a, f, st) : dp == 32 ? launch_fwd<T, 32>(a, f, st) : launch_fwd<T, 64>(a, f, st);
 }
 size_t stat_bytes(const sf_diff_attn_desc* p) { return (size_t)p->B * p->H * padded_rows(p) * STATS * sizeof(float); }
 template <typename T> int bwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
-                              const int* lengths, const float* maps, const float* lse, const void* dout, void* dq, void* dk,
+                              const int* lengths, const float* maps, const float* sums, const void* dout, void* dq, void* dk,
                               void* dv, void* dlam, char* ws, hipStream_t st) {
     Args<T> a = make_args<T>(p, q, k, v, lam, lengths);
-    a.maps_in = maps; a.lse_in = lse; a.dout = (const T*)dout;
+    a.maps_in = maps; a.sums_in = sums; a.dout = (const T*)dout;
     a.stat = (float*)ws;
     a.part = (float*)(ws + stat_bytes(p));
     a.dq = (T*)dq; a.dk = (T*)dk; a.dv = (T*)dv;
@@ -1288,16 +1348,17 @@ extern "C" size_t sf_diff_attn_fwd_workspace_bytes(const sf_diff_attn_desc* p) {
 }
 
 extern "C" int sf_diff_attn_fwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
-                                const int* lengths, void* o, float* maps, float* lse, void* ws, size_t ws_bytes, void* stream) {
+                                const int* lengths, void* o, float* maps, float* sums, void* ws, size_t ws_bytes, void* stream) {
     if (int rc = check_desc(p, "sf_diff_attn_fwd")) return rc;
     const void* ps[] = {q, k, v, o};
     if (int rc = check_align(ps, 4, "sf_diff_attn_fwd")) return rc;
-    SF_REQUIRE(lam && (!maps == !lse) && (uintptr_t)maps % 16 == 0, "sf_diff_attn_fwd: lam is missing, or maps and lse are not both given");
+    SF_REQUIRE(lam && (!maps == !sums) && (uintptr_t)maps % 16 == 0 && (uintptr_t)sums % 16 == 0,
+               "sf_diff_attn_fwd: lam is missing, or maps and sums are not both given and 16-byte aligned");
     const size_t need = sf_diff_attn_fwd_workspace_bytes(p);
     SF_REQUIRE(!need || (ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0), "sf_diff_attn_fwd: workspace of %zu bytes is too small (%zu)",
                ws_bytes, need);
-    return p->dtype == SF_BF16 ? fwd<bf16>(p, q, k, v, lam, lengths, o, maps, lse, (float*)ws, (hipStream_t)stream)
-                               : fwd<float>(p, q, k, v, lam, lengths, o, maps, lse, (float*)ws, (hipStream_t)stream);
+    return p->dtype == SF_BF16 ? fwd<bf16>(p, q, k, v, lam, lengths, o, maps, sums, (float*)ws, (hipStream_t)stream)
+                               : fwd<float>(p, q, k, v, lam, lengths, o, maps, sums, (float*)ws, (hipStream_t)stream);
 }
 
 extern "C" size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* p) {
@@ -1309,15 +1370,15 @@ extern "C" size_t sf_diff_attn_bwd_workspace_bytes(const sf_diff_attn_desc* p) {
 }
 
 extern "C" int sf_diff_attn_bwd(const sf_diff_attn_desc* p, const void* q, const void* k, const void* v, const void* lam,
-                                const int* lengths, const float* maps, const float* lse, const void* dout, void* dq, void* dk,
+                                const int* lengths, const float* maps, const float* sums, const void* dout, void* dq, void* dk,
                                 void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream) {
     if (int rc = check_bwd_desc(p, "sf_diff_attn_bwd")) return rc;
-    const void* ps[] = {q, k, v, maps, dout, dq, dk, dv, lse};
+    const void* ps[] = {q, k, v, maps, dout, dq, dk, dv, sums};
     if (int rc = check_align(ps, 9, "sf_diff_attn_bwd")) return rc;
     const size_t need = sf_diff_attn_bwd_workspace_bytes(p);
     SF_REQUIRE(lam && ws && ws_bytes >= need && (uintptr_t)ws % 16 == 0, "sf_diff_attn_bwd: workspace of %zu bytes is too small (%zu)",
                ws_bytes, need);
     return p->dtype == SF_BF16
-               ? bwd<bf16>(p, q, k, v, lam, lengths, maps, lse, dout, dq, dk, dv, dlam, (char*)ws, (hipStream_t)stream)
-               : bwd<float>(p, q, k, v, lam, lengths, maps, lse, dout, dq, dk, dv, dlam, (char*)ws, (hipStream_t)stream);
+               ? bwd<bf16>(p, q, k, v, lam, lengths, maps, sums, dout, dq, dk, dv, dlam, (char*)ws, (hipStream_t)stream)
+               : bwd<float>(p, q, k, v, lam, lengths, maps, sums, dout, dq, dk, dv, dlam, (char*)ws, (hipStream_t)stream);
 }

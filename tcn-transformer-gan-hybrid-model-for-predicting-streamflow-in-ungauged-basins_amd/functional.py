@@ -877,15 +877,15 @@ class DiffAttentionFn(torch.autograd.Function):
         need = any(ctx.needs_input_grad[:4])
         o, saved = ops.diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need, strides)
         if need:
-            ctx.desc, maps, lse = saved or (None, None, None)       # (no query or no key: nothing to save)
+            ctx.desc, maps, sums = saved or (None, None, None)       # (no query or no key: nothing to save)
             ctx.strides = (q.stride(), k.stride(), v.stride())
-            ctx.save_for_backward(q, k, v, lam, lengths, maps, lse)
+            ctx.save_for_backward(q, k, v, lam, lengths, maps, sums)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, lam, lengths, maps, lse = ctx.saved_tensors
+        q, k, v, lam, lengths, maps, sums = ctx.saved_tensors
         if ctx.desc is None:
             return (*(torch.zeros(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v, lam)), None, None, None, None)
         desc = ctx.desc
@@ -894,8 +894,8 @@ class DiffAttentionFn(torch.autograd.Function):
             (q, k, v), strides = ops.kernel_layouts(q, k, v)
             desc = ops.diff_attn_desc(q, k, v, lam, desc.causal, desc.scale, strides)
         # (a contiguous gradient may start anywhere: the backward pass of a concatenation hands over slices of a flat buffer)
-        maps, lse, do = (ops.aligned(t) for t in (maps, lse, do))
-        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, desc, maps, lse, do, ctx.needs_input_grad[3])
+        maps, sums, do = (ops.aligned(t) for t in (maps, sums, do))
+        grads = ops.diff_attn_bwd(q, k, v, lam, lengths, desc, maps, sums, do, ctx.needs_input_grad[3])
         return (*grads, None, None, None, None)
 
 

@@ -1210,28 +1210,28 @@ def diff_attn_fwd(q, k, v, lam, lengths, causal, scale, need_save=False, strides
         return o.zero_(), None
     desc = diff_attn_desc(q, k, v, lam, causal, scale, strides)
     at = ctypes.addressof(desc)
-    maps = lse = None
+    maps = sums = None
     if need_save:
         maps = torch.empty((B, Tq, H, 2, 2 * d), device=q.device, dtype=torch.float32)
-        lse = torch.empty((B, H, Tq, 2), device=q.device, dtype=torch.float32)
+        sums = torch.empty((B, H, Tq, 2, 2), device=q.device, dtype=torch.float32)
     nb = lib().sf_diff_attn_fwd_workspace_bytes(at)
     ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
     _check(lib().sf_diff_attn_fwd(at, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _at(lengths), o.data_ptr(),
-                                  _at(maps), _at(lse), _at(ws), nb, _stream_of(q)), "sf_diff_attn_fwd")
-    return o, (desc, maps, lse)
+                                  _at(maps), _at(sums), _at(ws), nb, _stream_of(q)), "sf_diff_attn_fwd")
+    return o, (desc, maps, sums)
 
 
-def diff_attn_bwd(q, k, v, lam, lengths, desc, maps, lse, do, need_dlam=True):
-    """(dq, dk, dv, dlam), contiguous; maps, lse: what diff_attn_fwd saved for the same q, k, v, lam, lengths; desc: the one it
+def diff_attn_bwd(q, k, v, lam, lengths, desc, maps, sums, do, need_dlam=True):
+    """(dq, dk, dv, dlam), contiguous; maps, sums: what diff_attn_fwd saved for the same q, k, v, lam, lengths; desc: the one it
     saved, if their layouts are still the same."""
-    _dev(lam, lengths, maps, lse, do, dtypes=[None, torch.int32, torch.float32, torch.float32, q.dtype])
+    _dev(lam, lengths, maps, sums, do, dtypes=[None, torch.int32, torch.float32, torch.float32, q.dtype])
     dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
     dlam = torch.empty_like(lam) if need_dlam else None
     at = ctypes.addressof(desc)
     nb = lib().sf_diff_attn_bwd_workspace_bytes(at)
     ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
     _check(lib().sf_diff_attn_bwd(at, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _at(lengths), maps.data_ptr(),
-                                  lse.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(dlam), ws.data_ptr(),
+                                  sums.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(dlam), ws.data_ptr(),
                                   nb, _stream_of(q)), "sf_diff_attn_bwd")
     return dq, dk, dv, dlam
 

@@ -579,3 +579,91 @@ def test_gradients_at_any_address(dtype):
     with torch.autograd.graph.saved_tensors_hooks(odd, lambda t: t):
         got = torch.autograd.grad(sf.functional.diff_attention(*leaves), leaves, do)
     assert all(torch.equal(a, want[n]) for a, n in zip(got, ("dq", "dk", "dv", "dlam")))
+
+
+def oracle_on_gpu(q, k, v, lam, causal, lengths, scale, do):
+    """oracle() with the heads of a sample at once, in 64 bits on the GPU: outputs and the sums of their terms' magnitudes."""
+    q, k, v, lam, do = (x.detach().double().cuda() for x in (q, k, v, lam, do))
+    B, Tq, H, _, d = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    g = H // Hk
+    out = {n: torch.zeros(s, dtype=torch.float64, device="cuda") for n, s in (
+        ("o", (B, Tq, H, 2 * d)), ("dq", q.shape), ("dk", k.shape), ("dv", v.shape), ("dlam", lam.shape))}
+    mag = {n: torch.zeros_like(x) for n, x in out.items()}
+    key = torch.arange(Tk, device="cuda")
+    w = lam.view(H, 1, 1)
+
+    def shared(x):          # gradients of the group's heads add up in their key / value head
+        return x.view(Hk, g, *x.shape[1:]).sum(1).transpose(0, 1)
+    for b in range(B):
+        n = Tk if lengths is None else max(0, min(Tk, int(lengths[b])))
+        hide = (key[None, :] >= n).expand(Tq, Tk)
+        if causal:
+            hide = hide | (key[None, :] > torch.arange(Tq, device="cuda")[:, None] + (Tk - Tq))
+        live = (key < n).double()
+        kb = (k[b] * live.view(Tk, 1, 1, 1)).permute(1, 2, 0, 3).repeat_interleave(g, 0)        # [H, 2, Tk, d]
+        vb = (v[b] * live.view(Tk, 1, 1)).transpose(0, 1).repeat_interleave(g, 0)               # [H, Tk, 2 d]
+        qb, G = q[b].permute(1, 2, 0, 3), do[b].transpose(0, 1)                                 # [H, 2, Tq, d], [H, Tq, 2 d]
+        z = (qb @ kb.transpose(-1, -2).contiguous() * scale).masked_fill(hide, -math.inf)
+        top = z.amax(-1, keepdim=True)
+        e = torch.exp(z - torch.where(top == -math.inf, 0.0, top))
+        P = e / e.sum(-1, keepdim=True).clamp_min(1e-300)
+        A, M = P[:, 0] - w * P[:, 1], P[:, 0] + w.abs() * P[:, 1]
+        va, Ga = vb.abs(), G.abs()
+        out["o"][b], mag["o"][b] = (A @ vb).transpose(0, 1), (M @ va).transpose(0, 1)
+        dP, dPm = G @ vb.transpose(-1, -2).contiguous(), G.abs()
+        out["dv"][b] = shared(A.transpose(-1, -2).contiguous() @ G)
+        mag["dv"][b] = shared(M.transpose(-1, -2).contiguous() @ Ga)
+        out["dlam"] -= (P[:, 1] * dP).sum((1, 2))
+        mag["dlam"] += (dPm * (P[:, 1] @ va)).sum((1, 2))
+        dm = (Ga * ((P[:, 0] + w.abs() * 2 * P[:, 1]) @ va)).sum(-1, keepdim=True)
+        for i, f in ((0, torch.ones_like(w)), (1, -w)):
+            delta = (P[:, i] * dP).sum(-1, keepdim=True)
+            dS = f * P[:, i] * (dP - delta) * scale
+            dSm = f.abs() * P[:, i] * (dP.abs() + dm) * scale
+            out["dq"][b, :, :, i], mag["dq"][b, :, :, i] = (dS @ kb[:, i]).transpose(0, 1), (dSm @ kb[:, i].abs()).transpose(0, 1)
+            out["dk"][b, :, :, i] = shared(dS.transpose(-1, -2).contiguous() @ qb[:, i])
+            mag["dk"][b, :, :, i] = shared(dSm.transpose(-1, -2).contiguous() @ qb[:, i].abs())
+    return out, mag
+
+
+def within_terms(sf, q, k, v, lam, do, causal=False, lengths=None):
+    """Every output of a forward and backward pass within the bound of its terms; returns the passes' outputs."""
+    o, g = run(sf, q, k, v, lam, do, causal=causal, lengths=lengths)
+    want, mag = oracle_on_gpu(q, k, v, lam, causal, lengths, q.shape[-1] ** -0.5, do)
+    for n, x in {"o": o, **g}.items():
+        err, lim = (x.detach().double() - want[n]).abs(), bound(want[n], mag[n], q.dtype) + 1e-30
+        assert bool((err <= lim).all()), f"{n}: off by {float((err / lim).max()):.3g} times the bound"     # (NaN fails too)
+    return o, g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [8, 13, 20, 24, 27, 33, 100])
+@pytest.mark.parametrize("d", [8, 32, 64])
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_finite_scores_of_any_size(power, d, dtype):
+    """Scores of about 2.25 * 2^power, positive in the first map and negative in the second, that differ by 0 to 12 small
+    steps: the softmax only knows the differences.  Ties for the largest lie in different tiles and parts.  The scores are exact
+    in f32: two products, one of two numbers of two bits, the other step n, the sum of at most 24 bits since a step is at least
+    2^(power - 22).  Queries are larger and smaller by powers of two, so rows of all sizes share a wave, down to a zero one whose
+    scores are the steps alone.  In the second form the scores climb by a factor 2^15 along the keys.
+    Bounds as for other scores: an exponent is a difference of scores times the scale in two roundings, 2^-23 of itself, and
+    a probability 2^-x has at most 2^-x x 2^-23 <= 2^-23 of an error from it (x 2^-x < 1), below the 2^-24 * 256 of its terms."""
+    sf = load_pkg()
+    e = power // 2
+    for (B, Tq, Tk, H, Hk), causal, lengths in (((2, 70, 300, 2, 1), True, [300, 77]), ((1, 1, 4000, 2, 2), False, None),
+                                                ((1, 300, 300, 2, 2), False, None), ((16, 260, 260, 8, 8), False, None)):
+        for climb in (False, True):
+            q, k, v, lam, do = make(B, Tq, Tk, H, Hk, d, F, seed=power + d)
+            gen = torch.Generator().manual_seed(power)
+            q.zero_()
+            k.zero_()
+            size = torch.tensor([1.0, 2.0 ** -4, 2.0 ** -8, 0.0])[torch.arange(Tq) % 4].view(1, Tq, 1)
+            n = torch.randint(0, 13, (B, Tk, Hk, 2), generator=gen).float()
+            n[:, [3, Tk // 2, Tk - 1]] = 0
+            rise = torch.ldexp(torch.ones(Tk), (torch.arange(Tk) * 16 // Tk if climb else torch.full((Tk,), 15)) - 15).view(1, Tk, 1)
+            for i, sign in ((0, 1.0), (1, -1.0)):
+                q[..., i, 0], q[..., i, 1] = sign * 1.5 * 2.0 ** e * size, 1.0
+                k[..., i, 0], k[..., i, 1] = 1.5 * 2.0 ** (power - e) * rise, -n[..., i] * 2.0 ** max(0, power - 22)
+            ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+            within_terms(sf, *(t.to(dtype) for t in (q, k, v)), lam, do.to(dtype), causal, ln)
