@@ -667,3 +667,44 @@ def test_finite_scores_of_any_size(power, d, dtype):
                 k[..., i, 0], k[..., i, 1] = 1.5 * 2.0 ** (power - e) * rise, -n[..., i] * 2.0 ** max(0, power - 22)
             ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
             within_terms(sf, *(t.to(dtype) for t in (q, k, v)), lam, do.to(dtype), causal, ln)
+
+
+# Shapes whose work items are more than one round of the chip and whose last ones are cut into parts (forward or query
+# gradients: by rows and by keys; key gradients: by keys and by rows), and causal ones of more than 512 items, every other 256 of
+# which are taken in reverse.  (B, Tq, Tk, H, Hk, d, causal)
+MANY = [(16, 775, 1191, 8, 2, 8, False), (33, 48, 231, 16, 16, 24, False), (33, 86, 720, 16, 8, 64, False), (33, 17, 1517, 16, 16, 64, False),
+        (33, 24, 1626, 16, 8, 8, False), (33, 652, 699, 4, 4, 8, False), (64, 1527, 398, 4, 1, 8, False), (33, 350, 130, 16, 8, 64, False),
+        (33, 98, 98, 16, 16, 8, True), (33, 70, 1773, 16, 2, 8, True), (33, 133, 866, 16, 2, 64, True), (33, 202, 1444, 8, 4, 24, True),
+        (33, 399, 399, 4, 4, 24, True), (64, 39, 1219, 8, 1, 64, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", MANY, ids=str)
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_many_items(shape, dtype):
+    *sizes, causal = shape
+    B, Tk = shape[0], shape[2]
+    x = make(*sizes, dtype, seed=21)
+    within_terms(load_pkg(), *x, causal=causal)
+    lengths = (torch.arange(B) * 37 % (Tk + 1)).to(torch.int32).cuda()
+    lengths[-1] = Tk
+    within_terms(load_pkg(), *x, causal=causal, lengths=lengths)
+
+
+def test_plans_of_many_items():
+    """The shapes above reach what they are for: a cut forward pass has a workspace, and a cut backward pass one
+    beyond its statistics (no GPU needed)."""
+    import ctypes
+    sf = load_pkg()
+    L, D = sf.ops.lib(), sf.ops.DiffAttnDesc
+    cut = {"fwd": 0, "bwd": 0}
+    for B, Tq, Tk, H, Hk, d, causal in MANY:
+        for code in (0, 1):
+            ll3 = ctypes.c_longlong * 3
+            w = 2 * d
+            desc = D(code, 0, B, Tq, Tk, H, Hk, d, int(causal), 0.25, ll3(Tq * H * w, H * w, w), ll3(Tk * Hk * w, Hk * w, w),
+                     ll3(Tk * Hk * w, Hk * w, w))
+            least = B * H * ((Tq + 127) // 128 * 128) * 9 * 4       # nine values of a row
+            cut["fwd"] += int(L.sf_diff_attn_fwd_workspace_bytes(ctypes.byref(desc))) > 0
+            cut["bwd"] += int(L.sf_diff_attn_bwd_workspace_bytes(ctypes.byref(desc))) > least
+    assert cut["fwd"] >= 8 and cut["bwd"] >= 16, cut
