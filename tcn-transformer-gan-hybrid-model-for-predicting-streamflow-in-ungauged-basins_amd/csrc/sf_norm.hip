@@ -5,9 +5,11 @@
 //   mu = mean(s),  var = mean((s - mu)^2),  r = 1 / sqrt(var + eps),  xh = (s - mu) r,  y = w xh + b
 //   backward, g = w dy:  ds_total = r (g - mean(g) - xh mean(g xh)) + ds,  dw = sum_rows dy xh,  db = sum_rows dy
 //
-// All statistics and sums are f32 (the variance from the centred values: no cancellation for rows far from
-// zero); values are rounded to bf16 once, at the store.  Both directions are bound by HBM: every array is
-// read or written exactly once, because a row lives in registers between its statistics and its output.
+// All statistics and sums are f32; values are rounded to bf16 once, at the store.  A row's first mean is off by a few f32 steps of
+// its size, which for rows far from zero may be more than their spread (0.05 at 1e5, where sqrt(eps) is 0.003): the centred
+// values' own mean, summed beside their squares, takes that out of the values, the variance and the mean that is kept.
+// Both directions are bound by HBM: rows of up to 8192 values are read and every array written exactly once,
+// because a row lives in registers between its statistics and its output.
 // A row belongs to G lanes (8 to 64 lanes of a wave, or the 256 threads of a workgroup), each holding NC
 // pieces of 16 bytes; G and NC follow from the width alone (row_plan).  Workgroups are persistent: a lane's
 // columns never change, so the weights and, backward, the sums of dw and db stay in its registers over all
@@ -20,6 +22,7 @@
 //   30011 x 999 f32: forward 41 us, 240 MB, 5.9 TB/s; backward 71 us, 360 MB, 5.0 TB/s, and 5 us for the fold
 //   160 x 128 bf16: 4, 6 and 3 us, all of it launch and latency
 #include "sf_common.h"
+#include <float.h>
 #include "../../include/sfhip.h"
 
 namespace {
@@ -48,6 +51,34 @@ template <int G> __device__ __forceinline__ float row_sum(float v, float* sm) {
     if constexpr (G == NT) return block_sum_256(v, sm);
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// the same of two values at once (sm: 8 floats)
+template <int G> __device__ __forceinline__ void row_sums(float& a, float& b, float* sm) {
+    if constexpr (G == NT) {
+        a = wave_sum(a);
+        b = wave_sum(b);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            sm[threadIdx.x >> 6] = a;
+            sm[4 + (threadIdx.x >> 6)] = b;
+        }
+        __syncthreads();
+        a = sm[0] + sm[1] + sm[2] + sm[3];
+        b = sm[4] + sm[5] + sm[6] + sm[7];
+    } else {
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) {
+            a += __shfl_xor(a, o, 64);
+            b += __shfl_xor(b, o, 64);
+        }
+    }
+}
+
+// a row's statistic where whole waves share a row: a scalar register
+template <int G> __device__ __forceinline__ float shared(float v) {
+    if constexpr (G >= 64) return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
     return v;
 }
 
@@ -81,7 +112,7 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(const T* __restrict__ x, c
                                                       const float* __restrict__ w, const float* __restrict__ b,
                                                       T* __restrict__ y, float* __restrict__ mean_out,
                                                       float* __restrict__ rstd_out, long long rows, int D, float eps) {
-    __shared__ float sm[4];
+    __shared__ float sm[8];
     constexpr int RPB = NT / G;
     const int q = threadIdx.x % G;
     const Cols<G, NC, V, FULL> C(q, D);
@@ -96,7 +127,7 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(const T* __restrict__ x, c
             if (!b) bv[c][j] = 0.f;
         }
     }
-    const float inv = 1.0f / (float)D;
+    const float count = (float)D;       // (divided by: a rounded reciprocal would put the mean of equal values off them)
     for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
         const long long row = r0 + threadIdx.x / G;
         const bool have = row < rows;                     // lanes behind the last row repeat it without a store
@@ -120,24 +151,29 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(const T* __restrict__ x, c
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int j = 0; j < V; ++j) a += j >= C.skip[c] ? v[c][j] : 0.f;
-        const float mean = row_sum<G>(a, sm) * inv;
+        const float mean = shared<G>(row_sum<G>(a, sm) / count);
         a = 0.f;
+        float off = 0.f;                                  // mean of the centred values
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 v[c][j] -= mean;
                 a += j >= C.skip[c] ? v[c][j] * v[c][j] : 0.f;
+                off += j >= C.skip[c] ? v[c][j] : 0.f;
             }
-        const float rstd = 1.0f / sqrtf(row_sum<G>(a, sm) * inv + eps);
+        row_sums<G>(a, off, sm);
+        off = shared<G>(off / count);
+        // (squares that overflow leave an infinite variance, not inf - inf)
+        const float rstd = shared<G>(1.0f / sqrtf(fmaxf(a / count - fminf(off * off, FLT_MAX), 0.f) + eps));
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[c][j] = v[c][j] * rstd * wv[c][j] + bv[c][j];
+            for (int j = 0; j < V; ++j) v[c][j] = (v[c][j] - off) * rstd * wv[c][j] + bv[c][j];
             if (have && C.live[c]) store_vec<T, V>(y + at + C.col[c], v[c]);
         }
         if (mean_out && have && q == 0) {
-            mean_out[row] = mean;
+            mean_out[row] = mean + off;
             rstd_out[row] = rstd;
         }
     }
@@ -250,35 +286,39 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(const T* __restrict__ dy, 
 }
 
 // Rows wider than the registers of a workgroup hold: one workgroup per row, the row read again for each of
-// its passes (from the L2 as far as it reaches).
+// its passes (three forward, two backward; from the L2 as far as it reaches).  A thread adds up to 65536 values one after the
+// other: in 64 bits.
 template <typename T>
 __global__ __launch_bounds__(NT) void norm_fwd_wide_kernel(const T* __restrict__ x, const T* __restrict__ res,
                                                            T* __restrict__ sum, const float* __restrict__ w,
                                                            const float* __restrict__ b, T* __restrict__ y,
                                                            float* __restrict__ mean_out, float* __restrict__ rstd_out,
                                                            long long rows, int D, float eps) {
-    __shared__ float sm[4];
-    const float inv = 1.0f / (float)D;
+    __shared__ double sm[4];
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
         const T* xr = x + row * D;
         const T* rr = res ? res + row * D : nullptr;
         auto value = [&](int i) { return rr ? to_f32(from_f32<T>(to_f32(xr[i]) + to_f32(rr[i]))) : to_f32(xr[i]); };
-        float a = 0.f;
-        for (int i = threadIdx.x; i < D; i += NT) a += value(i);
-        const float mean = block_sum_256(a, sm) * inv;
-        a = 0.f;
+        double a = 0.0;
+        for (int i = threadIdx.x; i < D; i += NT) a += (double)value(i);
+        const float mean = (float)(block_sum_256_d(a, sm) / D);
+        double q = 0.0;
+        a = 0.0;
         for (int i = threadIdx.x; i < D; i += NT) {
-            const float c = value(i) - mean;
-            a += c * c;
+            const double c = (double)(value(i) - mean);
+            q += c * c;
+            a += c;
         }
-        const float rstd = 1.0f / sqrtf(block_sum_256(a, sm) * inv + eps);
+        a = block_sum_256_d(a, sm) / D;
+        q = block_sum_256_d(q, sm) / D - a * a;
+        const float off = (float)a, rstd = 1.0f / sqrtf((float)fmax(q, 0.0) + eps);
         for (int i = threadIdx.x; i < D; i += NT) {
             const float v = value(i);
             if (rr) sum[row * D + i] = from_f32<T>(v);
-            y[row * D + i] = from_f32<T>((v - mean) * rstd * (w ? w[i] : 1.f) + (b ? b[i] : 0.f));
+            y[row * D + i] = from_f32<T>((v - mean - off) * rstd * (w ? w[i] : 1.f) + (b ? b[i] : 0.f));
         }
         if (mean_out && threadIdx.x == 0) {
-            mean_out[row] = mean;
+            mean_out[row] = mean + off;
             rstd_out[row] = rstd;
         }
     }
@@ -288,18 +328,16 @@ __global__ __launch_bounds__(NT) void norm_bwd_wide_kernel(const T* __restrict__
                                                            const T* __restrict__ s, const float* __restrict__ w,
                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
                                                            T* __restrict__ dx, long long rows, int D) {
-    __shared__ float sm[4];
-    const float inv = 1.0f / (float)D;
+    __shared__ double sm[4];
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
         const float mu = mean[row], rs = rstd[row];
-        float m1 = 0.f, m2 = 0.f;
+        double g1 = 0.0, g2 = 0.0;
         for (int i = threadIdx.x; i < D; i += NT) {
             const float g = to_f32(dy[row * D + i]) * (w ? w[i] : 1.f);
-            m1 += g;
-            m2 += g * (to_f32(s[row * D + i]) - mu) * rs;
+            g1 += (double)g;
+            g2 += (double)(g * ((to_f32(s[row * D + i]) - mu) * rs));
         }
-        m1 = block_sum_256(m1, sm) * inv;
-        m2 = block_sum_256(m2, sm) * inv;
+        const float m1 = (float)(block_sum_256_d(g1, sm) / D), m2 = (float)(block_sum_256_d(g2, sm) / D);
         for (int i = threadIdx.x; i < D; i += NT) {
             const float g = to_f32(dy[row * D + i]) * (w ? w[i] : 1.f);
             float v = rs * (g - m1 - (to_f32(s[row * D + i]) - mu) * rs * m2);

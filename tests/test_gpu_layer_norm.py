@@ -7,6 +7,8 @@ pairwise order keeps the error of a mean below a few f32 steps of the row's larg
 the largest magnitude of the row's terms cover the chain.  dw and db are f32 sums over the rows: every
 partial sum is rounded to f32, (64 + sqrt(rows)) steps of the sum of magnitudes / sqrt(rows) bound a random walk of
 them with room to spare; the bound used is rows-independent in the worst case: 2^-24 * 64 * sum |terms|."""
+import math
+
 import pytest
 import torch
 
@@ -355,3 +357,52 @@ def test_offsets_beyond_32_bits():
     yt = sf.functional.layer_norm(tail, w, None)
     dt, = torch.autograd.grad(yt, tail, tail.detach())
     assert torch.equal(y[-1000:], yt) and torch.equal(dx[-1000:], dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [96, 999, 1000, 4095, 8191, 8195, 50001, (1 << 20) + 3])
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_rows_without_spread(D, dtype):
+    """Rows of one value, far from zero: the centred values are zero, so y is the bias and dx is r (g - mean(g)), r = 1 / sqrt(eps).
+    The kernel's first mean is off by k steps of the value, k below the 32 + 8 roundings of its sum; k, k^2 and their sums over D
+    values are whole numbers below 2^24 of those steps (D <= 8192; wider rows are summed in 64 bits), hence exact, and so the second mean
+    takes all of the first one's error out: y is w * 0 + b exactly.  dx: mean(g) is off by at most 64 f32 half steps
+    of the mean magnitude, r by 4 of itself, and dx is rounded once."""
+    sf = load_pkg()
+    vals = torch.tensor([1e3, -3.3e4, 1e5, -1e6, 7.0, 0.0]).to(dtype)
+    x = vals.view(-1, 1).expand(-1, D).contiguous()
+    g = torch.Generator().manual_seed(D)
+    w, b = 1 + 0.3 * torch.randn(D, generator=g), 0.3 * torch.randn(D, generator=g)
+    dy = torch.randn(len(vals), D, generator=g).to(dtype)
+    y, _, grads = run(sf, x, None, w, b, dy, None)
+    assert torch.equal(y.detach().cpu(), b.to(dtype).expand(len(vals), D))
+    gw = dy.double() * w.double()
+    r = 1e-5 ** -0.5
+    want = r * (gw - gw.mean(1, keepdim=True))
+    check(grads["dx"], want, want.abs() * (torch.finfo(dtype).eps / 2 * 1.01 + 4 * U32) + r * 64 * U32 * (gw.abs().mean(1, keepdim=True) + gw.abs()), "dx")
+    assert float(grads["dw"].abs().max()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [999, 1000, 8192, 8195, (1 << 20) + 3])
+@pytest.mark.parametrize("offset", [1e3, 3e4, 1e6])
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_rows_of_few_values_far_from_zero(D, offset, dtype):
+    """Rows that differ by single steps of their type around a large value: the deviations are exact, so y is known to their
+    precision, not to that of the offset.  In steps s of f32 at the offset: the first mean is off by at most 40 s (1/2 s for wide rows,
+    in 64 bits), the centred values are exact multiples of s / 2 or so, rounded to U32 of their size (at most 44 s or the spread), their mean
+    likewise: 40 U32 of (44 s + the largest deviation) for all of it.  The variance loses as much again, relative to itself
+    or, where the correction is the larger part, 40 U32 of (44 s)^2."""
+    sf = load_pkg()
+    g = torch.Generator().manual_seed(D)
+    base = torch.full((4, D), offset).to(dtype)
+    step = torch.finfo(dtype).eps * 2.0 ** torch.floor(torch.log2(base.float().abs()))
+    x = (base.double() + torch.randint(-1, 3, (4, D), generator=g) * step.double()).to(dtype)
+    w, b = 1 + 0.3 * torch.randn(D, generator=g), 0.3 * torch.randn(D, generator=g)
+    y = sf.functional.layer_norm(x.cuda(), w.cuda(), b.cuda())
+    o = oracle(x, None, w, b, 1e-5)
+    s = torch.finfo(F).eps * 2.0 ** math.floor(math.log2(offset))
+    dev = (o["s"] - o["s"].mean(1, keepdim=True)).abs().amax(1, keepdim=True)
+    off = 40 * U32 * (44 * s + dev) * o["r"]                      # of the normalised value
+    rel = 40 * U32 * (1 + (44 * s * o["r"]) ** 2)                 # of r
+    check(y, o["y"], o["y"].abs() * (torch.finfo(dtype).eps / 2 * 1.01) + w.double().abs() * (off + rel * o["xh"].abs()) + 4 * U32 * (b.double().abs() + o["xh"].abs() * w.double().abs()), "y")
