@@ -42,7 +42,7 @@ struct Tensor {
     unsigned char* ve;
     bf16* shadow;
     long long n;
-    float lr, keep;                // keep = 1 - lr * weight decay
+    float lr, decay;               // decay = lr * weight decay
     int step_offset;
     int ordinal;                   // position in the call's list (enters the hash)
     int g_bf16;
@@ -197,7 +197,8 @@ __device__ __forceinline__ void adamw_chunk(const Tensor& T, const Hyper& h, lon
             const float gs = to_f32(g[u].e[j]) * h.grad_scale;
             m[u].e[j] = b1 * m[u].e[j] + a1 * gs;
             v[u].e[j] = b2 * v[u].e[j] + a2 * gs * gs;
-            p[u].e[j] = p[u].e[j] * T.keep - step * (m[u].e[j] / (sqrtf(v[u].e[j]) * root + h.eps));
+            // (decay and step are added up before the one rounding into p: a factor 1 - decay would lose a decay below 2^-25)
+            p[u].e[j] -= fmaf(T.decay, p[u].e[j], step * (m[u].e[j] / (sqrtf(v[u].e[j]) * root + h.eps)));
             // (elements behind the tensor's end hold zero: nothing was loaded)
             const unsigned bm = __float_as_uint(m[u].e[j]) & 0x7FFFFFFFu, bv = __float_as_uint(v[u].e[j]) & 0x7FFFFFFFu;
             mm = mm > bm ? mm : bm;
@@ -329,7 +330,7 @@ extern "C" int sf_adamw_step(int count, float* const* p, const void* const* g, v
     Hyper h{beta1, beta2, eps, grad_scale, (unsigned)seed, (unsigned)(seed >> 32), 0};
     auto fill = [&](Tensor& t, int i) {
         t = Tensor{p[i], g[i], m[i], v[i], state_bits == 8 ? m_exp[i] : nullptr, state_bits == 8 ? v_exp[i] : nullptr,
-                   shadow_bf16 ? (bf16*)shadow_bf16[i] : nullptr, n[i], (float)lr[i], (float)(1.0 - lr[i] * weight_decay[i]),
+                   shadow_bf16 ? (bf16*)shadow_bf16[i] : nullptr, n[i], (float)lr[i], (float)(lr[i] * weight_decay[i]),
                    step_offset ? step_offset[i] : 0, i, g_dtype[i] == SF_BF16, 0};
     };
     auto launch = [&](const Table& tab, int used, int groups) {

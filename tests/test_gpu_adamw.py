@@ -579,3 +579,27 @@ def test_derived_copies_go_stale_for_an_iterator():
     assert sf.ops.shadow_if_current(lin.weight) is None
     assert torch.equal(sf.ops.weight_shadow(lin.weight), lin.weight.detach().bfloat16())
     assert not torch.equal(shadow, lin.weight.detach().bfloat16())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("decay", [1e-6, 2e-7, 1e-7, 2e-8])
+def test_small_decay_counts(decay, bits):
+    """lr * weight_decay far below a step of f32 at one still takes part in the sum that is rounded into p.  Of the new value only that
+    last rounding is of the size of p: half a step of f32, 2^-24 in [1, 2) and less below one, 2^-23 where it ends above
+    two.  Everything before is of the size of the change, |step| <= lr: 16 u of it (the module's docstring), u of the decay's rounding
+    and u of the sum's, 18 u (lr + 2 decay) together.  (A factor 1 - lr * weight_decay, rounded to f32, is off by up to 2^-25 of the
+    value and its product by half a step more.)"""
+    sf = load_pkg()
+    n, lr = 1 << 20, 1e-3
+    gen = torch.Generator().manual_seed(6)
+    p0 = 1 + torch.rand(n, generator=gen)
+    g = torch.randn(n, generator=gen)
+    p = p0.cuda()
+    m, v = ([torch.zeros(n, device="cuda")] if bits == 32 else
+            [(torch.zeros(n, dtype=torch.uint8, device="cuda"), torch.zeros(n // BLOCK, dtype=torch.uint8, device="cuda"))] for _ in range(2))
+    sf.functional.adamw_step([p], [g.cuda()], m, v, torch.zeros(2, dtype=torch.int32, device="cuda"), lr, weight_decay=decay / lr)
+    z = torch.zeros(n)
+    want = oracle(p0, g, z, z, 1, lr, 0.9, 0.999, 1e-8, decay / lr)[0]
+    half = torch.exp2(torch.floor(torch.log2(want + 2.0 ** -22)) - 24)
+    check(p, want, half + 18 * U * (lr + 2 * decay), "p")
