@@ -228,6 +228,7 @@ class AdamW:
             if p.dtype != torch.float32 or not p.is_contiguous():
                 raise TypeError("AdamW: parameters are contiguous f32 tensors (the bf16 kernels read copies of them)")
         self.betas, self.eps, self.state_bits, self.seed = tuple(betas), eps, state_bits, int(seed)
+        self._check_groups()
         dev = self.params[0].device
         self.state = torch.zeros(2, device=dev, dtype=torch.int32)
         self.exp_avg, self.exp_avg_sq = ([_new_moment(p.numel(), dev, state_bits) for p in self.params] for _ in range(2))
@@ -243,8 +244,18 @@ class AdamW:
     def skipped(self) -> int:
         return int(self.state[1].item())
 
+    def _check_groups(self):
+        """A group has its own lr and weight_decay; the rest of the update is the same for all of them."""
+        for g in self.param_groups:
+            for k, own in (("betas", self.betas), ("eps", self.eps), ("amsgrad", False), ("maximize", False)):
+                v = g.get(k, own)
+                if (tuple(v) if k == "betas" else v) != own:
+                    raise ValueError(f"AdamW: {k} = {v} in a parameter group, but {own} for all of them (a group has its own lr and "
+                                     "weight_decay only)")
+
     @torch.no_grad()
     def step(self, grad_scale: float = 1.0, found_inf: Optional[torch.Tensor] = None):
+        self._check_groups()
         lrs = [g["lr"] for g in self.param_groups for _ in g["params"]]
         wds = [g["weight_decay"] for g in self.param_groups for _ in g["params"]]
         live = [i for i, p in enumerate(self.params) if p.grad is not None]

@@ -603,3 +603,19 @@ def test_small_decay_counts(decay, bits):
     want = oracle(p0, g, z, z, 1, lr, 0.9, 0.999, 1e-8, decay / lr)[0]
     half = torch.exp2(torch.floor(torch.log2(want + 2.0 ** -22)) - 24)
     check(p, want, half + 18 * U * (lr + 2 * decay), "p")
+
+
+def test_group_options_that_are_not_per_group():
+    """betas and eps are those of the optimiser: a group that brings others is turned away, not ignored; so are torch's variants
+    of the update.  Equal values, and keys that are no options, are fine."""
+    training = importlib.import_module(load_pkg().__name__ + ".training")
+    p = torch.nn.Parameter(torch.zeros(4))
+    for extra in ({"betas": (0.5, 0.9)}, {"eps": 1e-6}, {"amsgrad": True}, {"maximize": True}):
+        with pytest.raises(ValueError, match=next(iter(extra))):
+            training.AdamW([{"params": [p], **extra}])
+    opt = training.AdamW([{"params": [p], "lr": 1e-2, "weight_decay": 0.0, "betas": [0.9, 0.999], "eps": 1e-8, "amsgrad": False,
+                           "maximize": False, "name": "all"}])
+    opt.param_groups[0]["betas"] = (0.5, 0.9)
+    p.grad = torch.zeros(4)
+    with pytest.raises(ValueError, match="betas"):
+        opt.step()
