@@ -179,6 +179,8 @@ class FlatAdam:
         return out
 
     def load_state_by_name(self, module: nn.Module, state: Dict):
+        if int(state.get("state_bits", 32)) != 32:          # (FlatAdamW's)
+            raise RuntimeError(f"optimiser state of {state['state_bits']} bits, the optimiser keeps 32")
         names = {id(p): n for n, p in module.named_parameters()}
         for p, (o, n) in zip(self.params, self.ranges):
             k = names[id(p)]

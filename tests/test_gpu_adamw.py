@@ -619,3 +619,12 @@ def test_group_options_that_are_not_per_group():
     p.grad = torch.zeros(4)
     with pytest.raises(ValueError, match="betas"):
         opt.step()
+
+
+def test_8_bit_state_is_not_read_as_adam():
+    """A checkpoint of 8-bit moments says so when plain Adam is asked to resume from it."""
+    training = importlib.import_module(load_pkg().__name__ + ".training")
+    net = torch.nn.Linear(4, 4)
+    opt = training.FlatAdam(net, 1e-3)
+    with pytest.raises(RuntimeError, match="8 bits"):
+        opt.load_state_by_name(net, {"t": 3, "state_bits": 8, "seed": 0, "moments": {}})
