@@ -952,7 +952,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     to begin with).  state: int32 [2] on the device, steps taken and steps skipped, zeros to begin with; a
     step whose found_inf[0] is not zero changes nothing but the second count.  lr and weight_decay: one
     number, or one per tensor.  seed: of the stochastic rounding of 8-bit moments.  shadows: bf16 copies
-    of the parameters to refresh (entries may be None).  The parameters are written behind torch's
+    of the parameters to refresh (entries may be None).  Whatever the step writes (parameters, moments, exponents, shadows) must
+    not overlap; the same tensor twice is refused.  The parameters are written behind torch's
     back (a graph that saved them before the step would read the new values): copies the package derives from
     them (packed weights, shadows) are marked stale here."""
     if not state.is_cuda:

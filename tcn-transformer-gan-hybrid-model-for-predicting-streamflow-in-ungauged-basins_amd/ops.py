@@ -1399,6 +1399,12 @@ def _moment_addresses(ms, numels, index, what):
             _flat_addresses([x[1] for x in ms], [-(-n // ADAMW_BLOCK) for n in numels], index, what + " block exponents", torch.uint8))
 
 
+def _any_twice(numels, *lists):
+    """Whether an address of what a call writes is listed twice (tensors without elements and missing ones aside)."""
+    written = [a for at in lists if at is not None for a, k in zip(at, numels) if k and a is not None]
+    return len(set(written)) != len(written)
+
+
 def _pointers(values):
     return None if values is None else (_c_vp * len(values))(*values)
 
@@ -1435,9 +1441,8 @@ def adamw_step(ps, gs, ms, vs, state, lr, beta1, beta2, eps, weight_decay, seed=
     v_at, ve_at = _moment_addresses(vs, numels, index, "adamw_step: second moment")
     if (me_at is None) != (ve_at is None):
         raise TypeError("adamw_step: f32 and 8-bit moments cannot be mixed in one call")
-    written = [a for at in (p_at, m_at, v_at) for a, k in zip(at, numels) if k]
-    if len(set(written)) != len(written):
-        raise RuntimeError("adamw_step: the same parameter or moment is listed twice")
+    if _any_twice(numels, p_at, m_at, v_at, me_at, ve_at, sh_at):
+        raise RuntimeError("adamw_step: the same parameter, moment, block exponents or shadow is listed twice")
     if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0 and eps >= 0.0):
         raise ValueError(f"adamw_step: betas ({beta1}, {beta2}) must lie in [0, 1), eps ({eps}) must not be negative")
     if step_offsets is not None and any(o > 0 for o in step_offsets):
@@ -1465,6 +1470,8 @@ def adamw_moments(ms, vs, outs_m, outs_v):
     v_at, ve_at = _moment_addresses(vs, numels, index, "adamw_moments: second moment")
     if me_at is None or ve_at is None:
         raise TypeError("adamw_moments: f32 moments are their own values")
+    if _any_twice(numels, *to):
+        raise RuntimeError("adamw_moments: the same output is listed twice")
     _check(lib().sf_adamw_moments(n, _pointers(m_at), _pointers(v_at), _pointers(me_at), _pointers(ve_at), _pointers(to[0]),
                                   _pointers(to[1]), (_c_ll * n)(*numels), _stream_of(outs_m[0])), "sf_adamw_moments")
 

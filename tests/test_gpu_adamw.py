@@ -628,3 +628,22 @@ def test_8_bit_state_is_not_read_as_adam():
     opt = training.FlatAdam(net, 1e-3)
     with pytest.raises(RuntimeError, match="8 bits"):
         opt.load_state_by_name(net, {"t": 3, "state_bits": 8, "seed": 0, "moments": {}})
+
+
+@pytest.mark.gpu
+def test_shadows_and_exponents_listed_twice_are_refused():
+    sf = load_pkg()
+    z = lambda n=300, dt=torch.float32: torch.zeros(n, dtype=dt, device="cuda")
+    byte = lambda n=300: z(n, torch.uint8)
+    state, sh, e = z(2, torch.int32), z(300, torch.bfloat16), byte(2)
+    with pytest.raises(RuntimeError, match="twice"):
+        sf.functional.adamw_step([z(), z()], [z(), z()], [z(), z()], [z(), z()], state, 1e-3, shadows=[sh, sh])
+    for ms, vs in (([(byte(), e), (byte(), e)], [(byte(), byte(2)), (byte(), byte(2))]),
+                   ([(byte(), byte(2)), (byte(), byte(2))], [(byte(), e), (byte(), e)]), ([(byte(), e)], [(byte(), e)])):
+        n = len(ms)
+        with pytest.raises(RuntimeError, match="twice"):
+            sf.functional.adamw_step([z() for _ in range(n)], [z() for _ in range(n)], ms, vs, state, 1e-3)
+    with pytest.raises(RuntimeError, match="twice"):
+        sf.functional.adamw_moments([(byte(), byte(2))] * 2, [(byte(), byte(2))] * 2, out=([sh, sh], [z(300, torch.bfloat16) for _ in range(2)]))
+    assert state.tolist() == [0, 0]
+    sf.functional.adamw_step([z(), z()], [z(), z()], [z(), z()], [z(), z()], state, 1e-3, shadows=[None, None])
