@@ -955,11 +955,15 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     of the parameters to refresh (entries may be None).  Whatever the step writes (parameters, moments, exponents, shadows) must
     not overlap; the same tensor twice is refused.  The parameters are written behind torch's
     back (a graph that saved them before the step would read the new values): copies the package derives from
-    them (packed weights, shadows) are marked stale here."""
+    them (packed weights, shadows) are marked stale here.  A captured step writes them at every replay, so such copies
+    are made anew at each use from then on; it is refused while one is current (ops.touch(params) before the capture).
+    lr, weight_decay, betas and step_offsets are those of the capture."""
     if not state.is_cuda:
         raise RuntimeError("adamw_step: GPU tensors only (no CPU path exists)")
     params = list(params)               # (an iterator is read once, and both calls below need it)
     with ops.device_guard(state):
+        if torch.cuda.is_current_stream_capturing():
+            ops.touch_by_replays(params, shadows)
         ops.adamw_step(params, list(grads), list(exp_avgs), list(exp_avg_sqs), state, lr, betas[0], betas[1], eps,
                        weight_decay, seed, found_inf, grad_scale, shadows, step_offsets)
         ops.touch(params)

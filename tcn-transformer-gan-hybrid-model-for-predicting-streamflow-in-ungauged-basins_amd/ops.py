@@ -599,18 +599,40 @@ def touch(params):
         p.__dict__["_sf_epoch"] = p.__dict__.get("_sf_epoch", 0) + 1
 
 
+def touch_by_replays(params, shadows=None):
+    """A captured optimiser step is about to write these parameters, at every replay of its graph and without a word to
+    touch(): from here on nothing derived from them is ever taken for current.  Refused while a copy is current that
+    was made outside the graph and is not refreshed by the step (`shadows`): what came before the step in the graph may
+    read it, and a replay would not make it anew."""
+    params = list(params)
+    for i, p in enumerate(params):
+        shadow = shadow_if_current(p)
+        if any(ver == _derived_key(p) for ver, _ in p.__dict__.get("_sf_derived", {}).values()) \
+                or (shadow is not None and (shadows is None or shadow is not shadows[i])):
+            raise RuntimeError(f"parameter {i} has a derived copy (packed weights, a bf16 shadow) that replays of the graph would leave "
+                               "as it is: announce a change with ops.touch(parameters) before the capture")
+    for p in params:
+        p.__dict__["_sf_replayed"] = True
+
+
+def _derived_key(p: torch.Tensor):
+    return None if p.__dict__.get("_sf_replayed") else (WEIGHT_EPOCH, p.__dict__.get("_sf_epoch", 0), p._version, p.data_ptr())
+
+
 def derived(owner: torch.Tensor, key, build):
     """A tensor computed from parameter `owner` alone (a packed / staged copy of a conv weight),
     kept on the parameter object until the parameter changes: in place through torch (its version
     counter), behind torch's back by an optimiser kernel (touch / bump_weight_epoch), or by moving
-    elsewhere."""
-    ver = (WEIGHT_EPOCH, owner.__dict__.get("_sf_epoch", 0), owner._version, owner.data_ptr())
+    elsewhere.  Not kept: what is built while a graph is captured (its memory is the graph's, its values come with
+    the replays), or from a parameter that replays change (touch_by_replays)."""
+    ver = _derived_key(owner)
     cache = owner.__dict__.setdefault("_sf_derived", {})
     hit = cache.get(key)
     if hit is not None and hit[0] == ver:
         return hit[1]
     t = build()
-    cache[key] = (ver, t)
+    if ver is not None and not torch.cuda.is_current_stream_capturing():
+        cache[key] = (ver, t)
     return t
 
 
@@ -621,6 +643,8 @@ def _shadow_key(p: torch.Tensor):
 
 
 def shadow_if_current(p: torch.Tensor) -> Optional[torch.Tensor]:
+    if p.__dict__.get("_sf_replayed"):
+        return None
     sh = getattr(p, "_sf_shadow", None)
     return sh if sh is not None and getattr(p, "_sf_shadow_key", None) == _shadow_key(p) else None
 

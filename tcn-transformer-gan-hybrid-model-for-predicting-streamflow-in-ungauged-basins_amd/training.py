@@ -342,6 +342,8 @@ class FlatAdamW(FlatAdam):
         live = [i for i, p in enumerate(self.params) if p.grad is not None]
         grads = [self._small_views[i] if i < ns else self.params[i].grad.contiguous() for i in live]
         shadows = [ops.weight_shadow(self.params[i]) if self.shadow_big and i >= ns else None for i in live]
+        if self.state.is_cuda and torch.cuda.is_current_stream_capturing():
+            ops.touch_by_replays([self.params[i] for i in live], shadows)
         SF.adamw_step([self.params[i].data for i in live], grads, [self.moment_pairs[i][0] for i in live],
                       [self.moment_pairs[i][1] for i in live], self.state, self.lr, self.betas, self.eps,
                       [self.weight_decay if self.params[i].dim() > 1 else 0.0 for i in live], self.seed, found_inf, grad_scale,

@@ -647,3 +647,43 @@ def test_shadows_and_exponents_listed_twice_are_refused():
         sf.functional.adamw_moments([(byte(), byte(2))] * 2, [(byte(), byte(2))] * 2, out=([sh, sh], [z(300, torch.bfloat16) for _ in range(2)]))
     assert state.tolist() == [0, 0]
     sf.functional.adamw_step([z(), z()], [z(), z()], [z(), z()], [z(), z()], state, 1e-3, shadows=[None, None])
+
+
+@pytest.mark.gpu
+def test_captured_step_and_derived_copies():
+    """A replay updates the parameters without a call of Python: copies derived from them (shadows, packed weights) are never
+    taken for current once a step has been captured, copies built inside a graph are the graph's own, and a step is not captured
+    while a copy from outside is current, since what came before it in the graph may read that copy at every replay."""
+    sf = load_pkg()
+    p, q = (torch.nn.Parameter(torch.randn(64, 8, device="cuda")) for _ in range(2))
+    new = lambda: [torch.zeros(64, 8, device="cuda")]
+    copy = lambda x: sf.ops.derived(x, "copy", lambda: x.detach().clone())
+    state = torch.zeros(2, dtype=torch.int32, device="cuda")
+    grads, ms, vs = [torch.ones(64, 8, device="cuda")], new(), new()
+    sf.functional.adamw_step([p], grads, ms, vs, state, 0.1)
+    copy(p)
+    sf.ops.weight_shadow(p)
+    sf.ops.touch([p])                                   # (announced: the copies from outside are stale)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = copy(p)
+        sf.functional.adamw_step([p], grads, ms, vs, state, 0.1)
+    for _ in range(3):
+        before = p.detach().clone()
+        assert torch.equal(sf.ops.weight_shadow(p), before.bfloat16()) and torch.equal(copy(p), before)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(inside, before) and not torch.equal(p.detach(), before)
+    sf.functional.adamw_step([p], grads, ms, vs, state, 0.1)
+    assert torch.equal(sf.ops.weight_shadow(p), p.detach().bfloat16()) and torch.equal(copy(p), p.detach())
+    assert state.tolist() == [5, 0]
+    more = (new(), new())
+    for make_copy in (sf.ops.weight_shadow, copy):
+        q = torch.nn.Parameter(q.detach().clone())
+        make_copy(q)
+        with pytest.raises(RuntimeError, match="derived"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                sf.functional.adamw_step([q], grads, *more, state, 0.1)
+        torch.cuda.synchronize()
+        assert state.tolist() == [5, 0] and torch.equal(make_copy(q).float(), q.detach().to(make_copy(q).dtype).float())
