@@ -265,6 +265,8 @@ class DifferentialAttention(nn.Module):
         if x.dim() != 3 or x.shape[-1] != self.embed_dim:
             raise RuntimeError(f"DifferentialAttention: [B, T, {self.embed_dim}] tokens, not {tuple(x.shape)}")
         B, T, _ = x.shape
+        if B * T == 0:                  # no token to attend from (a product of no rows is no launch)
+            return x.to(torch.float32, copy=True)
         H, kv, d, dt = self.num_heads, self.num_kv_heads, self.head_dim, SF.compute_dtype()
         qkv = SF.linear(x.reshape(B * T, self.embed_dim), self.in_proj, dt).to(dt).view(B, T, -1)
         q, k, v = torch.split(qkv, [H * 2 * d, kv * 2 * d, kv * 2 * d], dim=-1)

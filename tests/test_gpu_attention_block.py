@@ -148,3 +148,19 @@ def test_refusals():
         sf.DifferentialAttention(64, 2, 3)
     with pytest.raises(RuntimeError, match="no CPU path"):
         sf.DifferentialAttention(64, 2)(torch.zeros(1, 2, 64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("amp", [False, True])
+@pytest.mark.parametrize("shape", [(0, 5), (3, 0)])
+def test_no_tokens(shape, amp):
+    """A batch without samples and samples without tokens: an empty result, gradients of zero."""
+    sf = load_pkg()
+    m = sf.DifferentialAttention(E, H, KV).cuda()
+    x = torch.zeros(*shape, E, device="cuda", requires_grad=True)
+    with torch.autocast("cuda", dtype=torch.bfloat16, enabled=amp):
+        y = m(x, torch.zeros(shape[0], dtype=torch.int32, device="cuda"))
+    assert y.shape == x.shape and y.dtype == torch.float32
+    y.sum().backward()
+    assert x.grad.shape == x.shape
+    assert all(p.grad is None or float(p.grad.abs().sum()) == 0 for p in m.parameters())
