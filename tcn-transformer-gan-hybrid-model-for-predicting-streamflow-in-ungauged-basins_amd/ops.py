@@ -631,7 +631,7 @@ def derived(owner: torch.Tensor, key, build):
     if hit is not None and hit[0] == ver:
         return hit[1]
     t = build()
-    if ver is not None and not torch.cuda.is_current_stream_capturing():
+    if ver is not None and not (owner.is_cuda and torch.cuda.is_current_stream_capturing()):
         cache[key] = (ver, t)
     return t
 

@@ -687,3 +687,13 @@ def test_captured_step_and_derived_copies():
                 sf.functional.adamw_step([q], grads, *more, state, 0.1)
         torch.cuda.synchronize()
         assert state.tolist() == [5, 0] and torch.equal(make_copy(q).float(), q.detach().to(make_copy(q).dtype).float())
+
+
+def test_copies_of_host_parameters_are_kept():
+    """Without a GPU the cache of derived copies asks no stream."""
+    ops = load_pkg().ops
+    p = torch.nn.Parameter(torch.zeros(4))
+    first = ops.derived(p, "copy", lambda: p.detach().clone())
+    assert ops.derived(p, "copy", lambda: p.detach().clone()) is first
+    ops.touch([p])
+    assert ops.derived(p, "copy", lambda: p.detach().clone()) is not first
