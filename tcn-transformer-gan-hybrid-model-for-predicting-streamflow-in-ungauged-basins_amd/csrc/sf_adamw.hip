@@ -22,6 +22,7 @@
 // 1.91 GB, 5.3 TB/s; bf16 gradients and 8-bit moments 196 us, 0.96 GB, 4.9 TB/s, and their values as bf16 (adamw_moments) 82 us,
 // 0.41 GB, 5.0 TB/s.  16 tensors with 2.8 M elements: 13 us, and the launch around it costs the host more.
 #include "sf_common.h"
+#include <float.h>
 #include "../../include/sfhip.h"
 
 namespace {
@@ -197,8 +198,10 @@ __device__ __forceinline__ void adamw_chunk(const Tensor& T, const Hyper& h, lon
             const float gs = to_f32(g[u].e[j]) * h.grad_scale;
             m[u].e[j] = b1 * m[u].e[j] + a1 * gs;
             v[u].e[j] = b2 * v[u].e[j] + a2 * gs * gs;
-            // (decay and step are added up before the one rounding into p: a factor 1 - decay would lose a decay below 2^-25)
-            p[u].e[j] -= fmaf(T.decay, p[u].e[j], step * (m[u].e[j] / (sqrtf(v[u].e[j]) * root + h.eps)));
+            // (decay and step are added up before the one rounding into p: a factor 1 - decay would lose a decay below 2^-25.  The
+            // product takes the largest finite value for an infinite one, which stays infinite so.)
+            const float finite = fminf(fmaxf(p[u].e[j], -FLT_MAX), FLT_MAX);
+            p[u].e[j] -= fmaf(T.decay, finite, step * (m[u].e[j] / (sqrtf(v[u].e[j]) * root + h.eps)));
             // (elements behind the tensor's end hold zero: nothing was loaded)
             const unsigned bm = __float_as_uint(m[u].e[j]) & 0x7FFFFFFFu, bv = __float_as_uint(v[u].e[j]) & 0x7FFFFFFFu;
             mm = mm > bm ? mm : bm;

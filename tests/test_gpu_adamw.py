@@ -697,3 +697,18 @@ def test_copies_of_host_parameters_are_kept():
     assert ops.derived(p, "copy", lambda: p.detach().clone()) is first
     ops.touch([p])
     assert ops.derived(p, "copy", lambda: p.detach().clone()) is not first
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("wd", [0.0, 0.1])
+def test_infinite_parameters_stay(bits, wd):
+    """A parameter that holds infinities (a learned mask) keeps them, as p (1 - lr wd) - step does; its other values step."""
+    sf = load_pkg()
+    p = torch.tensor([1.0, float("inf"), -2.0, float("-inf")], device="cuda")
+    m, v = ([torch.zeros(4, device="cuda")] if bits == 32 else
+            [(torch.zeros(4, dtype=torch.uint8, device="cuda"), torch.zeros(1, dtype=torch.uint8, device="cuda"))] for _ in range(2))
+    g = torch.tensor([1.0, 0.0, 1.0, 0.5], device="cuda")
+    sf.functional.adamw_step([p], [g], m, v, torch.zeros(2, dtype=torch.int32, device="cuda"), 1e-2, weight_decay=wd)
+    assert p[1] == float("inf") and p[3] == float("-inf")
+    assert bool(torch.isfinite(p[::2]).all()) and float(p[0]) < 1.0 and float(p[2]) < -1.99
