@@ -56,9 +56,12 @@ template <int G> __device__ __forceinline__ float row_sum(float v, float* sm) {
 
 // the same of two values at once (sm: 8 floats)
 template <int G> __device__ __forceinline__ void row_sums(float& a, float& b, float* sm) {
+#pragma unroll
+    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) {
+        a += __shfl_xor(a, o, 64);
+        b += __shfl_xor(b, o, 64);
+    }
     if constexpr (G == NT) {
-        a = wave_sum(a);
-        b = wave_sum(b);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) {
             sm[threadIdx.x >> 6] = a;
@@ -67,12 +70,6 @@ template <int G> __device__ __forceinline__ void row_sums(float& a, float& b, fl
         __syncthreads();
         a = sm[0] + sm[1] + sm[2] + sm[3];
         b = sm[4] + sm[5] + sm[6] + sm[7];
-    } else {
-#pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) {
-            a += __shfl_xor(a, o, 64);
-            b += __shfl_xor(b, o, 64);
-        }
     }
 }
 
