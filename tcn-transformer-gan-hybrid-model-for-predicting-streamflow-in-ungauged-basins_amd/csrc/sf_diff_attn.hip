@@ -767,21 +767,26 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
                 s[i] = mma(L::row_piece(kt, rl, sub, i * KS + n), qf[i][n], s[i]);
 #pragma unroll
         for (int n = 0; n < VS; ++n) dp = mma(L::row_piece(vt, rl, sub, n), gf[n], dp);
-        if (key0 + 32 > vmin) {
+        if ((key0 + 32 > vmin) | wide) {        // (one branch: the usual tile takes none)
+            if (key0 + 32 > vmin) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const bool see = key0 + acc_row(r, h2) < vis;
-                s[0][r] = see ? s[0][r] : -INFINITY;
-                s[1][r] = see ? s[1][r] : -INFINITY;
+                for (int r = 0; r < 16; ++r) {
+                    const bool see = key0 + acc_row(r, h2) < vis;
+                    s[0][r] = see ? s[0][r] : -INFINITY;
+                    s[1][r] = see ? s[1][r] : -INFINITY;
+                }
+            }
+            if (wide) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[0][r] -= ref[0];
+                    s[1][r] -= ref[1];
+                }
             }
         }
         Frag<T> df[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (wide) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] -= ref[i];
-            }
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -973,16 +978,18 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<
             const typename L::Lane ql = fresh(rl, L::row_off(rows0));
 #pragma unroll
             for (int n = 0; n < KS; ++n) s = mma(L::row_piece(cur, ql, 0, i * KS + n), kf[i][n], s);
-            if (edge) {
+            if (edge | wide) {              // (one branch: the usual tile takes none)
+                if (edge) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = t0 + acc_row(r, h2) >= t_min ? s[r] : -INFINITY;
-            }
-            if (wide) {
+                    for (int r = 0; r < 16; ++r) s[r] = t0 + acc_row(r, h2) >= t_min ? s[r] : -INFINITY;
+                }
+                if (wide) {
 #pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const f32x4 ref = *(const SF_LDS f32x4*)(stat + (4 + 2 * i) * QT + acc_row(r, h2));
+                    for (int r = 0; r < 16; r += 4) {
+                        const f32x4 ref = *(const SF_LDS f32x4*)(stat + (4 + 2 * i) * QT + acc_row(r, h2));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[r + e] -= ref[e];
+                        for (int e = 0; e < 4; ++e) s[r + e] -= ref[e];
+                    }
                 }
             }
             Frag<T> df[2];
