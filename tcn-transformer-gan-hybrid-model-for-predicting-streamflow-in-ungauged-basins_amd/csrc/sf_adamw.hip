@@ -1,6 +1,6 @@
 // AdamW over many tensors in one launch, moments held in f32 or in 8 bits.
 //
-//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p - (lr wd p + lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps))
 //
 // Bound by HBM: 28 bytes per element with f32 gradients and moments, 16 with 8-bit moments, each touched
 // once.  The tensors' pointers travel as kernel arguments (no table in device memory to fill, so a launch
@@ -16,10 +16,10 @@
 // code per step (the second by a thousandth of its value), so rounding to nearest would hold it in place
 // for ever: codes are rounded stochastically, with 16 bits of an integer hash of (seed, step, tensor,
 // element), which keeps the moments unbiased and a run reproducible.  A second moment is never rounded to
-// zero (its square root divides).  The update of p uses the moments before they are rounded.
+// zero (its square root divides): one below the smallest code, 2^-31 of the block's largest, is raised to it.  The update of p uses the moments before they are rounded.
 //
 // Measured on 68.3 M elements in 40 tensors (a copy of 1 GiB runs at 5.05 TB/s on the same card): f32 gradients and moments 360 us,
-// 1.91 GB, 5.3 TB/s; bf16 gradients and 8-bit moments 196 us, 0.96 GB, 4.9 TB/s, and their values as bf16 (adamw_moments) 82 us,
+// 1.91 GB, 5.3 TB/s; bf16 gradients and 8-bit moments 202 us, 0.96 GB, 4.7 TB/s, and their values as bf16 (adamw_moments) 82 us,
 // 0.41 GB, 5.0 TB/s.  16 tensors with 2.8 M elements: 13 us, and the launch around it costs the host more.
 #include "sf_common.h"
 #include <float.h>

@@ -316,10 +316,10 @@ template <typename T, int DP> __device__ __forceinline__ void store_cols(T* row,
 // ------------------------------------------------------------------------------ forward
 // The query rows of all the heads that share a key/value head are one list, row r = token r / group, head r % group:
 // one copy of the keys serves the whole group.  KEYS_SPLIT false: wave w takes rows 32 w .. of the workgroup's 128 and
-// all keys of the tile.  KEYS_SPLIT true (at most 32 rows, single tokens): all waves take the same 32 rows and wave w
-// the keys 32 w .. of the tile; the waves' results are joined through LDS at the end.
+// all keys of the tile.  KEYS_SPLIT true (single tokens, and wherever row_plan finds the wider items too few): all waves take the
+// same 32 rows and wave w the keys 32 w .. of the tile; the waves' results are joined through LDS at the end.
 // Measured, bf16 heads of 2 x 64: 8 heads, 2 x 5120 tokens: 340 to 375 us, 322 GFLOP, 0.9 PFLOP/s (a library product reaches 1.28);
-// the matrix pipe is busy 48 % of the time and the vector unit (32 exponentials a lane and tile of 32 x 32) nearly as long, hardly
+// the matrix pipe is busy 47 % of the time and the vector unit (32 exponentials a lane and tile of 32 x 32) nearly as long, hardly
 // at the same time, at a clock that power holds at 1.75 GHz.  1 x 8191 tokens, causal: 262 to 280 us, 206 GFLOP.  Single tokens,
 // 16 samples, 4 key heads, 8192 keys: 30 us, 134 MB, 4.4 TB/s, bound by HBM.
 // (narrow heads: four waves per SIMD, as many as slots_of counts on)
@@ -868,7 +868,7 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dq_kernel(Args<T
 // under way.  So a lane keeps two address registers for its row pieces and two for its column pieces and makes the
 // others where it uses them (fresh), and the maps come one after the other: no spill in the loop (2 x 5120 tokens, 8 heads:
 // 725 us with 13 spills, 592 us without; eight waves in pairs, with the keys in LDS too, 635 us).  540 to 600 us now, 429 GFLOP,
-// 0.75 PFLOP/s: the matrix pipe is busy 40 % of the time, LDS reads 35 %, and no registers are left to fetch operands ahead.
+// 0.75 PFLOP/s: the matrix pipe is busy 37 % of the time, LDS reads 33 %, and no registers are left to fetch operands ahead.
 template <typename T, int DP, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<T> a) {
     using L = Tile<T, DP>;
@@ -884,7 +884,7 @@ __global__ __launch_bounds__(64 * NW, (WAVES<T, DP>)) void attn_dkv_kernel(Args<
     int bh, x;
     locate(w.item, a.B * a.Hk, tiles, a.causal, bh, x);
     const int b = bh / a.Hk, hk = bh % a.Hk, k0 = x * KB;
-        const int kw = SPLIT ? 0 : wave * 32, rows0 = SPLIT ? wave * 32 : 0;       // the wave's keys, and its rows of a tile
+    const int kw = SPLIT ? 0 : wave * 32, rows0 = SPLIT ? wave * 32 : 0;       // the wave's keys, and its rows of a tile
     const int key = k0 + kw + (lane & 31);
     const int kend = keys_of(a, b), reach = a.Tk - a.Tq;
     const int t_min = key >= kend ? 1 << 30 : a.causal ? key - reach : 0;  // the key is seen by queries from t_min on

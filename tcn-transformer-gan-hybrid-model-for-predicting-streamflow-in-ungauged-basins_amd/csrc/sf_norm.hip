@@ -18,7 +18,7 @@
 //
 // Measured (a copy of 1 GiB runs at 5.05 TB/s on the same card):
 //   163840 x 256 bf16, residual, no statistics kept: 58 us, 335 MB, 5.8 TB/s
-//   16384 x 4096 bf16, residual: forward 102 us, 537 MB, 5.3 TB/s; backward 108 us, 537 MB, 5.0 TB/s, and 4 us for the fold
+//   16384 x 4096 bf16, residual: forward 106 us, 537 MB, 5.1 TB/s; backward 108 us, 537 MB, 5.0 TB/s, and 4 us for the fold
 //   30011 x 999 f32: forward 41 us, 240 MB, 5.9 TB/s; backward 71 us, 360 MB, 5.0 TB/s, and 5 us for the fold
 //   160 x 128 bf16: 4, 6 and 3 us, all of it launch and latency
 #include "sf_common.h"

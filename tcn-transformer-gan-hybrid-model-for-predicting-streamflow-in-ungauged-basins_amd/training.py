@@ -208,8 +208,10 @@ class AdamW:
     state_bits 32 keeps f32 moments; 8 keeps one byte per element and moment plus a byte per 256 elements
     (a quarter of the memory, 16 instead of 28 bytes of traffic per element and step), rounded
     stochastically from `seed`, so a run repeats exactly.  As in torch.optim.AdamW a parameter without a
-    gradient is left alone and its own step count stands still.  step(found_inf) with a device flag skips
-    the step on the device when the flag is set (see FlatAdam)."""
+    gradient is left alone and its own step count stands still (but for a call that is both skipped and missed by the parameter,
+    as in FlatAdam: the skip, known to the device alone, is then taken off its count).  step(found_inf) with a device flag skips
+    the step on the device when the flag is set (see FlatAdam).  betas and eps are the same for all groups.  A captured step
+    keeps the lr and weight_decay of its capture."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32, seed: int = 0):
