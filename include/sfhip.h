@@ -30,6 +30,7 @@ extern "C" {
 #define SF_OUT_IJ 2   /* out[i*ldo + j] */
 #define SF_OUT_OIHW 3 /* conv weight gradient, f32 OIHW [ldo][cin_real][RS], j = tap*C + c; rows i >= ldo dropped */
 
+/* 2: what sf_diff_attn_fwd keeps for the backward pass is twice as long (sums [B,H,Tq,2,2] in place of lse [B,H,Tq,2]) */
 int sf_version(void);
 const char* sf_last_error(void);
 

@@ -13,4 +13,4 @@ void sf_set_error(const char* fmt, ...) {
 }
 
 extern "C" const char* sf_last_error(void) { return g_err; }
-extern "C" int sf_version(void) { return 1; }
+extern "C" int sf_version(void) { return 2; }
