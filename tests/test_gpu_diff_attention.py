@@ -708,3 +708,40 @@ def test_plans_of_many_items():
             cut["fwd"] += int(L.sf_diff_attn_fwd_workspace_bytes(ctypes.byref(desc))) > 0
             cut["bwd"] += int(L.sf_diff_attn_bwd_workspace_bytes(ctypes.byref(desc))) > least
     assert cut["fwd"] >= 8 and cut["bwd"] >= 16, cut
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("scale", [2e-38, 1e-30, 1e-6, 1e4, 1e12, 1e25])
+def test_any_scale(scale, dtype):
+    """The smallest scales leave all probabilities equal, the largest decide every row by one key; rows without a key among the others (more
+    queries than keys, causal; an empty sample).  Scores are sums of 8 products of values of order one: two keys of a row
+    whose scores differ by less than the rounding of these sums, 2^-21 or so, would be told apart in 64 bits alone; values of
+    few bits make the scores exact instead.  Bounds as in the module's docstring, exponents being differences of scores times
+    the scale (2^-23 of themselves)."""
+    sf = load_pkg()
+    for B, Tq, Tk, H, Hk in ((2, 150, 70, 2, 1), (2, 40, 300, 4, 2), (2, 1, 3000, 2, 2)):
+        q, k, v, lam, do = make(B, Tq, Tk, H, Hk, 8, F, seed=31)
+        q, k = (torch.round(t * 4) / 4 for t in (q, k))
+        lengths = torch.tensor([Tk, 0], dtype=torch.int32, device="cuda")
+        for ln in (None, lengths):
+            xs = [t.to(dtype) for t in (q, k, v)]
+            o, g = run(sf, *xs, lam, do.to(dtype), causal=True, lengths=ln, scale=scale)
+            want, mag = oracle_on_gpu(*xs, lam, True, ln, scale, do.to(dtype))
+            for n, x in {"o": o, **g}.items():
+                err, lim = (x.detach().double() - want[n]).abs(), bound(want[n], mag[n], dtype) + 1e-30
+                assert bool((err <= lim).all()), (n, float((err / lim).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_rows_without_keys_beside_far_ones(dtype):
+    """Queries that see no key share waves with queries whose scores are of the order of 2^33."""
+    sf = load_pkg()
+    for d in (8, 64):
+        q, k, v, lam, do = make(2, 150, 70, 2, 1, d, F, seed=33)
+        q.zero_()
+        k.zero_()
+        q[..., 0], k[..., 0] = 1.5 * 2.0 ** 16, 1.5 * 2.0 ** 17
+        q[..., 1], k[..., 1] = 1.0, -2048.0 * torch.randint(0, 3, k.shape[:-1], generator=torch.Generator().manual_seed(1))
+        within_terms(sf, *(t.to(dtype) for t in (q, k, v)), lam, do.to(dtype), True, torch.tensor([70, 33], dtype=torch.int32, device="cuda"))
